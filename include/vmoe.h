@@ -310,6 +310,39 @@ int vmoe_permute_noalloc(const int32_t* topk_ids, const float* topk_weights,
                          int32_t* pair_slot, int32_t* gather_idx, float* scatter_weights,
                          void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Token rows sorted by expert and back, outside the fused layer: for experts of any kind that work on rows of bf16 /
+ * fp16 / f32, in serving and in training.  The tables are three plain arrays instead of a workspace:
+ *   expert_offsets [E + 1]  rows of expert e are expert_offsets[e] .. expert_offsets[e + 1] - 1
+ *   row_of_pair [M, T]      row of each (token, choice) pair, -1 = dropped
+ *   pair_of_row [M * T]     pair (token * T + choice) of each row, -1 behind the last kept row
+ * Kept pairs are those whose id (through expert_map [map_len] when given) lies in [0, E); all others, ids outside the
+ * map included, are dropped.  Rows are ordered by (expert, pair); a token may name an expert more than once.  The
+ * tables are what build_group_tables (fused-moe/csrc/verdict_fused_grouped.cu:655-691) makes for FP4 rows.
+ * Limits: T <= 16, E <= 8192, M * T < 2^31 - 1024 (VMOE_ERR_LIMIT).  Strides are in elements. */
+enum vmoe_dtype { VMOE_BF16 = 0, VMOE_F16 = 1, VMOE_F32 = 2 };
+
+int vmoe_plan_tokens(const int32_t* topk_ids, const int32_t* expert_map, int32_t map_len, int32_t M, int32_t T, int32_t E,
+                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* stream);
+
+/* rows[r] = x[pair_of_row[r] / T] for every kept row; zero_tail != 0: the rows behind them, up to M * T, become zero
+ * (otherwise they are left as they were). */
+int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K,
+                     const int32_t* expert_offsets, const int32_t* row_of_pair, int32_t zero_tail, void* rows, int64_t rows_stride,
+                     void* stream);
+
+/* out[m] = sum_t weights[m, t] * rows[row_of_pair[m, t]] over the kept pairs, t ascending, f32, rounded once (0 without
+ * a kept pair).  weights [M, T] f32, NULL = all 1, which is the gradient of vmoe_sort_tokens. */
+int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int32_t M, int32_t T, int32_t K,
+                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, void* stream);
+
+/* Gradient of vmoe_unsort_tokens: drows[r] = weights * dout[token] (rows behind the last kept one: 0) and
+ * dweights[m, t] = <rows[r], dout[m]> in f32 (dropped pairs: 0).  Either output may be NULL; rows may be NULL when
+ * dweights is. */
+int vmoe_unsort_tokens_grad(const void* dout, int64_t dout_stride, const void* rows, int64_t rows_stride, int32_t dtype, int32_t M,
+                            int32_t T, int32_t E, int32_t K, const int32_t* expert_offsets, const int32_t* row_of_pair,
+                            const float* weights, void* drows, int64_t drows_stride, float* dweights, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,432 @@
+// Token rows sorted by expert and back, for rows of bf16 / fp16 / f32, with the gradients of both directions.
+//
+//   plan    pairs p = m * T + t with a local expert, ordered by (expert, p):  offsets, row_of_pair, pair_of_row
+//   sort    rows[r] = x[pair_of_row[r] / T]
+//   unsort  y[m]    = sum_t w[m, t] * rows[row_of_pair[m, t]]          (w = 1: the gradient of sort)
+//   grad    drows[row_of_pair[m, t]] = w[m, t] * dy[m],   dw[m, t] = <rows[row_of_pair[m, t]], dy[m]>
+//
+// Unlike the tables inside the layer's workspace (vmoe_phases.cuh: one bit per expert and token) a token may name an
+// expert twice here; each pair has its own row.  All sums run over t in ascending order in f32 and are rounded once;
+// nothing is summed with atomics, so every result is reproducible bit for bit.
+#include "vmoe_common.cuh"
+#include "vmoe_rows.cuh"
+
+namespace vmoe {
+
+// ---------------------------------------------------------------------------------
+// Plan: a stable counting sort by one CTA, or by one cluster of eight CTAs whose totals meet in distributed shared
+// memory -- one launch at every size, no global scratch.  Each warp owns a contiguous run of pairs.  Pass 1 counts
+// them per expert into the warp's own row of counters; sums over warps, CTAs and experts turn the counters into the
+// first row of (expert, warp); pass 2 walks the run again, 32 pairs at a time: __match_any_sync gives a pair's rank
+// among the lanes with its expert.
+// ---------------------------------------------------------------------------------
+constexpr int PLAN_MAX_EXPERTS = 8192;
+constexpr int PLAN_CLUSTER = 8;
+constexpr int PLAN_ONE_CTA_PAIRS = 4096;
+constexpr int PLAN_SMEM = 200 * 1024;
+
+__device__ __forceinline__ uint32_t plan_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void plan_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int plan_peer_word(const int* p, uint32_t rank) {
+    uint32_t a;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ int plan_expert(const int32_t* ids, const int32_t* expert_map, int map_len, int E, long long p, long long end) {
+    if (p >= end) return -1;
+    int e = ids[p];
+    if (expert_map) e = (e >= 0 && e < map_len) ? expert_map[e] : -1;
+    return (e >= 0 && e < E) ? e : -1;
+}
+
+template <int CTAS>
+__global__ void __launch_bounds__(1024)
+plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ expert_map, int map_len, int P, int E, int run,
+            int32_t* __restrict__ offsets, int32_t* __restrict__ row_of_pair, int32_t* __restrict__ pair_of_row) {
+    extern __shared__ int s_plan[];
+    __shared__ int s_warp[33];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
+    int* count = s_plan;                      // [warps][E]
+    int* total = count + (size_t)warps * E;   // [E] pairs of this CTA (read by the other CTAs)
+    int* start = total + E;                   // [E] all CTAs' pairs, then the first row of this CTA's pairs
+    int* before = start + E;                  // [E] pairs of the CTAs in front
+    const int rank = CTAS > 1 ? (int)plan_cluster_rank() : 0;
+    for (int i = tid; i < warps * E; i += threads) count[i] = 0;
+    __syncthreads();
+    pdl_begin();
+
+    int* mine = count + (size_t)warp * E;
+    const long long first = ((long long)rank * warps + warp) * run;
+    const long long end = min(first + run, (long long)P);
+    {
+        int e = plan_expert(ids, expert_map, map_len, E, first + lane, end);
+        for (long long b = first; b < end; b += 32) {
+            const int next = plan_expert(ids, expert_map, map_len, E, b + 32 + lane, end);
+            if (e >= 0) atomicAdd(&mine[e], 1);
+            e = next;
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < E; e += threads) {
+        int n = 0;
+        for (int w = 0; w < warps; ++w) n += count[(size_t)w * E + e];
+        total[e] = n;
+    }
+    if (CTAS > 1) plan_cluster_sync(); else __syncthreads();
+    for (int e = tid; e < E; e += threads) {
+        int all = 0, front = 0;
+#pragma unroll
+        for (int r = 0; r < CTAS; ++r) {
+            const int n = CTAS > 1 ? plan_peer_word(&total[e], r) : total[e];
+            all += n;
+            if (r < rank) front += n;
+        }
+        start[e] = all;
+        before[e] = front;
+    }
+    __syncthreads();
+    if (CTAS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // done with the others' memory
+    // exclusive prefix over the experts: every thread a contiguous run of them
+    const int per = (E + threads - 1) / threads;
+    int sum = 0;
+    for (int k = 0; k < per; ++k) { const int e = tid * per + k; if (e < E) sum += start[e]; }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += v; }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        const int v = lane < warps ? s_warp[lane] : 0;
+        int in = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, in, o); if (lane >= o) in += u; }
+        s_warp[lane] = in - v;
+        if (lane == 31) s_warp[32] = in;
+    }
+    __syncthreads();
+    int at = s_warp[warp] + incl - sum;
+    for (int k = 0; k < per; ++k) {
+        const int e = tid * per + k;
+        if (e < E) {
+            const int n = start[e];
+            if (rank == 0) offsets[e] = at;
+            start[e] = at + before[e];
+            at += n;
+        }
+    }
+    const int kept = s_warp[32];
+    if (rank == 0 && tid == 0) offsets[E] = kept;
+    __syncthreads();
+    for (int e = tid; e < E; e += threads) {
+        int row = start[e];
+        for (int w = 0; w < warps; ++w) { const int n = count[(size_t)w * E + e]; count[(size_t)w * E + e] = row; row += n; }
+    }
+    __syncthreads();
+    {
+        int e = plan_expert(ids, expert_map, map_len, E, first + lane, end);
+        for (long long b = first; b < end; b += 32) {
+            const int next = plan_expert(ids, expert_map, map_len, E, b + 32 + lane, end);
+            const uint32_t same = __match_any_sync(0xffffffffu, e);
+            const int rank_in = __popc(same & ((1u << lane) - 1));
+            const int row = e >= 0 ? mine[e] + rank_in : -1;
+            __syncwarp();
+            if (e >= 0 && rank_in == 0) mine[e] += __popc(same);
+            __syncwarp();
+            if (b + lane < end) {
+                row_of_pair[b + lane] = row;
+                if (row >= 0) pair_of_row[row] = (int)(b + lane);
+            }
+            e = next;
+        }
+    }
+    for (long long r = (long long)kept + rank * threads + tid; r < P; r += CTAS * threads) pair_of_row[r] = -1;
+    if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // nobody leaves while its totals are read
+}
+
+// ---------------------------------------------------------------------------------
+// Sort: a thread reads one vector of one token and stores it to the token's T rows, so a token is read once and the
+// rest of the traffic is the rows' own writes.  Rows nobody owns (dropped pairs leave them behind the last kept row)
+// are zeroed when the caller wants every row defined.
+// ---------------------------------------------------------------------------------
+template <typename V>
+__global__ void __launch_bounds__(256)
+sort_kernel(const uint8_t* __restrict__ x, long long x_stride, uint8_t* __restrict__ rows, long long rows_stride, long long vecs,
+            int M, int T, const int32_t* __restrict__ row_of_pair, const int32_t* __restrict__ kept, int zero_tail) {
+    pdl_begin();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)M * vecs;
+    if (i >= all) return;
+    const long long m = i / vecs, c = i - m * vecs;
+    const V v = reinterpret_cast<const V*>(x + m * x_stride)[c];
+    const int32_t* rp = row_of_pair + m * T;
+    for (int t = 0; t < T; ++t) {
+        const int r = rp[t];
+        if (r >= 0) reinterpret_cast<V*>(rows + r * rows_stride)[c] = v;
+    }
+    if (zero_tail)
+        for (long long j = (long long)*kept * vecs + i; j < all * T; j += all)
+            reinterpret_cast<V*>(rows + (j / vecs) * rows_stride)[j % vecs] = V{};
+}
+
+// ---------------------------------------------------------------------------------
+// Unsort: a thread owns one vector of one token and sums it over the token's pairs in order; four rows are requested
+// at a time.
+// ---------------------------------------------------------------------------------
+constexpr int UNSORT_BATCH = 4;
+
+template <typename T_, int VB>
+__global__ void __launch_bounds__(256)
+unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* __restrict__ out, long long out_stride, long long vecs,
+              int M, int T, const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights) {
+    using R = RowVec<T_, VB>;
+    pdl_begin();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)M * vecs) return;
+    const long long m = i / vecs, c = i - m * vecs;
+    float acc[R::N];
+#pragma unroll
+    for (int k = 0; k < R::N; ++k) acc[k] = 0.f;
+    const int32_t* rp = row_of_pair + m * T;
+    for (int t0 = 0; t0 < T; t0 += UNSORT_BATCH) {
+        R v[UNSORT_BATCH];
+        int r[UNSORT_BATCH];
+#pragma unroll
+        for (int j = 0; j < UNSORT_BATCH; ++j) {
+            r[j] = t0 + j < T ? rp[t0 + j] : -1;
+            if (r[j] >= 0) v[j].load(rows + r[j] * rows_stride, c);
+        }
+#pragma unroll
+        for (int j = 0; j < UNSORT_BATCH; ++j)
+            if (r[j] >= 0) {
+                const float w = weights ? weights[m * T + t0 + j] : 1.f;
+#pragma unroll
+                for (int k = 0; k < R::N; ++k) acc[k] = fmaf(w, v[j].get(k), acc[k]);
+            }
+    }
+    R o;
+#pragma unroll
+    for (int k = 0; k < R::N; ++k) o.set(k, acc[k]);
+    o.store(out + m * out_stride, c);
+}
+
+// ---------------------------------------------------------------------------------
+// Gradient of unsort: WPT warps per token, eight warps per CTA.  Four pairs at a time: their rows are read for the
+// dot products with dy[m] and their gradients written in the same pass.  Order of a dot product: a thread's vectors
+// in ascending order, the warp's xor tree, the warps in order.
+// ---------------------------------------------------------------------------------
+template <typename T_, int VB, int WPT>
+__global__ void __launch_bounds__(256)
+unsort_grad_kernel(const uint8_t* __restrict__ dy, long long dy_stride, const uint8_t* __restrict__ rows, long long rows_stride,
+                   uint8_t* __restrict__ drows, long long drows_stride, float* __restrict__ dw, int vecs, int M, int T,
+                   const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights, const int32_t* __restrict__ kept) {
+    using R = RowVec<T_, VB>;
+    __shared__ float s_dot[8][MAX_TOPK];
+    pdl_begin();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long m = (long long)blockIdx.x * (8 / WPT) + warp / WPT;
+    const int part = (warp % WPT) * 32 + lane;
+    if (m < M) {
+        const int32_t* rp = row_of_pair + m * T;
+        for (int t0 = 0; t0 < T; t0 += UNSORT_BATCH) {
+            int r[UNSORT_BATCH];
+            float w[UNSORT_BATCH], dot[UNSORT_BATCH];
+#pragma unroll
+            for (int j = 0; j < UNSORT_BATCH; ++j) {
+                r[j] = t0 + j < T ? rp[t0 + j] : -1;
+                w[j] = r[j] >= 0 && weights ? weights[m * T + t0 + j] : 1.f;
+                dot[j] = 0.f;
+            }
+            for (int c = part; c < vecs; c += WPT * 32) {
+                R g, v[UNSORT_BATCH];
+                g.load(dy + m * dy_stride, c);
+                if (dw) {
+#pragma unroll
+                    for (int j = 0; j < UNSORT_BATCH; ++j)
+                        if (r[j] >= 0) v[j].load(rows + r[j] * rows_stride, c);
+                }
+#pragma unroll
+                for (int j = 0; j < UNSORT_BATCH; ++j)
+                    if (r[j] >= 0) {
+                        if (dw) {
+#pragma unroll
+                            for (int k = 0; k < R::N; ++k) dot[j] = fmaf(v[j].get(k), g.get(k), dot[j]);
+                        }
+                        if (drows) {
+                            R o;
+#pragma unroll
+                            for (int k = 0; k < R::N; ++k) o.set(k, w[j] * g.get(k));
+                            o.store(drows + r[j] * drows_stride, c);
+                        }
+                    }
+            }
+            if (dw) {
+#pragma unroll
+                for (int j = 0; j < UNSORT_BATCH; ++j) {
+                    float d = dot[j];
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+                    if (lane == 0 && t0 + j < T) s_dot[warp][t0 + j] = d;
+                }
+            }
+        }
+    }
+    if (dw) {
+        __syncthreads();
+        const int tok = threadIdx.x / MAX_TOPK, t = threadIdx.x % MAX_TOPK;
+        const long long mm = (long long)blockIdx.x * (8 / WPT) + tok;
+        if (tok < 8 / WPT && mm < M && t < T) {
+            float d = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPT; ++w) d += s_dot[tok * WPT + w][t];
+            dw[mm * T + t] = d;
+        }
+    }
+    if (drows) {       // rows nobody owns
+        using V = typename R::Raw;
+        const long long all = (long long)M * T * vecs, step = (long long)gridDim.x * 256;
+        for (long long j = (long long)*kept * vecs + (long long)blockIdx.x * 256 + threadIdx.x; j < all; j += step)
+            reinterpret_cast<V*>(drows + (j / vecs) * drows_stride)[j % vecs] = V{};
+    }
+}
+
+static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_len, int M, int T, int E, int32_t* offsets,
+                       int32_t* row_of_pair, int32_t* pair_of_row, cudaStream_t st) {
+    const int P = M * T;
+    const int ctas = P > PLAN_ONE_CTA_PAIRS ? PLAN_CLUSTER : 1;
+    int warps = (PLAN_SMEM / 4 - 3 * E) / E;
+    const int need = (int)(((long long)P + 32 * ctas - 1) / (32 * ctas));
+    if (warps > 32) warps = 32;
+    if (warps > need) warps = need > 0 ? need : 1;
+    const int chunks = ctas * warps;
+    int run = (int)(((long long)P + chunks - 1) / chunks);
+    run = (run + 31) / 32 * 32;
+    const size_t smem = (size_t)4 * E * (warps + 3);
+    auto* kernel = ctas > 1 ? plan_kernel<PLAN_CLUSTER> : plan_kernel<1>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(warps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = ctas > 1 ? 2 : 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ids, expert_map, map_len, P, E, run, offsets, row_of_pair, pair_of_row));
+}
+
+static unsigned blocks_of(long long threads) { return (unsigned)((threads + 255) / 256); }
+
+template <typename T_, int VB>
+static int launch_grad(const void* dy, long long dys, const void* rows, long long rs, void* drows, long long drs, float* dw, int K,
+                       int M, int T, const int32_t* rp, const float* w, const int32_t* kept, cudaStream_t st) {
+    const int vecs = (int)((long long)K * sizeof(T_) / VB);
+    const auto a = static_cast<const uint8_t*>(dy), b = static_cast<const uint8_t*>(rows);
+    const auto o = static_cast<uint8_t*>(drows);
+    if (vecs <= 64)
+        return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 1>, (unsigned)((M + 7) / 8), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+    if (vecs <= 256)
+        return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 4>, (unsigned)((M + 1) / 2), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+    return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 8>, (unsigned)M, 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+}
+
+static int check_rows(int32_t M, int32_t T, int32_t E, int32_t K, int32_t dtype) {
+    if (M < 0 || T <= 0 || K < 0 || E <= 0 || dtype < VMOE_BF16 || dtype > VMOE_F32) return VMOE_ERR_SHAPE;
+    if (T > MAX_TOPK || E > PLAN_MAX_EXPERTS || (long long)M * T > 0x7fffffffLL - 1024) return VMOE_ERR_LIMIT;
+    // one thread per vector (at least one element), 256 threads per block
+    if ((long long)M * K / 256 >= 0x7fffffffLL) return VMOE_ERR_LIMIT;
+    return VMOE_OK;
+}
+
+}  // namespace vmoe
+
+using namespace vmoe;
+
+extern "C" {
+
+int vmoe_plan_tokens(const int32_t* topk_ids, const int32_t* expert_map, int32_t map_len, int32_t M, int32_t T, int32_t E,
+                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* stream) {
+    const int rc = check_rows(M, T, E, 0, VMOE_BF16);
+    if (rc) return rc;
+    if (!expert_offsets || (M > 0 && (!topk_ids || !row_of_pair || !pair_of_row))) return VMOE_ERR_NULL;
+    if (expert_map && map_len < 0) return VMOE_ERR_SHAPE;
+    return launch_plan(topk_ids, expert_map, map_len, M, T, E, expert_offsets, row_of_pair, pair_of_row, static_cast<cudaStream_t>(stream));
+}
+
+int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K,
+                     const int32_t* expert_offsets, const int32_t* row_of_pair, int32_t zero_tail, void* rows, int64_t rows_stride,
+                     void* stream) {
+    const int rc = check_rows(M, T, E, K, dtype);
+    if (rc) return rc;
+    if (M == 0 || K == 0) return VMOE_OK;
+    if (!x || !expert_offsets || !row_of_pair || !rows) return VMOE_ERR_NULL;
+    if (rows_stride < K || x_stride < 0) return VMOE_ERR_SHAPE;
+    const long long el = dtype == VMOE_F32 ? 4 : 2, xs = x_stride * el, rs = rows_stride * el;
+    if (((uintptr_t)x | (uintptr_t)rows) & (el - 1)) return VMOE_ERR_ALIGN;
+    const int vb = vector_bytes((uintptr_t)x | (uintptr_t)rows, xs | rs | K * el);
+    const long long vecs = K * el / vb;
+    const unsigned grid = blocks_of((long long)M * vecs);
+    const auto a = static_cast<const uint8_t*>(x);
+    const auto o = static_cast<uint8_t*>(rows);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    const int32_t* kept = expert_offsets + E;
+    if (vb == 16) e = launch_pdl(sort_kernel<uint4>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
+    else if (vb == 8) e = launch_pdl(sort_kernel<uint2>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
+    else if (vb == 4) e = launch_pdl(sort_kernel<uint32_t>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
+    else e = launch_pdl(sort_kernel<uint16_t>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
+    return cuda_status(e);
+}
+
+int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int32_t M, int32_t T, int32_t K,
+                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, void* stream) {
+    const int rc = check_rows(M, T, 1, K, dtype);
+    if (rc) return rc;
+    if (M == 0 || K == 0) return VMOE_OK;
+    if (!rows || !row_of_pair || !out) return VMOE_ERR_NULL;
+    if (out_stride < K || rows_stride < 0) return VMOE_ERR_SHAPE;
+    const long long el = dtype == VMOE_F32 ? 4 : 2, rs = rows_stride * el, os = out_stride * el;
+    if (((uintptr_t)rows | (uintptr_t)out) & (el - 1)) return VMOE_ERR_ALIGN;
+    const int vb = vector_bytes((uintptr_t)rows | (uintptr_t)out, rs | os | K * el);
+    const auto a = static_cast<const uint8_t*>(rows);
+    const auto o = static_cast<uint8_t*>(out);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return with_rows(dtype, vb, [&](auto r) {
+        using R = decltype(r);
+        const long long vecs = (long long)K / R::N;
+        return cuda_status(launch_pdl(unsort_kernel<typename R::T, R::BYTES>, blocks_of((long long)M * vecs), 256u, 0, st,
+                                      a, rs, o, os, vecs, M, T, row_of_pair, weights));
+    });
+}
+
+int vmoe_unsort_tokens_grad(const void* dout, int64_t dout_stride, const void* rows, int64_t rows_stride, int32_t dtype, int32_t M,
+                            int32_t T, int32_t E, int32_t K, const int32_t* expert_offsets, const int32_t* row_of_pair,
+                            const float* weights, void* drows, int64_t drows_stride, float* dweights, void* stream) {
+    const int rc = check_rows(M, T, E, K, dtype);
+    if (rc) return rc;
+    if (M == 0 || (!drows && !dweights)) return VMOE_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (K > 0 && (!dout || !expert_offsets || !row_of_pair || (dweights && !rows))) return VMOE_ERR_NULL;
+    if (dout_stride < 0 || (dweights && rows_stride < 0) || (drows && drows_stride < K)) return VMOE_ERR_SHAPE;
+    if (K == 0)
+        return dweights ? cuda_status(cudaMemsetAsync(dweights, 0, (size_t)M * T * sizeof(float), st)) : VMOE_OK;
+    const long long el = dtype == VMOE_F32 ? 4 : 2, ds = dout_stride * el;
+    const long long rs = dweights ? rows_stride * el : 0, gs = drows ? drows_stride * el : 0;
+    const uintptr_t ptrs = (uintptr_t)dout | (dweights ? (uintptr_t)rows : 0) | (uintptr_t)drows;
+    if (ptrs & (el - 1)) return VMOE_ERR_ALIGN;
+    const int vb = vector_bytes(ptrs, ds | rs | gs | K * el);
+    return with_rows(dtype, vb, [&](auto r) {
+        using R = decltype(r);
+        return launch_grad<typename R::T, R::BYTES>(dout, ds, rows, rs, drows, gs, dweights, K, M, T, row_of_pair, weights,
+                                                    expert_offsets + E, st);
+    });
+}
+
+}  // extern "C"

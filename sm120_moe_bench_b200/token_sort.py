@@ -1,0 +1,219 @@
+"""Token rows sorted by expert and back, with the router's weights applied; both directions are differentiable.
+
+    plan = plan_tokens(topk_ids, num_experts)            # once per batch
+    rows = sort_tokens(hidden, plan)                     # [M * T, K], the rows of expert e at plan.expert_offsets[e]
+    ...                                                  # the experts' own work on the rows
+    out = unsort_tokens(rows, plan, topk_weights)        # [M, K] = sum over a token's rows of weight * row
+
+Rows are bf16, fp16 or f32 with any row stride (elements of a row next to each other).  Sums run in f32 over a token's
+choices in order and are rounded once; nothing depends on the order in which blocks run.  Dropped pairs (ids outside the
+experts, or not local under an ``expert_map``) take part in nothing: they have no row, add nothing to a sum, and their
+weights get a zero gradient.  They leave ``M * T - kept`` rows behind the last kept one; these are zero in every tensor
+made here (rows and gradients) and left as they were in a tensor given as ``out``.
+
+A backward pass is captured into a CUDA graph together with its forward pass; eager graphs of the same leaf tensors have
+to be gone by then, as for any operator of torch (a leaf's accumulator stays bound to the stream of the graph that made it).
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import check, lib
+
+DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+MAX_TOPK = 16
+MAX_EXPERTS = 8192
+
+
+class _on:
+    """The device of the tensors as the current one (nothing to do when it already is), and its current stream."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torch.device | None = None) -> torch.Tensor:
+    """``t`` as a matrix of rows the kernels can read: 2-D, on the device, elements of a row next to each other."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in DTYPE_CODES:
+        raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, got {t.dim()}")
+    if rows is not None and t.shape[0] != rows:
+        raise ValueError(f"{name} must have {rows} rows, got {t.shape[0]}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the plan on {device}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"the elements of a row of {name} must lie next to each other")
+    return t
+
+
+def check_out(out: torch.Tensor, rows: int, like: torch.Tensor) -> torch.Tensor:
+    check_rows(out, "out", rows, like.device)
+    if out.dtype != like.dtype or out.shape[1] != like.shape[1]:
+        raise ValueError(f"out must be {like.dtype} with {like.shape[1]} columns")
+    if rows > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("the rows of out must not overlap")
+    return out
+
+
+@dataclass(frozen=True, eq=False)
+class TokenPlan:
+    """Which row each (token, choice) pair has.  Made by ``plan_tokens``; the tensors stay on the device."""
+
+    expert_offsets: torch.Tensor     # int32 [E + 1]: rows of expert e are expert_offsets[e] .. expert_offsets[e + 1] - 1
+    row_of_pair: torch.Tensor        # int32 [M, T], -1 = dropped
+    pair_of_row: torch.Tensor        # int32 [M * T], -1 behind the last kept row
+    num_experts: int
+
+    @property
+    def tokens(self) -> int:
+        return self.row_of_pair.shape[0]
+
+    @property
+    def topk(self) -> int:
+        return self.row_of_pair.shape[1]
+
+    @property
+    def rows(self) -> int:
+        return self.pair_of_row.shape[0]
+
+
+def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tensor | None = None) -> TokenPlan:
+    """Tables of the stable sort of the ``[M, T]`` int32 expert ids by expert (one launch).
+
+    With ``expert_map`` (int32, -1 = not local) the ids are global and ``num_experts`` counts the local ones.  Ids outside
+    the map, or outside ``[0, num_experts)``, drop their pair.  ``T <= 16``, ``num_experts <= 8192``."""
+    if not topk_ids.is_cuda:
+        raise ValueError("topk_ids must be a CUDA tensor")
+    if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2:
+        raise ValueError("topk_ids must be an int32 tensor [tokens, choices]")
+    if not topk_ids.is_contiguous():
+        raise ValueError("topk_ids must be contiguous")
+    M, T = topk_ids.shape
+    if not 1 <= T <= MAX_TOPK:
+        raise ValueError(f"1 to {MAX_TOPK} choices per token, got {T}")
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
+    dev = topk_ids.device
+    if expert_map is not None:
+        if expert_map.device != dev or expert_map.dtype != torch.int32 or expert_map.dim() != 1 or not expert_map.is_contiguous():
+            raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids")
+        if expert_map.numel() == 0:
+            raise ValueError("expert_map is empty")
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    row_of_pair = torch.empty(M, T, dtype=torch.int32, device=dev)
+    pair_of_row = torch.empty(M * T, dtype=torch.int32, device=dev)
+    with _on(dev) as stream:
+        check(lib.vmoe_plan_tokens(topk_ids.data_ptr(), None if expert_map is None else expert_map.data_ptr(),
+                                   0 if expert_map is None else expert_map.numel(), M, T, num_experts, offsets.data_ptr(),
+                                   row_of_pair.data_ptr(), pair_of_row.data_ptr(), stream), "vmoe_plan_tokens")
+    return TokenPlan(offsets, row_of_pair, pair_of_row, num_experts)
+
+
+def _sort(x, plan: TokenPlan, out=None):
+    K = x.shape[1]
+    rows = torch.empty(plan.rows, K, dtype=x.dtype, device=x.device) if out is None else out
+    with _on(x.device) as stream:
+        check(lib.vmoe_sort_tokens(x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], plan.tokens, plan.topk, plan.num_experts, K,
+                                   plan.expert_offsets.data_ptr(), plan.row_of_pair.data_ptr(), out is None, rows.data_ptr(),
+                                   max(rows.stride(0), K), stream), "vmoe_sort_tokens")
+    return rows
+
+
+def _unsort(rows, plan: TokenPlan, weights=None, out=None):
+    K = rows.shape[1]
+    y = torch.empty(plan.tokens, K, dtype=rows.dtype, device=rows.device) if out is None else out
+    with _on(rows.device) as stream:
+        check(lib.vmoe_unsort_tokens(rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype], plan.tokens, plan.topk, K,
+                                     plan.row_of_pair.data_ptr(), None if weights is None else weights.data_ptr(), y.data_ptr(),
+                                     max(y.stride(0), K), stream), "vmoe_unsort_tokens")
+    return y
+
+
+def _dense_rows(g: torch.Tensor) -> torch.Tensor:
+    """A gradient as torch hands it over may be expanded along its columns (the gradient of a sum)."""
+    return g if g.shape[1] <= 1 or g.stride(1) == 1 else g.contiguous()
+
+
+class _SortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return _sort(x, plan)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _unsort(_dense_rows(grad), ctx.plan), None
+
+
+class _UnsortTokens(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, plan, weights):
+        ctx.plan = plan
+        ctx.save_for_backward(rows, weights)
+        return _unsort(rows, plan, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        rows, weights = ctx.saved_tensors
+        plan, grad = ctx.plan, _dense_rows(grad)
+        M, T, K = plan.tokens, plan.topk, rows.shape[1]
+        drows = torch.empty(plan.rows, K, dtype=rows.dtype, device=rows.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(M, T, dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[2] else None
+        with _on(rows.device) as stream:
+            check(lib.vmoe_unsort_tokens_grad(grad.data_ptr(), grad.stride(0), rows.data_ptr(), rows.stride(0),
+                                              DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan.expert_offsets.data_ptr(),
+                                              plan.row_of_pair.data_ptr(), None if weights is None else weights.data_ptr(),
+                                              None if drows is None else drows.data_ptr(), K, None if dw is None else dw.data_ptr(),
+                                              stream), "vmoe_unsort_tokens_grad")
+        return drows, None, dw
+
+
+def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rows[r] = x[token of row r]``: the token rows ``[M, K]`` in expert order, ``[M * T, K]``.  Differentiable in ``x``
+    (a token's gradient is the sum over its rows) unless ``out`` is given."""
+    check_rows(x, "x", plan.tokens, plan.expert_offsets.device)
+    if out is not None:
+        if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
+            raise ValueError("out cannot be given where a gradient is wanted")
+        return _sort(x, plan, check_out(out, plan.rows, x))
+    if x.requires_grad and torch.is_grad_enabled():
+        return _SortTokens.apply(x, plan)
+    return _sort(x, plan)
+
+
+def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[m] = sum_t weights[m, t] * rows[row of (m, t)]``: rows ``[M * T, K]`` in expert order back to tokens ``[M, K]``.
+    ``weights`` f32 ``[M, T]`` (None = 1).  Differentiable in ``rows`` and ``weights`` unless ``out`` is given."""
+    check_rows(rows, "rows", plan.rows, plan.expert_offsets.device)
+    if weights is not None:
+        if weights.device != rows.device or weights.dtype != torch.float32 or tuple(weights.shape) != (plan.tokens, plan.topk):
+            raise ValueError(f"weights must be a float32 tensor [{plan.tokens}, {plan.topk}] on the device of rows")
+        if not weights.is_contiguous():
+            raise ValueError("weights must be contiguous")
+    grad = torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))
+    if out is not None:
+        if grad or (torch.is_grad_enabled() and out.requires_grad):
+            raise ValueError("out cannot be given where a gradient is wanted")
+        return _unsort(rows, plan, weights, check_out(out, plan.tokens, rows))
+    if grad:
+        return _UnsortTokens.apply(rows, plan, weights)
+    return _unsort(rows, plan, weights)

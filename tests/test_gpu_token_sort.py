@@ -1,0 +1,314 @@
+"""Token rows sorted by expert and back against a plain implementation in 64 bits, with the gradients.
+
+Tolerances: copies are bit-equal.  A sum of T products in f32 is off by at most (T + 1) * 2^-24 * sum |w| |r| before it is
+rounded to the output type, which adds half a step (eps / 2 of the value; 2^-25 absolute among fp16's subnormals).  A dot
+product over K elements in f32, in any order, is off by at most (K + 1) * 2^-24 * sum |r| |dy|."""
+import os
+
+import pytest
+import torch
+
+os.environ.setdefault("VMOE_NO_VLLM", "1")
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def rows_of(M, K, dtype, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(M, K, generator=g, device="cuda").to(dtype)
+
+
+def ids_of(M, T, E, seed, repeat=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    if repeat:                                            # the same expert several times in a token
+        return torch.randint(0, E, (M, T), generator=g, device="cuda", dtype=torch.int32)
+    return torch.topk(torch.randn(M, E, generator=g, device="cuda"), T, dim=1).indices.int()
+
+
+def plain_plan(ids, E, expert_map=None):
+    flat = ids.cpu().reshape(-1).tolist()
+    emap = None if expert_map is None else expert_map.cpu().tolist()
+    local = []
+    for e in flat:
+        if emap is not None:
+            e = emap[e] if 0 <= e < len(emap) else -1
+        local.append(e if 0 <= e < E else -1)
+    order = sorted((e, p) for p, e in enumerate(local) if e >= 0)
+    row_of_pair = [-1] * len(flat)
+    for r, (_, p) in enumerate(order):
+        row_of_pair[p] = r
+    pair_of_row = [p for _, p in order] + [-1] * (len(flat) - len(order))
+    offsets = [sum(1 for e in local if 0 <= e < x) for x in range(E + 1)] if E <= 64 else \
+        torch.searchsorted(torch.tensor([e for e, _ in order], dtype=torch.int64), torch.arange(E + 1)).tolist()
+    return (torch.tensor(offsets, dtype=torch.int32), torch.tensor(row_of_pair, dtype=torch.int32).reshape(ids.shape),
+            torch.tensor(pair_of_row, dtype=torch.int32))
+
+
+def check_plan(plan, ids, E, expert_map=None):
+    offsets, row_of_pair, pair_of_row = plain_plan(ids, E, expert_map)
+    assert torch.equal(plan.expert_offsets.cpu(), offsets)
+    assert torch.equal(plan.row_of_pair.cpu(), row_of_pair)
+    assert torch.equal(plan.pair_of_row.cpu(), pair_of_row)
+
+
+def half_step(dtype, value):
+    return torch.finfo(dtype).eps / 2 * value.abs() * (1 + 2.0 ** -20) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126)
+
+
+def plain_unsort(rows, row_of_pair, w):
+    """(sum, sum of magnitudes) in 64 bits"""
+    kept = (row_of_pair >= 0).double()[:, :, None]
+    r = rows.double()[row_of_pair.clamp(min=0).long()]
+    r = torch.where(kept > 0, r, 0.0)
+    w = torch.ones(row_of_pair.shape, dtype=torch.float64, device=rows.device) if w is None else w.double()
+    w = torch.where(row_of_pair >= 0, w, 0.0)[:, :, None]
+    return (r * w).sum(1), (r * w).abs().sum(1)
+
+
+@pytest.mark.parametrize("M,T,E,repeat", [(0, 2, 4, False), (1, 1, 1, False), (1, 16, 16, False), (3, 2, 5, True), (64, 10, 512, False),
+                                          (409, 10, 512, False), (410, 10, 512, False), (1000, 7, 33, True), (2049, 8, 8, False),
+                                          (5000, 3, 8192, True), (700, 16, 1, True), (4097, 1, 2, False), (8192, 10, 512, False)])
+def test_plan(M, T, E, repeat):
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(M, T, E, 1, repeat) if M else torch.zeros(0, T, dtype=torch.int32, device="cuda")
+    check_plan(vm.plan_tokens(ids, E), ids, E)
+
+
+def test_plan_drops_ids_outside_the_experts_and_the_map():
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(300, 6, 40, 2, True)
+    ids[::7, 2] = -1
+    ids[::5, 1] = 40
+    ids[11] = 2 ** 31 - 1
+    ids[12] = -2 ** 31
+    check_plan(vm.plan_tokens(ids, 40), ids, 40)
+    emap = torch.full((40,), -1, dtype=torch.int32, device="cuda")
+    emap[8:20] = torch.arange(12, device="cuda", dtype=torch.int32)
+    emap[3] = 12                                          # a map entry outside the local experts
+    check_plan(vm.plan_tokens(ids, 12, emap), ids, 12, emap)
+    nothing = torch.full((9, 3), -1, dtype=torch.int32, device="cuda")
+    plan = vm.plan_tokens(nothing, 4)
+    check_plan(plan, nothing, 4)
+    x = rows_of(9, 24, torch.bfloat16, 3)
+    assert torch.count_nonzero(vm.sort_tokens(x, plan)) == 0
+    rows = torch.full((27, 24), float("nan"), dtype=torch.bfloat16, device="cuda")
+    assert torch.count_nonzero(vm.unsort_tokens(rows, plan, torch.full((9, 3), float("inf"), device="cuda"))) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,T,E,K", [(1, 1, 1, 1), (1, 10, 512, 4096), (5, 2, 3, 7), (33, 16, 64, 136), (64, 10, 512, 4096), (257, 3, 9, 1021),
+                                     (100, 5, 20, 1026), (129, 4, 8, 2052), (31, 8, 16, 5000)])
+def test_forward_and_gradients(M, T, E, K, dtype):
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(M, T, E, 5)
+    if M > 4:
+        ids[::4, T - 1] = -1
+    plan = vm.plan_tokens(ids, E)
+    check_plan(plan, ids, E)
+    rp, pr = plan.row_of_pair, plan.pair_of_row
+    x = rows_of(M, K, dtype, 6).requires_grad_()
+    rows = vm.sort_tokens(x, plan)
+    want = torch.where((pr >= 0)[:, None], x.detach()[(pr.clamp(min=0) // T).long()], 0.0)
+    assert torch.equal(rows, want)
+    g = rows_of(M * T, K, dtype, 7)
+    dx, = torch.autograd.grad(rows, x, g)
+    s, mag = plain_unsort(g, rp, None)
+    assert dx.dtype == dtype and bool(((dx.double() - s).abs() <= (T + 1) * 2.0 ** -24 * mag + half_step(dtype, s)).all())
+
+    w = torch.softmax(rows_of(M, T, torch.float32, 8), 1).requires_grad_()
+    r = rows_of(M * T, K, dtype, 9).requires_grad_()
+    y = vm.unsort_tokens(r, plan, w)
+    s, mag = plain_unsort(r.detach(), rp, w.detach())
+    assert y.dtype == dtype and bool(((y.double() - s).abs() <= (T + 1) * 2.0 ** -24 * mag + half_step(dtype, s)).all())
+    dy = rows_of(M, K, dtype, 10)
+    dr, dw = torch.autograd.grad(y, (r, w), dy)
+    tok, flat = (pr.clamp(min=0) // T).long(), w.detach().reshape(-1)[pr.clamp(min=0).long()].double()
+    want = torch.where((pr >= 0)[:, None], dy.double()[tok] * flat[:, None], 0.0)
+    assert bool(((dr.double() - want).abs() <= 2.0 ** -24 * want.abs() + half_step(dtype, want)).all())
+    assert torch.count_nonzero(dr[int(plan.expert_offsets[-1]):]) == 0
+    rr = torch.where((rp >= 0)[:, :, None], r.detach().double()[rp.clamp(min=0).long()], 0.0)
+    want, mag = (rr * dy.double()[:, None]).sum(2), (rr * dy.double()[:, None]).abs().sum(2)
+    assert bool(((dw.double() - want).abs() <= (K + 1) * 2.0 ** -24 * mag).all())
+
+
+def test_one_gradient_at_a_time():
+    import sm120_moe_bench_b200 as vm
+    plan = vm.plan_tokens(ids_of(20, 3, 6, 11), 6)
+    r, w, dy = rows_of(60, 72, torch.float32, 12), torch.rand(20, 3, device="cuda"), rows_of(20, 72, torch.float32, 13)
+    ra, wa = r.clone().requires_grad_(), w.clone().requires_grad_()
+    both = torch.autograd.grad(vm.unsort_tokens(ra, plan, wa), (ra, wa), dy)
+    rb = r.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(vm.unsort_tokens(rb, plan, w), rb, dy)[0], both[0])
+    wb = w.clone().requires_grad_()
+    assert torch.equal(torch.autograd.grad(vm.unsort_tokens(r, plan, wb), wb, dy)[0], both[1])
+    rc = r.clone().requires_grad_()
+    ones = torch.autograd.grad(vm.unsort_tokens(rc, plan), rc, dy)[0]
+    assert torch.equal(ones, vm.sort_tokens(dy, plan))
+    with torch.no_grad():
+        assert not vm.unsort_tokens(ra, plan, wa).requires_grad
+
+
+def test_gradients_against_differences():
+    """A scalar of the round trip is linear in x and in w: central differences are exact but for f32 rounding, which the step
+    keeps at 2^-24 * |scalar parts| / step."""
+    import sm120_moe_bench_b200 as vm
+    plan = vm.plan_tokens(ids_of(6, 3, 4, 14, True), 4)
+    x, w = rows_of(6, 10, torch.float32, 15).requires_grad_(), torch.rand(6, 3, device="cuda").requires_grad_()
+    c, gain = rows_of(6, 10, torch.float32, 16), rows_of(18, 10, torch.float32, 17)
+
+    def f(x, w):
+        return (vm.unsort_tokens(vm.sort_tokens(x, plan) * gain, plan, w) * c).double().sum()
+
+    dx, dw = torch.autograd.grad(f(x, w), (x, w))
+    step = 2.0 ** -3
+    scale = float((plain_unsort((vm.sort_tokens(x.detach(), plan) * gain), plan.row_of_pair, w.detach())[1] * c.double().abs()).sum())
+    tol = 16 * 2.0 ** -24 * (scale + 10) / step
+    with torch.no_grad():
+        for t, d in ((x, dx), (w, dw)):
+            for i in range(t.numel()):
+                e = torch.zeros_like(t)
+                e.view(-1)[i] = step
+                a, b = ((f(x + e, w), f(x - e, w)) if t is x else (f(x, w + e), f(x, w - e)))
+                assert abs(float((a - b) / (2 * step)) - float(d.view(-1)[i])) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_and_alignment(dtype):
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 37, 3, 5, 64
+    plan = vm.plan_tokens(ids_of(M, T, E, 18), E)
+    base = rows_of(M + 1, 2 * K + 3, dtype, 19)
+    for x in (base[:M, :K], base[:M, 1:K + 1], base[1:, 3:K + 3], base[::1][:M, K:2 * K], base[:1, :K].expand(M, K)):
+        assert torch.equal(vm.sort_tokens(x, plan), vm.sort_tokens(x.contiguous(), plan))
+    rows = rows_of(M * T, K + 5, dtype, 20)
+    w = torch.rand(M, T, device="cuda")
+    for r in (rows[:, :K], rows[:, 1:K + 1], rows[:, 5:]):
+        assert torch.equal(vm.unsort_tokens(r, plan, w), vm.unsort_tokens(r.contiguous(), plan, w))
+    # gradients that arrive expanded (of a sum) or strided
+    x = base[:M, 1:K + 1].detach().requires_grad_()
+    dx, = torch.autograd.grad(vm.sort_tokens(x, plan).sum(), x)
+    assert torch.equal(dx, torch.full_like(dx, T))
+    r = rows[:, 1:K + 1].detach().requires_grad_()
+    dr, = torch.autograd.grad(vm.unsort_tokens(r, plan, w), r, base[:M, 2:K + 2])
+    r2 = r.detach().contiguous().requires_grad_()
+    assert torch.equal(dr, torch.autograd.grad(vm.unsort_tokens(r2, plan, w), r2, base[:M, 2:K + 2].contiguous())[0])
+
+
+def test_out_keeps_what_is_behind_the_last_row():
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(10, 4, 6, 21)
+    ids[:, 0] = -1
+    plan = vm.plan_tokens(ids, 6)
+    x = rows_of(10, 40, torch.float16, 22)
+    buf = torch.full((41, 50), 7.0, dtype=torch.float16, device="cuda")
+    got = vm.sort_tokens(x, plan, out=buf[:40, 3:43])
+    assert got.data_ptr() == buf[:40, 3:43].data_ptr()
+    assert torch.equal(buf[:30, 3:43], vm.sort_tokens(x, plan)[:30])
+    assert bool((buf[30:] == 7).all()) and bool((buf[:, :3] == 7).all()) and bool((buf[:, 43:] == 7).all())
+    y = torch.full((11, 44), 5.0, dtype=torch.float16, device="cuda")
+    vm.unsort_tokens(buf[:40, 3:43], plan, out=y[:10, 2:42])
+    assert torch.equal(y[:10, 2:42], vm.unsort_tokens(buf[:40, 3:43].contiguous(), plan))
+    assert bool((y[10] == 5).all()) and bool((y[:, :2] == 5).all()) and bool((y[:, 42:] == 5).all())
+
+
+def test_non_finite_values_stay_in_their_tokens():
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(12, 2, 4, 23)
+    ids[5, 1] = -1
+    plan = vm.plan_tokens(ids, 4)
+    rows = rows_of(24, 16, torch.bfloat16, 24)
+    clean = vm.unsort_tokens(rows, plan, torch.ones(12, 2, device="cuda"))
+    w = torch.ones(12, 2, device="cuda")
+    w[5, 1] = float("nan")                                # the weight of a dropped pair
+    w[7, 0] = float("nan")
+    rows[23] = float("inf")                               # behind the last kept row
+    y = vm.unsort_tokens(rows, plan, w)
+    assert bool(y[7].isnan().all())
+    keep = torch.arange(12, device="cuda") != 7
+    assert torch.equal(y[keep], clean[keep])
+
+
+def test_more_than_four_gigabytes_of_rows():
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 40000, 16, 32, 4096
+    ids = ids_of(M, T, E, 25)
+    plan = vm.plan_tokens(ids, E)
+    x = rows_of(M, K, torch.bfloat16, 26)
+    rows = vm.sort_tokens(x, plan)
+    assert rows.numel() * 2 > 2 ** 32
+    for r in (0, M * T // 2, M * T - 1):
+        assert torch.equal(rows[r], x[int(plan.pair_of_row[r]) // T])
+    w = torch.full((M, T), 1 / 16, device="cuda")
+    assert torch.equal(vm.unsort_tokens(rows, plan, w), x)     # sixteen times a sixteenth, exact in f32
+    rows.requires_grad_()
+    dr, = torch.autograd.grad(vm.unsort_tokens(rows, plan, w), rows, x)
+    assert torch.equal(dr[-1], x[int(plan.pair_of_row[-1]) // T] / 16)
+
+
+def test_side_stream_and_graph():
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 50, 4, 16, 256
+    x, w = rows_of(M, K, torch.bfloat16, 27), torch.rand(M, T, device="cuda")
+    ids = ids_of(M, T, E, 28)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        plan = vm.plan_tokens(ids, E)
+        side = vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w)
+    torch.cuda.current_stream().wait_stream(s)
+    plan = vm.plan_tokens(ids, E)
+    assert torch.equal(side, vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w))
+    # forward and backward captured together, replayed on other inputs
+    xs, ws, ids_s, dy = x.clone().requires_grad_(), w.clone().requires_grad_(), ids.clone(), rows_of(M, K, torch.bfloat16, 29)
+
+    def step():
+        p = vm.plan_tokens(ids_s, E)
+        y = vm.unsort_tokens(vm.sort_tokens(xs, p), p, ws)
+        return (y.detach(), *torch.autograd.grad(y, (xs, ws), dy))
+
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = step()
+    for seed in (30, 31):
+        with torch.no_grad():
+            xs.copy_(rows_of(M, K, torch.bfloat16, seed))
+            ids_s.copy_(ids_of(M, T, E, seed))
+        g.replay()
+        eager = step()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager))
+
+
+def test_refusals():
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(8, 2, 4, 32)
+    for bad in (ids.long(), ids[0], ids[:, :1].expand(8, 2), ids.t()):
+        with pytest.raises(ValueError):
+            vm.plan_tokens(bad, 4)
+    for E in (0, 8193):
+        with pytest.raises(ValueError):
+            vm.plan_tokens(ids, E)
+    with pytest.raises(ValueError):
+        vm.plan_tokens(torch.zeros(4, 17, dtype=torch.int32, device="cuda"), 4)
+    for emap in (torch.zeros(4, dtype=torch.int32), torch.zeros(4, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError):
+            vm.plan_tokens(ids, 4, emap)
+    plan = vm.plan_tokens(ids, 4)
+    x = rows_of(8, 16, torch.float32, 33)
+    for bad in (x.double(), x[:7], x[0], x.t().contiguous().t(), rows_of(8, 32, torch.float32, 33)[:, ::2], x.cpu()):
+        with pytest.raises(ValueError):
+            vm.sort_tokens(bad, plan)
+    with pytest.raises(ValueError):
+        vm.sort_tokens(x.clone().requires_grad_(), plan, out=torch.empty(16, 16, device="cuda"))
+    for out in (torch.empty(15, 16, device="cuda"), torch.empty(16, 17, device="cuda"), torch.empty(16, 16, device="cuda").half(),
+                torch.empty(1, 16, device="cuda").expand(16, 16)):
+        with pytest.raises(ValueError):
+            vm.sort_tokens(x, plan, out=out)
+    rows, w = rows_of(16, 16, torch.float32, 34), torch.ones(8, 2, device="cuda")
+    for bad in (w.half(), w[:7], w.t().contiguous().t(), w.cpu()):
+        with pytest.raises(ValueError):
+            vm.unsort_tokens(rows, plan, bad)
+    with pytest.raises(ValueError):
+        vm.unsort_tokens(rows[:15], plan, w)
+    # the operator still answers afterwards
+    assert torch.equal(vm.unsort_tokens(vm.sort_tokens(x, plan), plan), 2 * x)

@@ -1,0 +1,74 @@
+"""Token sort without a GPU: argument checks of the C entry points and of the torch functions, none of which reach a device."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+os.environ.setdefault("VMOE_NO_VLLM", "1")
+
+
+def _lib():
+    from sm120_moe_bench_b200 import _lib
+    return _lib.lib
+
+
+def _buf(n=4096):
+    return (ctypes.c_char * n)()          # host memory: a call that got past its checks would not be made here
+
+
+def test_plan_checks():
+    lib, b = _lib(), ctypes.addressof(_buf())
+    plan = lambda M, T, E, ids=b, off=b, rp=b, pr=b, emap=None, n=0: lib.vmoe_plan_tokens(ids, emap, n, M, T, E, off, rp, pr, None)
+    assert plan(-1, 2, 4) == 2 and plan(4, 0, 4) == 2 and plan(4, 2, 0) == 2
+    assert plan(4, 17, 32) == 8 and plan(4, 2, 8193) == 8 and plan(2 ** 31 - 1, 16, 4) == 8 and plan(2 ** 27, 16, 4) == 8
+    assert plan(4, 2, 4, ids=None) == 1 and plan(4, 2, 4, off=None) == 1 and plan(4, 2, 4, rp=None) == 1 and plan(4, 2, 4, pr=None) == 1
+    assert plan(4, 2, 4, emap=b, n=-1) == 2
+
+
+def test_sort_checks():
+    lib, b = _lib(), ctypes.addressof(_buf())
+
+    def sort(M=4, T=2, E=4, K=8, dtype=0, x=b, xs=8, off=b, rp=b, rows=b, rs=8):
+        return lib.vmoe_sort_tokens(x, xs, dtype, M, T, E, K, off, rp, 1, rows, rs, None)
+
+    assert sort(M=0) == 0 and sort(K=0) == 0                       # nothing to do
+    assert sort(M=-1) == 2 and sort(T=0) == 2 and sort(K=-1) == 2 and sort(dtype=3) == 2 and sort(dtype=-1) == 2
+    assert sort(T=17) == 8 and sort(E=8193) == 8
+    assert sort(rs=7) == 2 and sort(xs=-1) == 2
+    for name in ("x", "off", "rp", "rows"):
+        assert sort(**{name: None}) == 1, name
+    assert sort(x=b + 1) == 3 and sort(dtype=2, rows=b + 2) == 3    # not a multiple of the element
+
+
+def test_unsort_checks():
+    lib, b = _lib(), ctypes.addressof(_buf())
+
+    def unsort(M=4, T=2, K=8, dtype=0, rows=b, rs=8, rp=b, out=b, os_=8):
+        return lib.vmoe_unsort_tokens(rows, rs, dtype, M, T, K, rp, None, out, os_, None)
+
+    assert unsort(M=0) == 0 and unsort(K=0) == 0
+    assert unsort(M=-1) == 2 and unsort(dtype=7) == 2 and unsort(os_=7) == 2 and unsort(rs=-1) == 2 and unsort(T=17) == 8
+    for name in ("rows", "rp", "out"):
+        assert unsort(**{name: None}) == 1, name
+    assert unsort(out=b + 1) == 3
+
+    def grad(M=4, T=2, E=4, K=8, dy=b, ds=8, rows=b, rs=8, off=b, rp=b, drows=b, gs=8, dw=b):
+        return lib.vmoe_unsort_tokens_grad(dy, ds, rows, rs, 0, M, T, E, K, off, rp, None, drows, gs, dw, None)
+
+    assert grad(M=0) == 0 and grad(drows=None, dw=None) == 0
+    assert grad(dy=None) == 1 and grad(off=None) == 1 and grad(rp=None) == 1 and grad(rows=None) == 1
+    assert grad(ds=-1) == 2 and grad(rs=-1) == 2 and grad(gs=7) == 2 and grad(T=17) == 8 and grad(dy=b + 1) == 3
+
+
+def test_host_tensors_are_refused():
+    import sm120_moe_bench_b200 as vm
+    ids = torch.zeros(4, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        vm.plan_tokens(ids, 4)
+    plan = vm.TokenPlan(torch.zeros(5, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), 4)
+    assert (plan.tokens, plan.topk, plan.rows) == (4, 2, 8)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        vm.sort_tokens(torch.zeros(4, 8), plan)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        vm.unsort_tokens(torch.zeros(8, 8), plan)
