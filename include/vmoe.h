@@ -332,9 +332,11 @@ int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
                      void* stream);
 
 /* out[m] = sum_t weights[m, t] * rows[row_of_pair[m, t]] over the kept pairs, t ascending, f32, rounded once (0 without
- * a kept pair).  weights [M, T] f32, NULL = all 1, which is the gradient of vmoe_sort_tokens. */
+ * a kept pair).  weights [M, T] f32, NULL = all 1, which is the gradient of vmoe_sort_tokens.  out_dtype = dtype, or any
+ * type when the rows are f32. */
 int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int32_t M, int32_t T, int32_t K,
-                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, void* stream);
+                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, int32_t out_dtype,
+                       void* stream);
 
 /* Gradient of vmoe_unsort_tokens: drows[r] = weights * dout[token] (rows behind the last kept one: 0) and
  * dweights[m, t] = <rows[r], dout[m]> in f32 (dropped pairs: 0).  Either output may be NULL; rows may be NULL when
@@ -342,6 +344,27 @@ int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int
 int vmoe_unsort_tokens_grad(const void* dout, int64_t dout_stride, const void* rows, int64_t rows_stride, int32_t dtype, int32_t M,
                             int32_t T, int32_t E, int32_t K, const int32_t* expert_offsets, const int32_t* row_of_pair,
                             const float* weights, void* drows, int64_t drows_stride, float* dweights, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit integer rows with one f32 scale each (activations: a scale per token; weights: a scale per output channel), and
+ * their product.  Strides are in elements.
+ *
+ * vmoe_int8_quantize: scales[r] = max|x[r]| / 127 and q[r, k] = rint(127 x[r, k] / max|x[r]|), the code of the exact
+ * quotient, ties to even.  A row of zeros gets scale 0, a row with an infinity or NaN scale NaN and codes 0.  With
+ * row_of_pair [rows, T] (the table of vmoe_plan_tokens) row r is a token and its codes and scale go to its T sorted rows.
+ * live_rows (device, may be NULL): rows from *live_rows on are not touched. */
+int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t rows, int32_t K, int32_t T, const int32_t* row_of_pair,
+                       const int32_t* live_rows, int8_t* q, int64_t q_stride, float* scales, void* stream);
+
+/* out[m, n] = (sum_k a[m, k] w[n, k]) * a_scale[m] * w_scale[n]; the sum is exact (K <= 131071, VMOE_ERR_LIMIT beyond),
+ * the scales are applied in f32 and the result is rounded once to out_dtype (vmoe_dtype).
+ * expert_offsets [E + 1] (vmoe_plan_tokens; NULL = dense, E = 1): rows expert_offsets[e] .. use w[e] and w_scale[e]; rows
+ * behind expert_offsets[E] are set to zero when zero_tail != 0, else left as they were.
+ * swiglu != 0: w has 2 N rows per expert, the N gate rows first, and out = silu(gate) * up.
+ * Operands whose addresses and strides are multiples of 16 bytes take the tensor cores. */
+int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, int32_t M, const int8_t* w, int64_t w_stride,
+                     int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
+                     int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -89,9 +89,13 @@ SIGNATURES = {
     "vmoe_plan_tokens": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     "vmoe_sort_tokens": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int32,
                                    _P, C.c_int64, _P]),
-    "vmoe_unsort_tokens": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P]),
+    "vmoe_unsort_tokens": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, C.c_int32,
+                                     _P]),
     "vmoe_unsort_tokens_grad": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                           _P, _P, _P, _P, C.c_int64, _P, _P]),
+    "vmoe_int8_quantize": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P, _P]),
+    "vmoe_int8_matmul": (C.c_int, [_P, C.c_int64, _P, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P,
+                                   C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P]),
 }
 
 

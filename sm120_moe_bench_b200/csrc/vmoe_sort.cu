@@ -178,11 +178,11 @@ sort_kernel(const uint8_t* __restrict__ x, long long x_stride, uint8_t* __restri
 
 // ---------------------------------------------------------------------------------
 // Unsort: a thread owns one vector of one token and sums it over the token's pairs in order; four rows are requested
-// at a time.
+// at a time.  Rows in f32 may leave as bf16 / fp16: the expert layer's rows stay in f32 until they are summed.
 // ---------------------------------------------------------------------------------
 constexpr int UNSORT_BATCH = 4;
 
-template <typename T_, int VB>
+template <typename T_, int VB, typename O_>
 __global__ void __launch_bounds__(256)
 unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* __restrict__ out, long long out_stride, long long vecs,
               int M, int T, const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights) {
@@ -211,7 +211,7 @@ unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* 
                 for (int k = 0; k < R::N; ++k) acc[k] = fmaf(w, v[j].get(k), acc[k]);
             }
     }
-    R o;
+    RowVec<O_, R::N * (int)sizeof(O_)> o;
 #pragma unroll
     for (int k = 0; k < R::N; ++k) o.set(k, acc[k]);
     o.store(out + m * out_stride, c);
@@ -386,23 +386,35 @@ int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
 }
 
 int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int32_t M, int32_t T, int32_t K,
-                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, void* stream) {
+                       const int32_t* row_of_pair, const float* weights, void* out, int64_t out_stride, int32_t out_dtype,
+                       void* stream) {
     const int rc = check_rows(M, T, 1, K, dtype);
     if (rc) return rc;
+    if (out_dtype != dtype && (dtype != VMOE_F32 || out_dtype < VMOE_BF16 || out_dtype > VMOE_F32)) return VMOE_ERR_SHAPE;
     if (M == 0 || K == 0) return VMOE_OK;
     if (!rows || !row_of_pair || !out) return VMOE_ERR_NULL;
     if (out_stride < K || rows_stride < 0) return VMOE_ERR_SHAPE;
-    const long long el = dtype == VMOE_F32 ? 4 : 2, rs = rows_stride * el, os = out_stride * el;
-    if (((uintptr_t)rows | (uintptr_t)out) & (el - 1)) return VMOE_ERR_ALIGN;
-    const int vb = vector_bytes((uintptr_t)rows | (uintptr_t)out, rs | os | K * el);
+    const long long el = dtype == VMOE_F32 ? 4 : 2, ol = out_dtype == VMOE_F32 ? 4 : 2, rs = rows_stride * el, os = out_stride * ol;
+    if (((uintptr_t)rows & (el - 1)) || ((uintptr_t)out & (ol - 1))) return VMOE_ERR_ALIGN;
+    // a vector of n row elements becomes n output elements: both sides have to allow it
+    int vb = vector_bytes((uintptr_t)rows, rs | K * el);
+    const int ob = vector_bytes((uintptr_t)out, os) / (int)ol * (int)el;
+    if (vb > ob) vb = ob;
     const auto a = static_cast<const uint8_t*>(rows);
     const auto o = static_cast<uint8_t*>(out);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_rows(dtype, vb, [&](auto r) {
         using R = decltype(r);
+        using T_ = typename R::T;
         const long long vecs = (long long)K / R::N;
-        return cuda_status(launch_pdl(unsort_kernel<typename R::T, R::BYTES>, blocks_of((long long)M * vecs), 256u, 0, st,
-                                      a, rs, o, os, vecs, M, T, row_of_pair, weights));
+        const unsigned grid = blocks_of((long long)M * vecs);
+        if constexpr (sizeof(T_) == 4) {
+            if (out_dtype == VMOE_BF16)
+                return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, __nv_bfloat16>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
+            if (out_dtype == VMOE_F16)
+                return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, __half>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
+        }
+        return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, T_>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
     });
 }
 

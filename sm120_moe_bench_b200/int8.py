@@ -1,0 +1,193 @@
+"""8-bit integer products with a scale for each token and each output channel, dense and per expert.
+
+    w = quantize_int8(weight)                            # once: codes [N, K] and a scale per output channel
+    y = int8_linear(x, w)                                # quantises the rows of x, multiplies
+
+    w13, w2 = quantize_int8(gate_up), quantize_int8(down)    # [E, 2N, K] (gate rows first) and [E, K, N]
+    y = int8_experts(x, w13, w2, topk_ids, topk_weights)     # the whole expert layer
+
+The integer sums are exact, the scales are applied in f32 and the result is rounded once; a result does not depend on the
+batch around it.  These are inference operators: they have no gradient, and floating tensors that require one are refused
+while gradients are enabled.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import check, lib
+from .token_sort import DTYPE_CODES, TokenPlan, _on, _unsort, check_out, check_rows, plan_tokens
+
+MAX_K = 131071
+
+
+@dataclass(frozen=True, eq=False)
+class Int8Rows:
+    """Rows of 8-bit codes ``q`` int8 ``[..., rows, K]`` and a scale each, ``scale`` f32 ``[..., rows]``: row = q * scale.
+
+    A row's codes lie next to each other; rows (and the matrices of several experts) may have any stride.  Where address
+    and strides are multiples of 16 bytes the tensor cores read them as they are; ``quantize_int8`` makes them so."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    def __post_init__(self):
+        q, scale = self.q, self.scale
+        if not q.is_cuda or q.dtype != torch.int8 or q.dim() not in (2, 3):
+            raise ValueError("q must be an int8 CUDA tensor [rows, K] or [experts, rows, K]")
+        if scale.dtype != torch.float32 or scale.device != q.device or scale.shape != q.shape[:-1] or not scale.is_contiguous():
+            raise ValueError("scale must be a contiguous float32 tensor, one value for each row of q, on its device")
+        if q.shape[-1] > 1 and q.stride(-1) != 1:
+            raise ValueError("the codes of a row must lie next to each other")
+        if q.shape[-1] > MAX_K:
+            raise ValueError(f"rows of at most {MAX_K} codes")
+
+    def dequantize(self) -> torch.Tensor:
+        """f32 values."""
+        return self.q.float() * self.scale[..., None]
+
+
+def _no_grad(t: torch.Tensor, name: str) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the 8-bit operators have none")
+
+
+def _codes(rows: int, K: int, device) -> torch.Tensor:
+    """Rows that start on 16-byte boundaries, whatever K is."""
+    pitch = (K + 15) // 16 * 16
+    q = torch.empty(rows, pitch, dtype=torch.int8, device=device)
+    return q if pitch == K else q[:, :K]
+
+
+def _quantize(x, plan: TokenPlan | None = None, live: torch.Tensor | None = None):
+    M, K = x.shape
+    rows = M if plan is None else plan.rows
+    q = _codes(rows, K, x.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    with _on(x.device) as stream:
+        check(lib.vmoe_int8_quantize(x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, K, 0 if plan is None else plan.topk,
+                                     None if plan is None else plan.row_of_pair.data_ptr(), None if live is None else live.data_ptr(),
+                                     q.data_ptr(), max(q.stride(0), K), scale.data_ptr(), stream), "vmoe_int8_quantize")
+    return q, scale
+
+
+def quantize_int8(x: torch.Tensor, plan: TokenPlan | None = None) -> Int8Rows:
+    """bf16 / fp16 / f32 rows to 8-bit rows: ``scale = max|row| / 127``, codes = the exact ``127 * x / max|row|`` rounded to the
+    nearest integer (ties to even).  A row of zeros has scale 0; a row with an infinity or NaN has scale NaN, so that what
+    it is multiplied with becomes NaN.
+
+    ``x`` is ``[rows, K]``, or ``[E, rows, K]`` contiguous for the weights of several experts.  With ``plan`` the rows of ``x``
+    are tokens and the codes come sorted by expert, ``[M * T, K]`` (rows behind the last kept one are undefined)."""
+    _no_grad(x, "x")
+    if x.dim() == 3:
+        if plan is not None:
+            raise ValueError("a plan sorts token rows [M, K]")
+        if not x.is_contiguous():
+            raise ValueError("x must be contiguous")
+        E, N, K = x.shape
+        flat = quantize_int8(x.view(E * N, K))
+        return Int8Rows(flat.q.as_strided((E, N, K), (N * flat.q.stride(0), flat.q.stride(0), 1)), flat.scale.view(E, N))
+    check_rows(x, "x", None if plan is None else plan.tokens, None if plan is None else plan.expert_offsets.device)
+    if x.shape[1] > MAX_K:
+        raise ValueError(f"rows of at most {MAX_K} elements")
+    return Int8Rows(*_quantize(x, plan))
+
+
+def _matmul(q, scale, w: Int8Rows, N: int, offsets, swiglu: bool, zero_tail: bool, out):
+    M, K = q.shape
+    wq = w.q
+    grouped = wq.dim() == 3
+    with _on(q.device) as stream:
+        check(lib.vmoe_int8_matmul(q.data_ptr(), q.stride(0), scale.data_ptr(), M, wq.data_ptr(), wq.stride(-2),
+                                   wq.stride(0) if grouped else 0, w.scale.data_ptr(), N, K, wq.shape[0] if grouped else 1,
+                                   None if offsets is None else offsets.data_ptr(), swiglu, zero_tail, out.data_ptr(),
+                                   max(out.stride(0), N), DTYPE_CODES[out.dtype], stream), "vmoe_int8_matmul")
+    return out
+
+
+def _out_columns(w: Int8Rows, K: int, device, swiglu: bool, experts: int | None) -> int:
+    if w.q.device != device:
+        raise ValueError(f"the weights are on {w.q.device}, the rows on {device}")
+    if w.q.dim() != (2 if experts is None else 3):
+        raise ValueError("weights of several experts go with a plan, a single matrix goes without")
+    if experts is not None and w.q.shape[0] != experts:
+        raise ValueError(f"the plan has {experts} experts, the weights {w.q.shape[0]}")
+    if w.q.shape[-1] != K:
+        raise ValueError(f"rows of {K} codes times weights of {w.q.shape[-1]}")
+    n = w.q.shape[-2]
+    if swiglu and n % 2:
+        raise ValueError("swiglu needs gate and up rows")
+    if n == 0:
+        raise ValueError("the weights have no rows")
+    return n // 2 if swiglu else n
+
+
+def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swiglu: bool = False,
+                out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[m, n] = (a.q[m] . w.q[n]) * a.scale[m] * w.scale[n]``.
+
+    With ``plan`` the rows are sorted by expert (``quantize_int8(x, plan)``) and each meets its expert's matrix of ``w``
+    ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``).  ``swiglu``: ``w``
+    holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``, ``[M, N]``."""
+    if a.q.dim() != 2:
+        raise ValueError("a must be rows [M, K]")
+    if plan is not None and (a.q.shape[0] != plan.rows or plan.expert_offsets.device != a.q.device):
+        raise ValueError(f"the plan has {plan.rows} rows on {plan.expert_offsets.device}, a {a.q.shape[0]} on {a.q.device}")
+    N = _out_columns(w, a.q.shape[1], a.q.device, swiglu, None if plan is None else plan.num_experts)
+    if out is None:
+        if out_dtype not in DTYPE_CODES:
+            raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
+        y = torch.empty(a.q.shape[0], N, dtype=out_dtype, device=a.q.device)
+    else:
+        y = check_out(out, a.q.shape[0], out)
+        if out.device != a.q.device or out.shape[1] != N:
+            raise ValueError(f"out must have {N} columns on {a.q.device}")
+        _no_grad(out, "out")
+    return _matmul(a.q, a.scale, w, N, None if plan is None else plan.expert_offsets, swiglu, out is None, y)
+
+
+def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x [M, K]`` (bf16 / fp16 / f32) quantised row by row, times ``w [N, K]``: ``[M, N]`` in the type of ``x``."""
+    _no_grad(x, "x")
+    check_rows(x, "x")
+    N = _out_columns(w, x.shape[1], x.device, swiglu, None)
+    if out is None:
+        out = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
+    else:
+        check_rows(out, "out", x.shape[0], x.device)
+        if out.dtype != x.dtype or out.shape[1] != N or (x.shape[0] > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
+        _no_grad(out, "out")
+    q, scale = _quantize(x)
+    return _matmul(q, scale, w, N, None, swiglu, False, out)
+
+
+def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+                 expert_map: torch.Tensor | None = None) -> torch.Tensor:
+    """The expert layer on 8-bit weights: ``out[m] = sum_t weight[m, t] * w2[e] (silu(gate) * up)``, ``[gate; up] = w13[e] x[m]``.
+
+    ``x [M, K]`` bf16 / fp16 / f32; ``w13 [E, 2N, K]`` (gate rows first); ``w2 [E, K, N]``; ids int32 and weights f32 ``[M, T]``.
+    Tokens are quantised once and copied into expert order, the activations between the two products once more per row;
+    everything between is f32, and the sum is rounded once to the type of ``x``.  ``expert_map`` as in ``plan_tokens``."""
+    _no_grad(x, "x")
+    _no_grad(topk_weights, "topk_weights")
+    check_rows(x, "x", topk_ids.shape[0], topk_ids.device)
+    if w13.q.dim() != 3 or w2.q.dim() != 3:
+        raise ValueError("w13 and w2 hold one matrix per expert")
+    E, K = w13.q.shape[0], x.shape[1]
+    N = _out_columns(w13, K, x.device, True, E)
+    if _out_columns(w2, N, x.device, False, E) != K:
+        raise ValueError(f"w2 must be [{E}, {K}, {N}]")
+    if topk_weights.dtype != torch.float32 or topk_weights.shape != topk_ids.shape or topk_weights.device != x.device \
+            or not topk_weights.is_contiguous():
+        raise ValueError("topk_weights must be a contiguous float32 tensor of the shape of topk_ids")
+    plan = plan_tokens(topk_ids, E, expert_map)
+    kept = plan.expert_offsets[E:]
+    q, scale = _quantize(x, plan)
+    h = torch.empty(plan.rows, N, dtype=torch.float32, device=x.device)
+    _matmul(q, scale, w13, N, plan.expert_offsets, True, False, h)
+    q, scale = _quantize(h, None, kept)
+    y = torch.empty(plan.rows, K, dtype=torch.float32, device=x.device)
+    _matmul(q, scale, w2, K, plan.expert_offsets, False, False, y)
+    return _unsort(y, plan, topk_weights, torch.empty_like(x, memory_format=torch.contiguous_format))

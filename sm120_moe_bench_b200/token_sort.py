@@ -142,7 +142,7 @@ def _unsort(rows, plan: TokenPlan, weights=None, out=None):
     with _on(rows.device) as stream:
         check(lib.vmoe_unsort_tokens(rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype], plan.tokens, plan.topk, K,
                                      plan.row_of_pair.data_ptr(), None if weights is None else weights.data_ptr(), y.data_ptr(),
-                                     max(y.stride(0), K), stream), "vmoe_unsort_tokens")
+                                     max(y.stride(0), K), DTYPE_CODES[y.dtype], stream), "vmoe_unsort_tokens")
     return y
 
 

@@ -44,14 +44,15 @@ def test_sort_checks():
 def test_unsort_checks():
     lib, b = _lib(), ctypes.addressof(_buf())
 
-    def unsort(M=4, T=2, K=8, dtype=0, rows=b, rs=8, rp=b, out=b, os_=8):
-        return lib.vmoe_unsort_tokens(rows, rs, dtype, M, T, K, rp, None, out, os_, None)
+    def unsort(M=4, T=2, K=8, dtype=0, rows=b, rs=8, rp=b, out=b, os_=8, to=None):
+        return lib.vmoe_unsort_tokens(rows, rs, dtype, M, T, K, rp, None, out, os_, dtype if to is None else to, None)
 
     assert unsort(M=0) == 0 and unsort(K=0) == 0
     assert unsort(M=-1) == 2 and unsort(dtype=7) == 2 and unsort(os_=7) == 2 and unsort(rs=-1) == 2 and unsort(T=17) == 8
     for name in ("rows", "rp", "out"):
         assert unsort(**{name: None}) == 1, name
-    assert unsort(out=b + 1) == 3
+    assert unsort(out=b + 1) == 3 and unsort(dtype=2, rows=b + 2) == 3
+    assert unsort(to=1) == 2 and unsort(to=2) == 2 and unsort(dtype=2, to=3) == 2      # only f32 rows change their type
 
     def grad(M=4, T=2, E=4, K=8, dy=b, ds=8, rows=b, rs=8, off=b, rp=b, drows=b, gs=8, dw=b):
         return lib.vmoe_unsort_tokens_grad(dy, ds, rows, rs, 0, M, T, E, K, off, rp, None, drows, gs, dw, None)
