@@ -322,8 +322,10 @@ int vmoe_permute_noalloc(const int32_t* topk_ids, const float* topk_weights,
  * Limits: T <= 16, E <= 8192, M * T < 2^31 - 1024 (VMOE_ERR_LIMIT).  Strides are in elements. */
 enum vmoe_dtype { VMOE_BF16 = 0, VMOE_F16 = 1, VMOE_F32 = 2 };
 
+size_t vmoe_plan_scratch_bytes(int32_t M, int32_t T, int32_t E);      /* 0 up to 4096 pairs */
 int vmoe_plan_tokens(const int32_t* topk_ids, const int32_t* expert_map, int32_t map_len, int32_t M, int32_t T, int32_t E,
-                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* stream);
+                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* scratch, size_t scratch_bytes,
+                     void* stream);
 
 /* rows[r] = x[pair_of_row[r] / T] for every kept row; zero_tail != 0: the rows behind them, up to M * T, become zero
  * (otherwise they are left as they were). */
@@ -365,6 +367,10 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
 int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, int32_t M, const int8_t* w, int64_t w_stride,
                      int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
                      int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream);
+
+/* Status word of the 8-bit products on the current device: VMOE_OK, or VMOE_ERR_TIMEOUT when a bounded wait inside one of
+ * them ran out since the last reading (that product's output is not complete).  Synchronises the stream, clears the word. */
+int vmoe_int8_read_status(void* stream);
 
 #ifdef __cplusplus
 }

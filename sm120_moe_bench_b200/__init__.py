@@ -12,5 +12,5 @@ Public surface:
 from . import _lib  # noqa: F401  (fails loudly when the CUDA library is absent)
 from .ops import (MoEShape, MoEWeights, Workspace, build_tables, dequantize, fused_moe,  # noqa: F401
                   quantize, route)
-from .int8 import Int8Rows, int8_experts, int8_linear, int8_matmul, quantize_int8  # noqa: F401
+from .int8 import Int8Rows, int8_experts, int8_linear, int8_matmul, int8_status, quantize_int8  # noqa: F401
 from .token_sort import TokenPlan, plan_tokens, sort_tokens, unsort_tokens  # noqa: F401

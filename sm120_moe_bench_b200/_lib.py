@@ -86,7 +86,8 @@ SIGNATURES = {
     "vmoe_ep_read_status": (C.c_int, [C.POINTER(VmoeEpCtx), C.POINTER(VmoeShape), _P, _P]),
     "vmoe_permute_noalloc": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                        _P, _P, _P, _P, _P, _P]),
-    "vmoe_plan_tokens": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
+    "vmoe_plan_scratch_bytes": (C.c_size_t, [C.c_int32, C.c_int32, C.c_int32]),
+    "vmoe_plan_tokens": (C.c_int, [_P, _P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P, C.c_size_t, _P]),
     "vmoe_sort_tokens": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, C.c_int32,
                                    _P, C.c_int64, _P]),
     "vmoe_unsort_tokens": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, C.c_int32,
@@ -96,6 +97,7 @@ SIGNATURES = {
     "vmoe_int8_quantize": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P, _P]),
     "vmoe_int8_matmul": (C.c_int, [_P, C.c_int64, _P, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P,
                                    C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P]),
+    "vmoe_int8_read_status": (C.c_int, [_P]),
 }
 
 

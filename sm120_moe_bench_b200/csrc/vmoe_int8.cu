@@ -1,4 +1,4 @@
-// 8-bit integer rows: the row quantiser and the product's entry point.
+// 8-bit integer rows: the row quantiser and the product's entry point.  (No pointer is __restrict__: see vmoe_sort.cu.)
 #include "vmoe_int8.cuh"
 
 namespace vmoe {
@@ -19,8 +19,8 @@ __device__ __forceinline__ int i8_code(float x, float inv, float amax) {
 
 template <typename T_, int VB, int WPR>
 __global__ void __launch_bounds__(256)
-i8_quantize_kernel(const uint8_t* __restrict__ x, long long x_stride, long long rows, int vecs, int T, const int32_t* __restrict__ row_of_pair,
-                   const int32_t* __restrict__ live, int8_t* __restrict__ q, long long q_stride, float* __restrict__ scales) {
+i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vecs, int T, const int32_t* row_of_pair,
+                   const int32_t* live, int8_t* q, long long q_stride, float* scales) {
     using R = RowVec<T_, VB>;
     __shared__ uint32_t s_max[8];
     pdl_begin();
@@ -218,7 +218,15 @@ int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, in
     p.w = w; p.w_stride = w_stride; p.w_expert_stride = w_expert_stride; p.w_scale = w_scale;
     p.out = out; p.out_stride = out_stride; p.offsets = expert_offsets;
     p.M = M; p.N = N; p.K = K; p.E = E; p.wrows = swiglu ? 2 * N : N; p.swiglu = swiglu; p.out_dtype = out_dtype; p.zero_tail = zero_tail;
-    return launch_i8_tile(p, static_cast<cudaStream_t>(stream));
+    if (M == 1) p.a_stride = (K + 15) / 16 * 16;             // the stride of a single row says nothing
+    if (p.wrows == 1) p.w_stride = (K + 15) / 16 * 16;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!i8_tc_ok(p) || E > I8_TC_MAX_EXPERTS) return launch_i8_tile(p, st);
+    if (!expert_offsets) {
+        const long long items = (M + 255LL) / 256 * ((N + (swiglu ? 63LL : 127LL)) / (swiglu ? 64 : 128));
+        if (items < 148) return launch_i8_split(p, st);
+    }
+    return launch_i8_tc(p, st);
 }
 
 }  // extern "C"

@@ -29,4 +29,10 @@ __device__ __forceinline__ void i8_store(void* out, long long at, int dtype, flo
     else static_cast<__half*>(out)[at] = __float2half_rn(v);
 }
 
+// tensor-core kernels (vmoe_int8_tc.cu)
+constexpr int I8_TC_MAX_EXPERTS = 16384;                 // their tables lie in shared memory
+bool i8_tc_ok(const I8Problem& p);                       // addresses and strides are multiples of 16 bytes
+int  launch_i8_tc(const I8Problem& p, cudaStream_t st);
+int  launch_i8_split(const I8Problem& p, cudaStream_t st);   // dense only
+
 }  // namespace vmoe

@@ -1,0 +1,564 @@
+// The 8-bit integer product on the tensor cores (tcgen05.mma kind::i8, s8 x s8 -> s32, accumulators in tensor memory).
+//
+// In both kernels the MMA's rows (operand A) are output channels and its columns (operand B) are tokens, so the number of
+// tokens of an item is free in steps of 16 or 32: an expert with 5 rows costs 32 columns, one with 320 costs 192 + 128, and a
+// decode batch streams every weight once.  A thread of the epilogue owns a channel; 32 lanes store 32 neighbours of a row.
+// swiglu: the 32 channels of a TMEM lane quadrant are 16 gate rows followed by the 16 matching up rows.
+//
+//   i8_tc_kernel      persistent, grouped or large: 128 channels x up to 256 tokens per item
+//   i8_split_kernel   dense products too small to fill the GPU that way: 128 channels x up to 128 tokens per CTA, the
+//                     reduction split over a cluster, partial sums met in distributed shared memory (exact: integers)
+#include "vmoe_int8.cuh"
+#include "vmoe_tc_common.cuh"
+
+#include <string.h>
+
+namespace vmoe {
+
+// A wait that ran out leaves its status here (read and cleared by vmoe_int8_read_status).
+__device__ int g_i8_status;
+
+__device__ __forceinline__ uint32_t i8_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void i8_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t i8_cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void i8_load_3d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void i8_mma(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ uint32_t i8_idesc(int m, int n) {
+    // accumulator s32 (2), operands signed 8-bit (1), both K-major
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+constexpr int I8_KB = 128;                                // bytes of K per stage: one swizzled row
+constexpr int I8_A_BYTES = 128 * I8_KB;                   // 128 channels
+constexpr int I8_BOX_BIG = 64, I8_BOX_SMALL = 16;         // token rows per copy
+
+// ----------------------------------------------------------------------------------------------------- persistent
+constexpr int I8P_MAX_STAGES = 8;
+constexpr int I8P_EPI_WARPS = 8;
+constexpr int I8P_THREADS = 64 + 32 * I8P_EPI_WARPS;
+constexpr int I8P_TOKENS = 256;                           // tokens per item at most (UMMA N): two accumulators fill tensor memory
+
+struct I8Shared {
+    uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
+    uint64_t tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    int blocks;                                           // token blocks of all experts
+    int pad;
+    float row_scale[I8P_EPI_WARPS][I8P_TOKENS / 2];       // of the item in hand, each epilogue warp its own tokens
+};
+
+struct I8TcParams {
+    CUtensorMap map_w;                                    // [E, channels, K]
+    CUtensorMap map_a64, map_a16;                         // token rows [M, K] in boxes of 64 and 16 (split: of the tile's tokens)
+    I8Problem p;
+    int kblocks, ctiles, stages, tokens;                  // tokens: most of an item
+};
+
+struct I8Item { int expert, ctile, row0, rows, n; };
+__device__ __forceinline__ int i8_blocks(int count, int most) { return (max(count, 0) + most - 1) / most; }
+__device__ __forceinline__ I8Item i8_item(const I8TcParams& P, const int* s_pref, const int* s_off, long long item) {
+    I8Item r;
+    const int block = (int)(item / P.ctiles);
+    r.ctile = (int)(item - (long long)block * P.ctiles);
+    int lo = 0, hi = P.p.E;                               // s_pref[lo] <= block < s_pref[lo + 1]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_pref[mid] <= block) lo = mid; else hi = mid;
+    }
+    r.expert = lo;
+    const int count = s_off[lo + 1] - s_off[lo], nb = s_pref[lo + 1] - s_pref[lo], j = block - s_pref[lo];
+    r.n = min(((count + nb - 1) / nb + 15) & ~15, P.tokens);      // the expert's rows in equal blocks
+    if (r.n > 16) r.n = (r.n + 31) & ~31;                 // two epilogue warps share the columns in chunks of 16
+    r.row0 = s_off[lo] + j * r.n;
+    r.rows = min(r.n, max(s_off[lo + 1] - r.row0, 0));
+    return r;
+}
+
+__device__ __forceinline__ void i8_abort(int* flag) {
+    atomicExch(&g_i8_status, VMOE_ERR_TIMEOUT);
+    atomicExch(flag, 1);
+}
+// After a wait that ran out: the copies of the last stages have to land (or their own limit pass) before the CTA leaves.
+__device__ __forceinline__ void i8_drain(uint64_t* full, uint32_t issued, int stages) {
+    for (uint32_t g = issued > (uint32_t)stages ? issued - stages : 0; g < issued; ++g) mbar_wait(&full[g % stages], (g / stages) & 1);
+}
+
+template <bool SWIGLU>
+__global__ void __launch_bounds__(I8P_THREADS, 1)
+i8_tc_kernel(const __grid_constant__ I8TcParams P) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int stage_bytes = I8_A_BYTES + P.tokens * I8_KB;
+    I8Shared* sh = reinterpret_cast<I8Shared*>(smem + (size_t)P.stages * stage_bytes);
+    int* s_pref = reinterpret_cast<int*>(sh + 1);         // [E + 1] token blocks of the experts in front
+    int* s_off = s_pref + P.p.E + 1;                      // [E + 1] first row of each expert
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const I8Problem& p = P.p;
+    const int stages = P.stages;
+
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh->tmem_full[i], 1); mbar_init(&sh->tmem_empty[i], I8P_EPI_WARPS); }
+        sh->abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(TC_TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    pdl_begin();
+
+    const int E = p.E;
+    for (int e = tid; e <= E; e += I8P_THREADS) s_off[e] = p.offsets ? min(max(p.offsets[e], 0), p.M) : (e ? p.M : 0);
+    __syncthreads();
+    if (warp == 0) {                  // exclusive prefix of the experts' token blocks
+        const int per = (E + 31) / 32;
+        int sum = 0;
+        for (int k = 0; k < per; ++k) { const int e = lane * per + k; if (e < E) sum += i8_blocks(s_off[e + 1] - s_off[e], P.tokens); }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int t = __shfl_up_sync(0xffffffffu, incl, o); if (lane >= o) incl += t; }
+        int run = incl - sum;
+        for (int k = 0; k < per; ++k) {
+            const int e = lane * per + k;
+            if (e < E) { s_pref[e] = run; run += i8_blocks(s_off[e + 1] - s_off[e], P.tokens); }
+        }
+        if (lane == 31) { s_pref[E] = incl; sh->blocks = incl; }
+    }
+    __syncthreads();
+    const long long total = (long long)sh->blocks * P.ctiles;
+    const int kblocks = P.kblocks;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------- producer: 128 channels and the item's token rows
+        const bool leader = elect_one();
+        uint32_t g = 0;
+        bool ok = true;
+        for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
+            const I8Item u = i8_item(P, s_pref, s_off, item);
+            const int ch = u.ctile * (SWIGLU ? 64 : 128);
+            for (int kb = 0; kb < kblocks; ++kb) {
+                const int slot = g % stages;
+                bool w = true;
+                if (g >= (uint32_t)stages) w = mbar_wait(&sh->empty[slot], ((g / stages) - 1) & 1);
+                if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+                if (*reinterpret_cast<volatile int*>(&sh->abort_flag)) { ok = false; break; }
+                uint8_t* st = smem + (size_t)slot * stage_bytes;
+                uint64_t* bar = &sh->full[slot];
+                if (leader) {
+                    mbar_arrive_expect_tx(bar, I8_A_BYTES + u.n * I8_KB);
+                    if (SWIGLU) {
+#pragma unroll
+                        for (int b = 0; b < 8; ++b)       // 16 gate rows, then the 16 matching up rows, per lane quadrant
+                            i8_load_3d(st + b * 16 * I8_KB, &P.map_w, kb * I8_KB, (b & 1) * p.N + ch + (b >> 1) * 16, u.expert, bar);
+                    } else {
+                        i8_load_3d(st, &P.map_w, kb * I8_KB, ch, u.expert, bar);
+                    }
+                    int r = 0;
+                    for (; r + I8_BOX_BIG <= u.n; r += I8_BOX_BIG)
+                        tma_load_2d(st + I8_A_BYTES + r * I8_KB, &P.map_a64, kb * I8_KB, u.row0 + r, bar);
+                    for (; r < u.n; r += I8_BOX_SMALL)
+                        tma_load_2d(st + I8_A_BYTES + r * I8_KB, &P.map_a16, kb * I8_KB, u.row0 + r, bar);
+                }
+                __syncwarp();
+                ++g;
+            }
+        }
+        if (!ok) {
+            if (leader) i8_abort(&sh->abort_flag);
+            __syncwarp();
+            i8_drain(sh->full, g, stages);
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA issuer (warp-uniform loop, one elected lane
+        // issues); two accumulators of 256 columns take turns
+        const bool leader = elect_one();
+        uint32_t g = 0, it = 0;
+        bool ok = true;
+        const uint32_t smem16 = smem_u32(smem) >> 4;
+        for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
+            const I8Item u = i8_item(P, s_pref, s_off, item);
+            const uint32_t idesc = i8_idesc(128, u.n);
+            const uint32_t buf = it & 1, acc = tmem + buf * I8P_TOKENS;
+            bool w = true;
+            if (it >= 2) w = mbar_wait(&sh->tmem_empty[buf], ((it >> 1) - 1) & 1);
+            if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+            for (int kb = 0; kb < kblocks; ++kb) {
+                const int slot = g % stages;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[slot], (g / stages) & 1))) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t st16 = smem16 + slot * (stage_bytes >> 4);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t da = make_desc(st16 + ((j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                    const uint64_t db = make_desc(st16 + ((I8_A_BYTES + j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                    if (leader) i8_mma(acc, da, db, idesc, (kb | j) ? 1u : 0u);
+                }
+                if (leader) tc_commit(&sh->empty[slot]);
+                ++g;
+            }
+            if (!ok) break;
+            if (leader) tc_commit(&sh->tmem_full[buf]);
+            ++it;
+        }
+        if (!ok && leader) i8_abort(&sh->abort_flag);
+        __syncwarp();
+    } else {
+        // ------------------------------------------------------------- epilogue: a lane is a channel, two warps per lane
+        // quadrant take half of the item's tokens each
+        const int quad = warp & 3, sub = (warp - 2) >> 2, et = tid - 64;
+        if (p.offsets && p.zero_tail) {
+            for (long long m = (long long)s_off[E] + blockIdx.x; m < p.M; m += gridDim.x)
+                for (int n = et; n < p.N; n += 32 * I8P_EPI_WARPS) i8_store(p.out, m * p.out_stride + n, p.out_dtype, 0.f);
+        }
+        uint32_t it = 0;
+        for (long long item = blockIdx.x; item < total; item += gridDim.x, ++it) {
+            const I8Item u = i8_item(P, s_pref, s_off, item);
+            const uint32_t buf = it & 1;
+            const int half = u.n > 16 ? u.n >> 1 : 16;    // an item of 16 columns is the first warp's alone
+            const int c_first = sub * half, c_end = min(c_first + half, u.n);
+            float* rs = sh->row_scale[warp - 2];
+            __syncwarp();
+            for (int c = c_first + lane; c < c_end; c += 32) rs[c - c_first] = c < u.rows ? p.a_scale[u.row0 + c] : 0.f;
+            __syncwarp();
+            const int ch = SWIGLU ? u.ctile * 64 + quad * 16 + (lane & 15) : u.ctile * 128 + quad * 32 + lane;
+            const float sw = ch < p.N ? p.w_scale[(long long)u.expert * p.wrows + (SWIGLU ? (lane >> 4) * p.N : 0) + ch] : 0.f;
+            const bool w = mbar_wait(&sh->tmem_full[buf], (it >> 1) & 1);
+            if (!__all_sync(0xffffffffu, w)) { if (lane == 0) i8_abort(&sh->abort_flag); break; }
+            tc_fence_after();
+            const uint32_t tacc = tmem + buf * I8P_TOKENS + ((uint32_t)(quad * 32) << 16);
+            for (int c = c_first; c < c_end; c += 16) {
+                const float* cs = rs + (c - c_first);
+                uint32_t v[16];
+                __syncwarp();
+                tc_ld16(tacc + c, v);
+                tc_ld_wait();
+                if (SWIGLU) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        // lanes 0-15 hold gate values and take token c + i, lanes 16-31 hold up values and take c + i + 1
+                        const bool lo = lane < 16;
+                        const float v0 = i8_scaled((int)v[i], cs[i], sw), v1 = i8_scaled((int)v[i + 1], cs[i + 1], sw);
+                        const float other = __shfl_xor_sync(0xffffffffu, lo ? v1 : v0, 16);
+                        const float gate = lo ? v0 : other, up = lo ? other : v1;
+                        const int j = c + i + (lo ? 0 : 1);
+                        if (j < u.rows && ch < p.N)
+                            i8_store(p.out, (long long)(u.row0 + j) * p.out_stride + ch, p.out_dtype, up * i8_silu(gate));
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = c + i;
+                        if (j < u.rows && ch < p.N)
+                            i8_store(p.out, (long long)(u.row0 + j) * p.out_stride + ch, p.out_dtype, i8_scaled((int)v[i], cs[i], sw));
+                    }
+                }
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(&sh->tmem_empty[buf]);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_TMEM_COLS) : "memory");
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------- split
+constexpr int I8S_THREADS = 192;                          // producer, MMA issuer, four epilogue warps
+constexpr int I8S_TOKENS = 128;                           // tokens per tile at most
+constexpr int I8S_MAX_STAGES = 8;
+constexpr int I8S_SMEM = 200 * 1024;
+constexpr size_t I8S_SMEM_LEAST = 116 * 1024;
+
+struct I8SplitShared {
+    uint64_t full[I8S_MAX_STAGES], empty[I8S_MAX_STAGES];
+    uint64_t done;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+__device__ __forceinline__ int4 i8_ld_peer(uint32_t addr) {
+    int4 r;
+    asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
+    return r;
+}
+
+template <bool SWIGLU>
+__global__ void __launch_bounds__(I8S_THREADS, 1)
+i8_split_kernel(const __grid_constant__ I8TcParams P) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ I8SplitShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const I8Problem& p = P.p;
+    const int split = (int)gridDim.x, rank = (int)blockIdx.x, n = P.tokens, stages = P.stages;
+    const int stage_bytes = I8_A_BYTES + n * I8_KB;
+    const int ch0 = (int)blockIdx.y * (SWIGLU ? 64 : 128), tok0 = (int)blockIdx.z * n;
+    const int kb0 = (int)((long long)P.kblocks * rank / split), kb1 = (int)((long long)P.kblocks * (rank + 1) / split);
+
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+        mbar_init(&sh.done, 1);
+        sh.abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_base)), "r"(I8S_TOKENS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+
+    if (warp == 0) {
+        const bool leader = elect_one();
+        bool ok = true;
+        uint32_t issued = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int g = kb - kb0, slot = g % stages;
+            bool w = true;
+            if (g >= stages) w = mbar_wait(&sh.empty[slot], ((g / stages) - 1) & 1);
+            if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
+            uint8_t* st = smem + (size_t)slot * stage_bytes;
+            if (leader) {
+                mbar_arrive_expect_tx(&sh.full[slot], stage_bytes);
+                if (SWIGLU) {
+#pragma unroll
+                    for (int b = 0; b < 8; ++b)
+                        i8_load_3d(st + b * 16 * I8_KB, &P.map_w, kb * I8_KB, (b & 1) * p.N + ch0 + (b >> 1) * 16, 0, &sh.full[slot]);
+                } else {
+                    i8_load_3d(st, &P.map_w, kb * I8_KB, ch0, 0, &sh.full[slot]);
+                }
+                tma_load_2d(st + I8_A_BYTES, &P.map_a64, kb * I8_KB, tok0, &sh.full[slot]);
+            }
+            ++issued;
+        }
+        if (!ok) {
+            if (leader) i8_abort(&sh.abort_flag);
+            i8_drain(sh.full, issued, stages);
+        }
+    } else if (warp == 1) {
+        const bool leader = elect_one();
+        bool ok = true;
+        const uint32_t smem16 = smem_u32(smem) >> 4, idesc = i8_idesc(128, n);
+        for (int kb = kb0; kb < kb1; ++kb) {
+            const int g = kb - kb0, slot = g % stages;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[slot], (g / stages) & 1))) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t st16 = smem16 + slot * (stage_bytes >> 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t da = make_desc(st16 + ((j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                const uint64_t db = make_desc(st16 + ((I8_A_BYTES + j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                if (leader) i8_mma(tmem, da, db, idesc, (g | j) ? 1u : 0u);
+            }
+            if (leader) tc_commit(&sh.empty[slot]);
+        }
+        if (ok && leader) tc_commit(&sh.done);
+        if (!ok && leader) i8_abort(&sh.abort_flag);
+    } else {
+        // partial sums to shared memory, [token][channel]; the stages are free once every MMA has completed
+        const int quad = warp & 3;
+        if (!mbar_wait(&sh.done, 0)) {
+            if (lane == 0) i8_abort(&sh.abort_flag);
+        } else {
+            tc_fence_after();
+            int* part = reinterpret_cast<int*>(smem) + quad * 32 + lane;
+            for (int c = 0; c < n; c += 16) {
+                uint32_t v[16];
+                tc_ld16(tmem + c + ((uint32_t)(quad * 32) << 16), v);
+                tc_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part[(c + i) * 128] = (int)v[i];
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) i8_cluster_sync();
+    // The CTAs of the cluster share the tile's tokens out; a thread owns four neighbouring channels of a token.
+    const uint32_t base = smem_u32(smem);
+    const int rows = min(n, p.M - tok0), per = (n + split - 1) / split;
+    const int t_end = min(rows, (rank + 1) * per);
+    constexpr int QUADS = SWIGLU ? 16 : 32;               // groups of four channels per token
+    const bool vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && p.N % 4 == 0;
+    if (!sh.abort_flag)
+        for (int i = tid + rank * per * QUADS; i < t_end * QUADS; i += I8S_THREADS) {
+            const int t = i / QUADS, c = (i % QUADS) * 4, ch = ch0 + c;
+            if (ch >= p.N) continue;
+            int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
+            const uint32_t at = base + (uint32_t)(t * 128 + (SWIGLU ? (c >> 4) * 32 + (c & 15) : c)) * 4;
+            for (int r = 0; r < split; ++r) {
+                const uint32_t a = i8_cluster_addr(at, r);
+                const int4 x = i8_ld_peer(a);
+                s0[0] += x.x; s0[1] += x.y; s0[2] += x.z; s0[3] += x.w;
+                if (SWIGLU) {
+                    const int4 y = i8_ld_peer(a + 64);
+                    s1[0] += y.x; s1[1] += y.y; s1[2] += y.z; s1[3] += y.w;
+                }
+            }
+            const float sa = p.a_scale[tok0 + t];
+            float o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int n_ = min(ch + k, p.N - 1);
+                o[k] = i8_scaled(s0[k], sa, p.w_scale[n_]);
+                if (SWIGLU) o[k] = i8_scaled(s1[k], sa, p.w_scale[p.N + n_]) * i8_silu(o[k]);
+            }
+            const long long at_out = (long long)(tok0 + t) * p.out_stride + ch;
+            if (vec && p.out_dtype == VMOE_F32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at_out) = make_float4(o[0], o[1], o[2], o[3]);
+            } else if (vec) {
+                union { uint2 w; __nv_bfloat16 b[4]; __half h[4]; } q;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (p.out_dtype == VMOE_BF16) q.b[k] = __float2bfloat16_rn(o[k]); else q.h[k] = __float2half_rn(o[k]);
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at_out) = q.w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (ch + k < p.N) i8_store(p.out, at_out + k, p.out_dtype, o[k]);
+            }
+        }
+    __syncthreads();
+    if (split > 1) i8_cluster_sync();                     // nobody leaves while its partial sums are read
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(I8S_TOKENS) : "memory");
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------- host
+static int i8_map_w(CUtensorMap* map, const I8Problem& p, uint32_t box_rows) {
+    const unsigned long long dims[3] = {(unsigned long long)p.K, (unsigned long long)p.wrows, (unsigned long long)p.E};
+    const unsigned long long experts = p.E > 1 ? (unsigned long long)p.w_expert_stride : (unsigned long long)p.w_stride * p.wrows;
+    const unsigned long long strides[2] = {(unsigned long long)p.w_stride, experts};
+    const uint32_t box[3] = {I8_KB, box_rows, 1};
+    return encode_byte_map(map, p.w, 3, dims, strides, box);
+}
+static int i8_map_a(CUtensorMap* map, const I8Problem& p, uint32_t box_rows) {
+    const unsigned long long dims[2] = {(unsigned long long)p.K, (unsigned long long)p.M};
+    const unsigned long long strides[1] = {(unsigned long long)p.a_stride};
+    const uint32_t box[2] = {I8_KB, box_rows};
+    return encode_byte_map(map, p.a, 2, dims, strides, box);
+}
+
+// Whether the copies of the tensor-core kernels can read the operands as they are.
+bool i8_tc_ok(const I8Problem& p) {
+    const unsigned long long all = (unsigned long long)(uintptr_t)p.a | (unsigned long long)p.a_stride | (unsigned long long)(uintptr_t)p.w |
+                                   (unsigned long long)p.w_stride | (p.E > 1 ? (unsigned long long)p.w_expert_stride : 0ULL);
+    if (all & 15) return false;
+    if (p.K < 1 || p.a_stride < p.K || p.w_stride < p.K) return false;
+    return p.E == 1 || p.w_expert_stride >= p.w_stride * p.wrows;
+}
+
+constexpr size_t I8P_SMEM = 227 * 1024;
+
+template <bool SWIGLU>
+static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
+    I8TcParams P;
+    memset(&P, 0, sizeof(P));
+    P.p = p;
+    P.kblocks = (p.K + I8_KB - 1) / I8_KB;
+    P.ctiles = SWIGLU ? (p.N + 63) / 64 : (p.N + 127) / 128;
+    // Few rows per expert: items of at most 64 tokens, so that the stages hold more weight bytes in flight.
+    P.tokens = p.E > 1 && (long long)p.M <= 32LL * p.E ? 64 : I8P_TOKENS;
+    const size_t stage = I8_A_BYTES + (size_t)P.tokens * I8_KB;
+    const size_t rest = sizeof(I8Shared) + 2 * ((size_t)p.E + 1) * sizeof(int) + 1024;
+    P.stages = I8P_MAX_STAGES;
+    while (P.stages > 2 && P.stages * stage + rest > I8P_SMEM) --P.stages;
+    const size_t smem = P.stages * stage + rest;
+    if (smem > I8P_SMEM) return VMOE_ERR_LIMIT;
+    int rc;
+    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 16 : 128))) return rc;
+    if ((rc = i8_map_a(&P.map_a64, p, I8_BOX_BIG))) return rc;
+    if ((rc = i8_map_a(&P.map_a16, p, I8_BOX_SMALL))) return rc;
+    // one CTA per SM (tc_sm_count), but no more than there can be items
+    const long long blocks = ((long long)p.M + P.tokens - 1) / P.tokens + (p.E > 1 ? (p.E < p.M ? p.E : p.M) : 0);
+    const long long items = blocks * P.ctiles;
+    const unsigned grid = (unsigned)(items < tc_sm_count() ? items : tc_sm_count());
+    if (cudaFuncSetAttribute(i8_tc_kernel<SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8P_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    return cuda_status(launch_pdl(i8_tc_kernel<SWIGLU>, grid, (unsigned)I8P_THREADS, smem, st, P));
+}
+int launch_i8_tc(const I8Problem& p, cudaStream_t st) { return p.swiglu ? launch_i8_tc_t<true>(p, st) : launch_i8_tc_t<false>(p, st); }
+
+template <bool SWIGLU>
+static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
+    I8TcParams P;
+    memset(&P, 0, sizeof(P));
+    P.p = p;
+    P.kblocks = (p.K + I8_KB - 1) / I8_KB;
+    P.ctiles = SWIGLU ? (p.N + 63) / 64 : (p.N + 127) / 128;
+    const int ttiles = (p.M + I8S_TOKENS - 1) / I8S_TOKENS;
+    P.tokens = ((p.M + ttiles - 1) / ttiles + 15) & ~15;
+    if (P.ctiles > 65535 || ttiles > 65535) return VMOE_ERR_LIMIT;
+    const long long tiles = (long long)P.ctiles * ttiles;
+    int split = 1;
+    while (split < 8 && 2 * split * tiles <= 148 && 2 * split <= P.kblocks) split *= 2;
+    const size_t stage = I8_A_BYTES + (size_t)P.tokens * I8_KB;
+    const int per = (P.kblocks + split - 1) / split;
+    P.stages = (int)((I8S_SMEM - 1024) / stage);
+    if (P.stages > I8S_MAX_STAGES) P.stages = I8S_MAX_STAGES;
+    if (P.stages > per) P.stages = per;
+    size_t smem = P.stages * stage;
+    const size_t part = (size_t)P.tokens * 128 * sizeof(int);
+    if (smem < part) smem = part;
+    smem += 1024;
+    // More than half of an SM's shared memory: one CTA per SM.  CTAs that wait for tensor memory which a CTA of another
+    // cluster holds, while that one waits for its own cluster, could otherwise wait in a circle.
+    if (smem < I8S_SMEM_LEAST) smem = I8S_SMEM_LEAST;
+    int rc;
+    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 16 : 128))) return rc;
+    if ((rc = i8_map_a(&P.map_a64, p, (uint32_t)P.tokens))) return rc;
+    if (cudaFuncSetAttribute(i8_split_kernel<SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8S_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)split, (unsigned)P.ctiles, (unsigned)ttiles); cfg.blockDim = dim3(I8S_THREADS);
+    cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    // in plain stream order: a cluster kernel here neither starts under its predecessor nor lets its successor start early
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, i8_split_kernel<SWIGLU>, P));
+}
+int launch_i8_split(const I8Problem& p, cudaStream_t st) { return p.swiglu ? launch_i8_split_t<true>(p, st) : launch_i8_split_t<false>(p, st); }
+
+}  // namespace vmoe
+
+extern "C" int vmoe_int8_read_status(void* stream) {
+    int v = 0;
+    const int zero = 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (cudaMemcpyFromSymbolAsync(&v, vmoe::g_i8_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return VMOE_ERR_CUDA;
+    if (cudaStreamSynchronize(st) != cudaSuccess) return VMOE_ERR_CUDA;
+    if (v != 0) cudaMemcpyToSymbolAsync(vmoe::g_i8_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
+    return v;
+}

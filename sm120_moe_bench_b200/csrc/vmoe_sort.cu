@@ -8,37 +8,31 @@
 // Unlike the tables inside the layer's workspace (vmoe_phases.cuh: one bit per expert and token) a token may name an
 // expert twice here; each pair has its own row.  All sums run over t in ascending order in f32 and are rounded once;
 // nothing is summed with atomics, so every result is reproducible bit for bit.
+//
+// No pointer is __restrict__: these kernels may start while the kernel that writes their inputs still runs
+// (pdl_begin), and loads through the non-coherent path are only defined for data that does not change meanwhile.
 #include "vmoe_common.cuh"
 #include "vmoe_rows.cuh"
 
 namespace vmoe {
 
 // ---------------------------------------------------------------------------------
-// Plan: a stable counting sort by one CTA, or by one cluster of eight CTAs whose totals meet in distributed shared
-// memory -- one launch at every size, no global scratch.  Each warp owns a contiguous run of pairs.  Pass 1 counts
-// them per expert into the warp's own row of counters; sums over warps, CTAs and experts turn the counters into the
-// first row of (expert, warp); pass 2 walks the run again, 32 pairs at a time: __match_any_sync gives a pair's rank
-// among the lanes with its expert.
+// Plan: a stable counting sort.  Each warp owns a contiguous run of pairs.  Pass 1 counts them per expert into the warp's
+// own row of counters; sums over warps, CTAs and experts turn the counters into the first row of (expert, warp); pass 2
+// walks the run again, 32 pairs at a time: __match_any_sync gives a pair's rank among the lanes with its expert.
+// Up to 4096 pairs one CTA does it all.  Above, every CTA needs the others' counts: a first launch leaves them in the
+// caller's scratch [CTAs][E], the second reads them (a few times E words each) and places its own run.
 // ---------------------------------------------------------------------------------
 constexpr int PLAN_MAX_EXPERTS = 8192;
-constexpr int PLAN_CLUSTER = 8;
 constexpr int PLAN_ONE_CTA_PAIRS = 4096;
+constexpr int PLAN_PAIRS_PER_CTA = 2048;
+constexpr int PLAN_MAX_CTAS = 64;
 constexpr int PLAN_SMEM = 200 * 1024;
 
-__device__ __forceinline__ uint32_t plan_cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void plan_cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ int plan_peer_word(const int* p, uint32_t rank) {
-    uint32_t a;
-    int v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
+static int plan_ctas(long long pairs) {
+    if (pairs <= PLAN_ONE_CTA_PAIRS) return 1;
+    const long long n = (pairs + PLAN_PAIRS_PER_CTA - 1) / PLAN_PAIRS_PER_CTA;
+    return (int)(n < PLAN_MAX_CTAS ? n : PLAN_MAX_CTAS);
 }
 
 __device__ __forceinline__ int plan_expert(const int32_t* ids, const int32_t* expert_map, int map_len, int E, long long p, long long end) {
@@ -48,18 +42,33 @@ __device__ __forceinline__ int plan_expert(const int32_t* ids, const int32_t* ex
     return (e >= 0 && e < E) ? e : -1;
 }
 
-template <int CTAS>
 __global__ void __launch_bounds__(1024)
-plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ expert_map, int map_len, int P, int E, int run,
-            int32_t* __restrict__ offsets, int32_t* __restrict__ row_of_pair, int32_t* __restrict__ pair_of_row) {
+plan_count_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, int E, int per_cta,
+                  int32_t* counts) {
+    extern __shared__ int s_plan[];
+    for (int e = threadIdx.x; e < E; e += blockDim.x) s_plan[e] = 0;
+    __syncthreads();
+    pdl_begin();
+    const long long first = (long long)blockIdx.x * per_cta, end = min(first + per_cta, (long long)P);
+    for (long long p = first + threadIdx.x; p < end; p += blockDim.x) {
+        const int e = plan_expert(ids, expert_map, map_len, E, p, end);
+        if (e >= 0) atomicAdd(&s_plan[e], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += blockDim.x) counts[(size_t)blockIdx.x * E + e] = s_plan[e];
+}
+
+template <bool MANY>
+__global__ void __launch_bounds__(1024)
+plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, int E, int run,
+            const int32_t* counts, int32_t* offsets, int32_t* row_of_pair, int32_t* pair_of_row) {
     extern __shared__ int s_plan[];
     __shared__ int s_warp[33];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     int* count = s_plan;                      // [warps][E]
-    int* total = count + (size_t)warps * E;   // [E] pairs of this CTA (read by the other CTAs)
-    int* start = total + E;                   // [E] all CTAs' pairs, then the first row of this CTA's pairs
+    int* start = count + (size_t)warps * E;   // [E] all CTAs' pairs, then the first row of this CTA's pairs
     int* before = start + E;                  // [E] pairs of the CTAs in front
-    const int rank = CTAS > 1 ? (int)plan_cluster_rank() : 0;
+    const int rank = (int)blockIdx.x, ctas = (int)gridDim.x;
     for (int i = tid; i < warps * E; i += threads) count[i] = 0;
     __syncthreads();
     pdl_begin();
@@ -77,24 +86,20 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ expert_
     }
     __syncthreads();
     for (int e = tid; e < E; e += threads) {
-        int n = 0;
-        for (int w = 0; w < warps; ++w) n += count[(size_t)w * E + e];
-        total[e] = n;
-    }
-    if (CTAS > 1) plan_cluster_sync(); else __syncthreads();
-    for (int e = tid; e < E; e += threads) {
         int all = 0, front = 0;
-#pragma unroll
-        for (int r = 0; r < CTAS; ++r) {
-            const int n = CTAS > 1 ? plan_peer_word(&total[e], r) : total[e];
-            all += n;
-            if (r < rank) front += n;
+        if (MANY) {
+            for (int r = 0; r < ctas; ++r) {
+                const int n = counts[(size_t)r * E + e];
+                all += n;
+                if (r < rank) front += n;
+            }
+        } else {
+            for (int w = 0; w < warps; ++w) all += count[(size_t)w * E + e];
         }
         start[e] = all;
         before[e] = front;
     }
     __syncthreads();
-    if (CTAS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // done with the others' memory
     // exclusive prefix over the experts: every thread a contiguous run of them
     const int per = (E + threads - 1) / threads;
     int sum = 0;
@@ -148,8 +153,7 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ expert_
             e = next;
         }
     }
-    for (long long r = (long long)kept + rank * threads + tid; r < P; r += CTAS * threads) pair_of_row[r] = -1;
-    if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");     // nobody leaves while its totals are read
+    for (long long r = (long long)kept + rank * threads + tid; r < P; r += (long long)ctas * threads) pair_of_row[r] = -1;
 }
 
 // ---------------------------------------------------------------------------------
@@ -157,19 +161,25 @@ plan_kernel(const int32_t* __restrict__ ids, const int32_t* __restrict__ expert_
 // rest of the traffic is the rows' own writes.  Rows nobody owns (dropped pairs leave them behind the last kept row)
 // are zeroed when the caller wants every row defined.
 // ---------------------------------------------------------------------------------
+constexpr int SORT_BATCH = 4;
+
 template <typename V>
 __global__ void __launch_bounds__(256)
-sort_kernel(const uint8_t* __restrict__ x, long long x_stride, uint8_t* __restrict__ rows, long long rows_stride, long long vecs,
-            int M, int T, const int32_t* __restrict__ row_of_pair, const int32_t* __restrict__ kept, int zero_tail) {
+sort_kernel(const uint8_t* x, long long x_stride, uint8_t* rows, long long rows_stride, long long vecs,
+            int M, int T, const int32_t* row_of_pair, const int32_t* kept, int zero_tail) {
     pdl_begin();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)M * vecs;
     if (i >= all) return;
     const long long m = i / vecs, c = i - m * vecs;
     const V v = reinterpret_cast<const V*>(x + m * x_stride)[c];
     const int32_t* rp = row_of_pair + m * T;
-    for (int t = 0; t < T; ++t) {
-        const int r = rp[t];
-        if (r >= 0) reinterpret_cast<V*>(rows + r * rows_stride)[c] = v;
+    for (int t0 = 0; t0 < T; t0 += SORT_BATCH) {
+        int r[SORT_BATCH];
+#pragma unroll
+        for (int j = 0; j < SORT_BATCH; ++j) r[j] = t0 + j < T ? rp[t0 + j] : -1;
+#pragma unroll
+        for (int j = 0; j < SORT_BATCH; ++j)
+            if (r[j] >= 0) reinterpret_cast<V*>(rows + r[j] * rows_stride)[c] = v;
     }
     if (zero_tail)
         for (long long j = (long long)*kept * vecs + i; j < all * T; j += all)
@@ -184,8 +194,8 @@ constexpr int UNSORT_BATCH = 4;
 
 template <typename T_, int VB, typename O_>
 __global__ void __launch_bounds__(256)
-unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* __restrict__ out, long long out_stride, long long vecs,
-              int M, int T, const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights) {
+unsort_kernel(const uint8_t* rows, long long rows_stride, uint8_t* out, long long out_stride, long long vecs,
+              int M, int T, const int32_t* row_of_pair, const float* weights) {
     using R = RowVec<T_, VB>;
     pdl_begin();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -198,17 +208,18 @@ unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* 
     for (int t0 = 0; t0 < T; t0 += UNSORT_BATCH) {
         R v[UNSORT_BATCH];
         int r[UNSORT_BATCH];
+        float w[UNSORT_BATCH];
 #pragma unroll
         for (int j = 0; j < UNSORT_BATCH; ++j) {
             r[j] = t0 + j < T ? rp[t0 + j] : -1;
+            w[j] = r[j] >= 0 && weights ? weights[m * T + t0 + j] : 1.f;
             if (r[j] >= 0) v[j].load(rows + r[j] * rows_stride, c);
         }
 #pragma unroll
         for (int j = 0; j < UNSORT_BATCH; ++j)
             if (r[j] >= 0) {
-                const float w = weights ? weights[m * T + t0 + j] : 1.f;
 #pragma unroll
-                for (int k = 0; k < R::N; ++k) acc[k] = fmaf(w, v[j].get(k), acc[k]);
+                for (int k = 0; k < R::N; ++k) acc[k] = fmaf(w[j], v[j].get(k), acc[k]);
             }
     }
     RowVec<O_, R::N * (int)sizeof(O_)> o;
@@ -224,9 +235,9 @@ unsort_kernel(const uint8_t* __restrict__ rows, long long rows_stride, uint8_t* 
 // ---------------------------------------------------------------------------------
 template <typename T_, int VB, int WPT>
 __global__ void __launch_bounds__(256)
-unsort_grad_kernel(const uint8_t* __restrict__ dy, long long dy_stride, const uint8_t* __restrict__ rows, long long rows_stride,
-                   uint8_t* __restrict__ drows, long long drows_stride, float* __restrict__ dw, int vecs, int M, int T,
-                   const int32_t* __restrict__ row_of_pair, const float* __restrict__ weights, const int32_t* __restrict__ kept) {
+unsort_grad_kernel(const uint8_t* dy, long long dy_stride, const uint8_t* rows, long long rows_stride,
+                   uint8_t* drows, long long drows_stride, float* dw, int vecs, int M, int T,
+                   const int32_t* row_of_pair, const float* weights, const int32_t* kept) {
     using R = RowVec<T_, VB>;
     __shared__ float s_dot[8][MAX_TOPK];
     pdl_begin();
@@ -298,28 +309,25 @@ unsort_grad_kernel(const uint8_t* __restrict__ dy, long long dy_stride, const ui
 }
 
 static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_len, int M, int T, int E, int32_t* offsets,
-                       int32_t* row_of_pair, int32_t* pair_of_row, cudaStream_t st) {
-    const int P = M * T;
-    const int ctas = P > PLAN_ONE_CTA_PAIRS ? PLAN_CLUSTER : 1;
-    int warps = (PLAN_SMEM / 4 - 3 * E) / E;
+                       int32_t* row_of_pair, int32_t* pair_of_row, int32_t* scratch, cudaStream_t st) {
+    const int P = M * T, ctas = plan_ctas(P);
+    int warps = (PLAN_SMEM / 4 - 2 * E) / E;
     const int need = (int)(((long long)P + 32 * ctas - 1) / (32 * ctas));
     if (warps > 32) warps = 32;
     if (warps > need) warps = need > 0 ? need : 1;
-    const int chunks = ctas * warps;
-    int run = (int)(((long long)P + chunks - 1) / chunks);
+    int run = (int)(((long long)P + (long long)ctas * warps - 1) / ((long long)ctas * warps));
     run = (run + 31) / 32 * 32;
-    const size_t smem = (size_t)4 * E * (warps + 3);
-    auto* kernel = ctas > 1 ? plan_kernel<PLAN_CLUSTER> : plan_kernel<1>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas); cfg.blockDim = dim3(warps * 32); cfg.dynamicSmemBytes = smem; cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ctas; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = ctas > 1 ? 2 : 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ids, expert_map, map_len, P, E, run, offsets, row_of_pair, pair_of_row));
+    const size_t smem = (size_t)4 * E * (warps + 2);
+    if (ctas == 1) {
+        if (cudaFuncSetAttribute(plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+        return cuda_status(launch_pdl(plan_kernel<false>, 1u, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
+                                      (const int32_t*)nullptr, offsets, row_of_pair, pair_of_row));
+    }
+    if (cudaFuncSetAttribute(plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    const cudaError_t e = launch_pdl(plan_count_kernel, (unsigned)ctas, 1024u, (size_t)4 * E, st, ids, expert_map, map_len, P, E, run * warps, scratch);
+    if (e != cudaSuccess) return VMOE_ERR_CUDA;
+    return cuda_status(launch_pdl(plan_kernel<true>, (unsigned)ctas, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
+                                  (const int32_t*)scratch, offsets, row_of_pair, pair_of_row));
 }
 
 static unsigned blocks_of(long long threads) { return (unsigned)((threads + 255) / 256); }
@@ -351,13 +359,23 @@ using namespace vmoe;
 
 extern "C" {
 
+size_t vmoe_plan_scratch_bytes(int32_t M, int32_t T, int32_t E) {
+    if (check_rows(M, T, E, 0, VMOE_BF16) != VMOE_OK) return 0;
+    const int ctas = plan_ctas((long long)M * T);
+    return ctas > 1 ? (size_t)ctas * E * sizeof(int32_t) : 0;
+}
+
 int vmoe_plan_tokens(const int32_t* topk_ids, const int32_t* expert_map, int32_t map_len, int32_t M, int32_t T, int32_t E,
-                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* stream) {
+                     int32_t* expert_offsets, int32_t* row_of_pair, int32_t* pair_of_row, void* scratch, size_t scratch_bytes,
+                     void* stream) {
     const int rc = check_rows(M, T, E, 0, VMOE_BF16);
     if (rc) return rc;
     if (!expert_offsets || (M > 0 && (!topk_ids || !row_of_pair || !pair_of_row))) return VMOE_ERR_NULL;
     if (expert_map && map_len < 0) return VMOE_ERR_SHAPE;
-    return launch_plan(topk_ids, expert_map, map_len, M, T, E, expert_offsets, row_of_pair, pair_of_row, static_cast<cudaStream_t>(stream));
+    const size_t need = vmoe_plan_scratch_bytes(M, T, E);
+    if (need && (!scratch || scratch_bytes < need)) return VMOE_ERR_WORKSPACE;
+    return launch_plan(topk_ids, expert_map, map_len, M, T, E, expert_offsets, row_of_pair, pair_of_row, static_cast<int32_t*>(scratch),
+                       static_cast<cudaStream_t>(stream));
 }
 
 int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K,

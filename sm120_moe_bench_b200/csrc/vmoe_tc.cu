@@ -675,6 +675,20 @@ int make_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t ro
     return VMOE_OK;
 }
 
+// A byte tensor of two or three dimensions (innermost first), 128-byte swizzle; encoded anew at every call.
+int encode_byte_map(CUtensorMap* map, const void* base, int ndim, const unsigned long long* dims, const unsigned long long* strides,
+                    const uint32_t* box) {
+    const int rc = get_encoder();
+    if (rc) return rc;
+    cuuint64_t d[3], s[2];
+    cuuint32_t b[3];
+    const cuuint32_t estr[3] = {1, 1, 1};
+    for (int i = 0; i < ndim; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i + 1 < ndim) s[i] = strides[i]; }
+    return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)ndim, const_cast<void*>(base), d, s, b, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? VMOE_OK : VMOE_ERR_CUDA;
+}
+
 // Scale atoms as a 2-D tensor: rows of one 512-byte atom (128 words), box = the four atoms of one 256-element k-step.
 int make_sf_map(CUtensorMap* map, const void* base, uint64_t atoms) {
     int dev = 0;

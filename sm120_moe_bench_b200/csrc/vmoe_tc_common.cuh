@@ -133,6 +133,8 @@ __device__ __forceinline__ void tc_timeout(const Workspace& ws, TcShared* sh) {
 // host: cached cuTensorMapEncodeTiled of a 2-D byte tensor [rows, row_bytes], box [box_rows, 128 B], 128-byte swizzle
 int get_encoder();
 int make_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint32_t box_rows);
+int encode_byte_map(CUtensorMap* map, const void* base, int ndim, const unsigned long long* dims, const unsigned long long* strides,
+                    const uint32_t* box);
 int make_sf_map(CUtensorMap* map, const void* base, uint64_t atoms);   // scale atoms [atoms, 512 B], box = 4 atoms
 int tc_sm_count();
 

@@ -106,6 +106,13 @@ def _matmul(q, scale, w: Int8Rows, N: int, offsets, swiglu: bool, zero_tail: boo
     return out
 
 
+def int8_status(device: torch.device | str | int = "cuda") -> int:
+    """0, or the status of a bounded wait that ran out inside an 8-bit product on this device since the last call (6 = time-out,
+    as ``Workspace.status``).  Waits for the current stream."""
+    with torch.cuda.device(device):
+        return lib.vmoe_int8_read_status(torch.cuda.current_stream().cuda_stream)
+
+
 def _out_columns(w: Int8Rows, K: int, device, swiglu: bool, experts: int | None) -> int:
     if w.q.device != device:
         raise ValueError(f"the weights are on {w.q.device}, the rows on {device}")

@@ -95,7 +95,7 @@ class TokenPlan:
 
 
 def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tensor | None = None) -> TokenPlan:
-    """Tables of the stable sort of the ``[M, T]`` int32 expert ids by expert (one launch).
+    """Tables of the stable sort of the ``[M, T]`` int32 expert ids by expert (one launch up to 4096 pairs, else two).
 
     With ``expert_map`` (int32, -1 = not local) the ids are global and ``num_experts`` counts the local ones.  Ids outside
     the map, or outside ``[0, num_experts)``, drop their pair.  ``T <= 16``, ``num_experts <= 8192``."""
@@ -119,10 +119,13 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     row_of_pair = torch.empty(M, T, dtype=torch.int32, device=dev)
     pair_of_row = torch.empty(M * T, dtype=torch.int32, device=dev)
+    need = lib.vmoe_plan_scratch_bytes(M, T, num_experts)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     with _on(dev) as stream:
         check(lib.vmoe_plan_tokens(topk_ids.data_ptr(), None if expert_map is None else expert_map.data_ptr(),
                                    0 if expert_map is None else expert_map.numel(), M, T, num_experts, offsets.data_ptr(),
-                                   row_of_pair.data_ptr(), pair_of_row.data_ptr(), stream), "vmoe_plan_tokens")
+                                   row_of_pair.data_ptr(), pair_of_row.data_ptr(), scratch.data_ptr() if need else None, need, stream),
+              "vmoe_plan_tokens")
     return TokenPlan(offsets, row_of_pair, pair_of_row, num_experts)
 
 

@@ -19,11 +19,16 @@ def _buf(n=4096):
 
 def test_plan_checks():
     lib, b = _lib(), ctypes.addressof(_buf())
-    plan = lambda M, T, E, ids=b, off=b, rp=b, pr=b, emap=None, n=0: lib.vmoe_plan_tokens(ids, emap, n, M, T, E, off, rp, pr, None)
+    plan = lambda M, T, E, ids=b, off=b, rp=b, pr=b, emap=None, n=0, ws=None, bytes_=0: \
+        lib.vmoe_plan_tokens(ids, emap, n, M, T, E, off, rp, pr, ws, bytes_, None)
     assert plan(-1, 2, 4) == 2 and plan(4, 0, 4) == 2 and plan(4, 2, 0) == 2
     assert plan(4, 17, 32) == 8 and plan(4, 2, 8193) == 8 and plan(2 ** 31 - 1, 16, 4) == 8 and plan(2 ** 27, 16, 4) == 8
     assert plan(4, 2, 4, ids=None) == 1 and plan(4, 2, 4, off=None) == 1 and plan(4, 2, 4, rp=None) == 1 and plan(4, 2, 4, pr=None) == 1
     assert plan(4, 2, 4, emap=b, n=-1) == 2
+    need = lib.vmoe_plan_scratch_bytes
+    assert need(64, 10, 512) == 0 and need(512, 8, 512) == 0 and need(4097, 1, 8) == 3 * 8 * 4 and need(2 ** 20, 16, 4) == 64 * 4 * 4
+    assert need(-1, 2, 4) == 0
+    assert plan(4097, 1, 8) == 4 and plan(4097, 1, 8, ws=b, bytes_=95) == 4
 
 
 def test_sort_checks():
