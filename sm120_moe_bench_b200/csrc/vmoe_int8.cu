@@ -5,16 +5,36 @@ namespace vmoe {
 
 // ---------------------------------------------------------------------------------
 // Row quantiser: scale = max|x| / 127, code = rint(127 x / max|x|), ties to even -- the code of the exact quotient, not of
-// a rounded one.  y = x * RN(127 / max|x|) is off by at most 127 * 2^-23 < 2e-5, so only a y within 1e-4 of a border
-// between two codes is decided in 64 bits.  A row of zeros has scale 0 and codes 0; a row with an infinity or a NaN has
+// a rounded one.  y = x * RN(127 / max|x|) is off by at most 127 * 2^-23 < 2e-5, so only vectors with a y within 1e-4 of a
+// border between two codes are decided in 64 bits.  A row of zeros has scale 0 and codes 0; a row with an infinity or a NaN has
 // scale NaN and codes 0, so that its outputs are NaN and no other row's are.
 // WPR warps per row, eight per CTA.  With row_of_pair a row is a token and its codes go to the token's T sorted rows.
+// A thread keeps up to four vectors of the row in registers, so that rows of up to 4 * 32 * WPR vectors are read once.
+// Rounding adds 1.5 * 2^23: the sum's low byte is the code, and taking the constant off again gives the rounded value.
 // ---------------------------------------------------------------------------------
-__device__ __forceinline__ int i8_code(float x, float inv, float amax) {
-    const float y = x * inv;
-    float r = rintf(y);
-    if (fabsf(fabsf(y - r) - 0.5f) < 1e-4f) r = (float)rint(127.0 * (double)x / (double)amax);
-    return (int)r;
+constexpr float I8_ROUND = 12582912.f;
+constexpr int I8_KEPT = 4;
+
+template <typename R>
+__device__ __forceinline__ void i8_codes(const R& v, float up, float inv, float amax, uint32_t (&w)[2]) {
+    float t[R::N], far = 0.f;
+#pragma unroll
+    for (int k = 0; k < R::N; ++k) {
+        const float y = v.get(k) * up * inv;
+        t[k] = y + I8_ROUND;
+        far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
+    }
+    if (far > 0.5f - 1e-4f) {                            // next to a border
+#pragma unroll
+        for (int k = 0; k < R::N; ++k) t[k] = I8_ROUND + (float)rint(127.0 * (double)(v.get(k) * up) / (double)amax);
+    }
+#pragma unroll
+    for (int h = 0; h < (R::N + 3) / 4; ++h) {
+        uint32_t b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) b[k] = 4 * h + k < R::N ? __float_as_uint(t[4 * h + k < R::N ? 4 * h + k : 0]) : 0u;
+        w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
 }
 
 template <typename T_, int VB, int WPR>
@@ -30,13 +50,24 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
     const bool on = m < rows && (!live || m < *live);
     const uint8_t* src = x + m * x_stride;
     uint32_t top = 0;                                    // magnitudes ordered as integers: NaN > infinity > finite
-    if (on)
-        for (int c = part; c < vecs; c += WPR * 32) {
+    R keep[I8_KEPT];
+    if (on) {
+#pragma unroll
+        for (int i = 0; i < I8_KEPT; ++i)
+            if (part + i * WPR * 32 < vecs) keep[i].load(src, part + i * WPR * 32);
+#pragma unroll
+        for (int i = 0; i < I8_KEPT; ++i)
+            if (part + i * WPR * 32 < vecs) {
+#pragma unroll
+                for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(keep[i].get(k)) & 0x7fffffffu);
+            }
+        for (int c = part + I8_KEPT * WPR * 32; c < vecs; c += WPR * 32) {
             R v;
             v.load(src, c);
 #pragma unroll
             for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(v.get(k)) & 0x7fffffffu);
         }
+    }
     top = __reduce_max_sync(0xffffffffu, top);
     if (WPR > 1) {
         if (lane == 0) s_max[warp] = top;
@@ -57,24 +88,26 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
             const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
             if (r >= 0) scales[r] = scale;
         }
-    for (int c = part; c < vecs; c += WPR * 32) {
-        R v;
-        v.load(src, c);
-        union { int8_t b[8]; uint32_t w[2]; } code;
-        code.w[0] = code.w[1] = 0;
-        if (inv > 0.f) {
-#pragma unroll
-            for (int k = 0; k < R::N; ++k) code.b[k] = (int8_t)i8_code(v.get(k) * up, inv, amax);
-        }
+    auto put = [&](const R& v, int c) {
+        uint32_t w[2] = {0, 0};
+        if (inv > 0.f) i8_codes(v, up, inv, amax, w);
         for (int t = 0; t < copies; ++t) {
             const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
             if (r < 0) continue;
             int8_t* dst = q + r * q_stride + (long long)c * R::N;
-            if (R::N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(code.w[0], code.w[1]);
-            else if (R::N == 4) *reinterpret_cast<uint32_t*>(dst) = code.w[0];
-            else if (R::N == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)code.w[0];
-            else *dst = code.b[0];
+            if (R::N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+            else if (R::N == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+            else if (R::N == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w[0];
+            else *dst = (int8_t)w[0];
         }
+    };
+#pragma unroll
+    for (int i = 0; i < I8_KEPT; ++i)
+        if (part + i * WPR * 32 < vecs) put(keep[i], part + i * WPR * 32);
+    for (int c = part + I8_KEPT * WPR * 32; c < vecs; c += WPR * 32) {
+        R v;
+        v.load(src, c);
+        put(v, c);
     }
 }
 
@@ -197,6 +230,9 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
             return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 1>, (unsigned)((rows + 7LL) / 8), 256u, 0, st, a, xs,
                                           (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
         if (vecs <= 256)
+            return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 2>, (unsigned)((rows + 3LL) / 4), 256u, 0, st, a, xs,
+                                          (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
+        if (vecs <= 512)
             return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 4>, (unsigned)((rows + 1LL) / 2), 256u, 0, st, a, xs,
                                           (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
         return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 8>, (unsigned)rows, 256u, 0, st, a, xs, (long long)rows,
@@ -223,7 +259,7 @@ int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, in
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (!i8_tc_ok(p) || E > I8_TC_MAX_EXPERTS) return launch_i8_tile(p, st);
     if (!expert_offsets) {
-        const long long items = (M + 255LL) / 256 * ((N + (swiglu ? 63LL : 127LL)) / (swiglu ? 64 : 128));
+        const long long items = (M + 127LL) / 128 * ((N + (swiglu ? 127LL : 255LL)) / (swiglu ? 128 : 256));
         if (items < 148) return launch_i8_split(p, st);
     }
     return launch_i8_tc(p, st);

@@ -3,9 +3,8 @@
 // In both kernels the MMA's rows (operand A) are output channels and its columns (operand B) are tokens, so the number of
 // tokens of an item is free in steps of 16 or 32: an expert with 5 rows costs 32 columns, one with 320 costs 192 + 128, and a
 // decode batch streams every weight once.  A thread of the epilogue owns a channel; 32 lanes store 32 neighbours of a row.
-// swiglu: the 32 channels of a TMEM lane quadrant are 16 gate rows followed by the 16 matching up rows.
 //
-//   i8_tc_kernel      persistent, grouped or large: 128 channels x up to 256 tokens per item
+//   i8_tc_kernel      persistent, grouped or large: 256 weight rows x up to 256 tokens per item
 //   i8_split_kernel   dense products too small to fill the GPU that way: 128 channels x up to 128 tokens per CTA, the
 //                     reduction split over a cluster, partial sums met in distributed shared memory (exact: integers)
 #include "vmoe_int8.cuh"
@@ -50,10 +49,16 @@ constexpr int I8_A_BYTES = 128 * I8_KB;                   // 128 channels
 constexpr int I8_BOX_BIG = 64, I8_BOX_SMALL = 16;         // token rows per copy
 
 // ----------------------------------------------------------------------------------------------------- persistent
+// An item is 256 weight rows (two MMA row tiles: 256 channels, or 128 gate rows and the 128 matching up rows, so that a lane
+// of the epilogue has both) times at most P.tokens tokens of one expert.  A stage of U tokens is 32 KB + U * 128 bytes
+// for 8 MMAs of U columns: at 64 bytes per clock an SM ingests it in 512 + 2 U cycles, the tensor pipe needs 4 U -- the
+// two meet at 256 tokens.  Items of up to 128 tokens leave room in tensor memory for two accumulator sets, so that the
+// epilogue of one runs under the MMAs of the next; above there is one set.
 constexpr int I8P_MAX_STAGES = 8;
-constexpr int I8P_EPI_WARPS = 8;
+constexpr int I8P_EPI_WARPS = 16;
 constexpr int I8P_THREADS = 64 + 32 * I8P_EPI_WARPS;
-constexpr int I8P_TOKENS = 256;                           // tokens per item at most (UMMA N): two accumulators fill tensor memory
+constexpr int I8P_ROWS = 256;                             // weight rows per item
+constexpr int I8P_TOKENS = 256;                           // tokens per item at most (UMMA N)
 
 struct I8Shared {
     uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
@@ -66,7 +71,7 @@ struct I8Shared {
 };
 
 struct I8TcParams {
-    CUtensorMap map_w;                                    // [E, channels, K]
+    CUtensorMap map_w;                                    // [E, weight rows, K]
     CUtensorMap map_a64, map_a16;                         // token rows [M, K] in boxes of 64 and 16 (split: of the tile's tokens)
     I8Problem p;
     int kblocks, ctiles, stages, tokens;                  // tokens: most of an item
@@ -86,7 +91,7 @@ __device__ __forceinline__ I8Item i8_item(const I8TcParams& P, const int* s_pref
     r.expert = lo;
     const int count = s_off[lo + 1] - s_off[lo], nb = s_pref[lo + 1] - s_pref[lo], j = block - s_pref[lo];
     r.n = min(((count + nb - 1) / nb + 15) & ~15, P.tokens);      // the expert's rows in equal blocks
-    if (r.n > 16) r.n = (r.n + 31) & ~31;                 // two epilogue warps share the columns in chunks of 16
+    if (r.n > 16) r.n = (r.n + 31) & ~31;
     r.row0 = s_off[lo] + j * r.n;
     r.rows = min(r.n, max(s_off[lo + 1] - r.row0, 0));
     return r;
@@ -101,18 +106,25 @@ __device__ __forceinline__ void i8_drain(uint64_t* full, uint32_t issued, int st
     for (uint32_t g = issued > (uint32_t)stages ? issued - stages : 0; g < issued; ++g) mbar_wait(&full[g % stages], (g / stages) & 1);
 }
 
-template <bool SWIGLU>
+template <typename O_> __device__ __forceinline__ void i8_put(O_* at, float v);
+template <> __device__ __forceinline__ void i8_put<float>(float* at, float v) { *at = v; }
+template <> __device__ __forceinline__ void i8_put<__nv_bfloat16>(__nv_bfloat16* at, float v) { *at = __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ void i8_put<__half>(__half* at, float v) { *at = __float2half_rn(v); }
+
+template <bool SWIGLU, typename O_>
 __global__ void __launch_bounds__(I8P_THREADS, 1)
 i8_tc_kernel(const __grid_constant__ I8TcParams P) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int stage_bytes = I8_A_BYTES + P.tokens * I8_KB;
+    const int stage_bytes = 2 * I8_A_BYTES + P.tokens * I8_KB;
     I8Shared* sh = reinterpret_cast<I8Shared*>(smem + (size_t)P.stages * stage_bytes);
     int* s_pref = reinterpret_cast<int*>(sh + 1);         // [E + 1] token blocks of the experts in front
     int* s_off = s_pref + P.p.E + 1;                      // [E + 1] first row of each expert
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const I8Problem& p = P.p;
     const int stages = P.stages;
+    const bool two = P.tokens <= I8P_TOKENS / 2;          // two accumulator sets
+    const uint32_t second = two ? I8P_TOKENS / 2 : I8P_TOKENS;    // column of the second row tile's accumulator
 
     if (tid == 0) {
         for (int i = 0; i < stages; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], 1); }
@@ -152,13 +164,13 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
     const int kblocks = P.kblocks;
 
     if (warp == 0) {
-        // ------------------------------------------------------------- producer: 128 channels and the item's token rows
+        // ------------------------------------------------------------- producer: the item's weight rows and token rows
         const bool leader = elect_one();
         uint32_t g = 0;
         bool ok = true;
         for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
             const I8Item u = i8_item(P, s_pref, s_off, item);
-            const int ch = u.ctile * (SWIGLU ? 64 : 128);
+            const int ch = u.ctile * (SWIGLU ? 128 : I8P_ROWS);
             for (int kb = 0; kb < kblocks; ++kb) {
                 const int slot = g % stages;
                 bool w = true;
@@ -168,19 +180,14 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
                 uint8_t* st = smem + (size_t)slot * stage_bytes;
                 uint64_t* bar = &sh->full[slot];
                 if (leader) {
-                    mbar_arrive_expect_tx(bar, I8_A_BYTES + u.n * I8_KB);
-                    if (SWIGLU) {
-#pragma unroll
-                        for (int b = 0; b < 8; ++b)       // 16 gate rows, then the 16 matching up rows, per lane quadrant
-                            i8_load_3d(st + b * 16 * I8_KB, &P.map_w, kb * I8_KB, (b & 1) * p.N + ch + (b >> 1) * 16, u.expert, bar);
-                    } else {
-                        i8_load_3d(st, &P.map_w, kb * I8_KB, ch, u.expert, bar);
-                    }
+                    mbar_arrive_expect_tx(bar, 2 * I8_A_BYTES + u.n * I8_KB);
+                    i8_load_3d(st, &P.map_w, kb * I8_KB, ch, u.expert, bar);
+                    if (SWIGLU) i8_load_3d(st + I8_A_BYTES, &P.map_w, kb * I8_KB, p.N + ch, u.expert, bar);
                     int r = 0;
                     for (; r + I8_BOX_BIG <= u.n; r += I8_BOX_BIG)
-                        tma_load_2d(st + I8_A_BYTES + r * I8_KB, &P.map_a64, kb * I8_KB, u.row0 + r, bar);
+                        tma_load_2d(st + 2 * I8_A_BYTES + r * I8_KB, &P.map_a64, kb * I8_KB, u.row0 + r, bar);
                     for (; r < u.n; r += I8_BOX_SMALL)
-                        tma_load_2d(st + I8_A_BYTES + r * I8_KB, &P.map_a16, kb * I8_KB, u.row0 + r, bar);
+                        tma_load_2d(st + 2 * I8_A_BYTES + r * I8_KB, &P.map_a16, kb * I8_KB, u.row0 + r, bar);
                 }
                 __syncwarp();
                 ++g;
@@ -192,8 +199,7 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
             i8_drain(sh->full, g, stages);
         }
     } else if (warp == 1) {
-        // ------------------------------------------------------------- MMA issuer (warp-uniform loop, one elected lane
-        // issues); two accumulators of 256 columns take turns
+        // ------------------------------------------------------------- MMA issuer (warp-uniform loop, one elected lane issues)
         const bool leader = elect_one();
         uint32_t g = 0, it = 0;
         bool ok = true;
@@ -201,9 +207,9 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
         for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
             const I8Item u = i8_item(P, s_pref, s_off, item);
             const uint32_t idesc = i8_idesc(128, u.n);
-            const uint32_t buf = it & 1, acc = tmem + buf * I8P_TOKENS;
+            const uint32_t buf = two ? it & 1 : 0, use = two ? it >> 1 : it, acc = tmem + buf * I8P_TOKENS;
             bool w = true;
-            if (it >= 2) w = mbar_wait(&sh->tmem_empty[buf], ((it >> 1) - 1) & 1);
+            if (use >= 1) w = mbar_wait(&sh->tmem_empty[buf], (use - 1) & 1);
             if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
             for (int kb = 0; kb < kblocks; ++kb) {
                 const int slot = g % stages;
@@ -211,11 +217,13 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
                 tc_fence_after();
                 const uint32_t st16 = smem16 + slot * (stage_bytes >> 4);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint64_t da = make_desc(st16 + ((j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
-                    const uint64_t db = make_desc(st16 + ((I8_A_BYTES + j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
-                    if (leader) i8_mma(acc, da, db, idesc, (kb | j) ? 1u : 0u);
-                }
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t da = make_desc(st16 + ((t * I8_A_BYTES + j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                        const uint64_t db = make_desc(st16 + ((2 * I8_A_BYTES + j * 32) >> 4) + DESC_SW128_LBO, DESC_SW128_HI);
+                        if (leader) i8_mma(acc + t * second, da, db, idesc, (kb | j) ? 1u : 0u);
+                    }
                 if (leader) tc_commit(&sh->empty[slot]);
                 ++g;
             }
@@ -226,53 +234,67 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
         if (!ok && leader) i8_abort(&sh->abort_flag);
         __syncwarp();
     } else {
-        // ------------------------------------------------------------- epilogue: a lane is a channel, two warps per lane
-        // quadrant take half of the item's tokens each
+        // ------------------------------------------------------------- epilogue: a lane is a channel; the four warps of a
+        // lane quadrant take the item's units (16 tokens of one row tile, with swiglu of both) in turn
         const int quad = warp & 3, sub = (warp - 2) >> 2, et = tid - 64;
+        O_* const out = static_cast<O_*>(p.out);
         if (p.offsets && p.zero_tail) {
             for (long long m = (long long)s_off[E] + blockIdx.x; m < p.M; m += gridDim.x)
-                for (int n = et; n < p.N; n += 32 * I8P_EPI_WARPS) i8_store(p.out, m * p.out_stride + n, p.out_dtype, 0.f);
+                for (int n = et; n < p.N; n += 32 * I8P_EPI_WARPS) i8_put(out + m * p.out_stride + n, 0.f);
         }
+        float* const rs = sh->row_scale[warp - 2];
         uint32_t it = 0;
         for (long long item = blockIdx.x; item < total; item += gridDim.x, ++it) {
             const I8Item u = i8_item(P, s_pref, s_off, item);
-            const uint32_t buf = it & 1;
-            const int half = u.n > 16 ? u.n >> 1 : 16;    // an item of 16 columns is the first warp's alone
-            const int c_first = sub * half, c_end = min(c_first + half, u.n);
-            float* rs = sh->row_scale[warp - 2];
+            const uint32_t buf = two ? it & 1 : 0, use = two ? it >> 1 : it;
+            const int units = SWIGLU ? u.n >> 4 : u.n >> 3;
             __syncwarp();
-            for (int c = c_first + lane; c < c_end; c += 32) rs[c - c_first] = c < u.rows ? p.a_scale[u.row0 + c] : 0.f;
+            for (int k = sub * 16 + (lane & 15), slot = lane; ; k += 64, slot += 16) {      // scales of unit (k >> 4)
+                if ((k >> 4) >= units) break;
+                const int c = (SWIGLU ? k >> 4 : k >> 5) * 16 + (k & 15);
+                if (lane < 16) rs[slot] = c < u.rows ? p.a_scale[u.row0 + c] : 0.f;
+            }
             __syncwarp();
-            const int ch = SWIGLU ? u.ctile * 64 + quad * 16 + (lane & 15) : u.ctile * 128 + quad * 32 + lane;
-            const float sw = ch < p.N ? p.w_scale[(long long)u.expert * p.wrows + (SWIGLU ? (lane >> 4) * p.N : 0) + ch] : 0.f;
-            const bool w = mbar_wait(&sh->tmem_full[buf], (it >> 1) & 1);
+            const int ch = u.ctile * (SWIGLU ? 128 : I8P_ROWS) + quad * 32 + lane;
+            const float* wsc = p.w_scale + (long long)u.expert * p.wrows;
+            const int ch2 = SWIGLU ? p.N + ch : ch + 128;
+            const float sw0 = ch < p.N ? wsc[ch] : 0.f;
+            const float sw1 = (SWIGLU ? ch : ch2) < p.N ? wsc[ch2] : 0.f;
+            const bool w = mbar_wait(&sh->tmem_full[buf], use & 1);
             if (!__all_sync(0xffffffffu, w)) { if (lane == 0) i8_abort(&sh->abort_flag); break; }
             tc_fence_after();
             const uint32_t tacc = tmem + buf * I8P_TOKENS + ((uint32_t)(quad * 32) << 16);
-            for (int c = c_first; c < c_end; c += 16) {
-                const float* cs = rs + (c - c_first);
-                uint32_t v[16];
+            for (int k = sub, slot = 0; k < units; k += 4, slot += 16) {
+                const int c = (SWIGLU ? k : k >> 1) * 16, left = u.rows - c;
+                const float* cs = rs + slot;
+                uint32_t v[16], v2[SWIGLU ? 16 : 1];
                 __syncwarp();
-                tc_ld16(tacc + c, v);
-                tc_ld_wait();
                 if (SWIGLU) {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        // lanes 0-15 hold gate values and take token c + i, lanes 16-31 hold up values and take c + i + 1
-                        const bool lo = lane < 16;
-                        const float v0 = i8_scaled((int)v[i], cs[i], sw), v1 = i8_scaled((int)v[i + 1], cs[i + 1], sw);
-                        const float other = __shfl_xor_sync(0xffffffffu, lo ? v1 : v0, 16);
-                        const float gate = lo ? v0 : other, up = lo ? other : v1;
-                        const int j = c + i + (lo ? 0 : 1);
-                        if (j < u.rows && ch < p.N)
-                            i8_store(p.out, (long long)(u.row0 + j) * p.out_stride + ch, p.out_dtype, up * i8_silu(gate));
-                    }
+                    tc_ld16(tacc + c, v);
+                    tc_ld16(tacc + second + c, reinterpret_cast<uint32_t (&)[16]>(v2));
                 } else {
+                    tc_ld16(tacc + (k & 1) * second + c, v);
+                }
+                tc_ld_wait();
+                const int chn = SWIGLU || !(k & 1) ? ch : ch2;
+                if (chn < p.N) {
+                    const float sw = SWIGLU || !(k & 1) ? sw0 : sw1;
+                    O_* o = out + (long long)(u.row0 + c) * p.out_stride + chn;
+                    if (left >= 16) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int j = c + i;
-                        if (j < u.rows && ch < p.N)
-                            i8_store(p.out, (long long)(u.row0 + j) * p.out_stride + ch, p.out_dtype, i8_scaled((int)v[i], cs[i], sw));
+                        for (int i = 0; i < 16; ++i, o += p.out_stride) {
+                            float x = i8_scaled((int)v[i], cs[i], sw);
+                            if (SWIGLU) x = i8_scaled((int)v2[SWIGLU ? i : 0], cs[i], sw1) * i8_silu(x);
+                            i8_put(o, x);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i, o += p.out_stride) {
+                            if (i >= left) break;
+                            float x = i8_scaled((int)v[i], cs[i], sw);
+                            if (SWIGLU) x = i8_scaled((int)v2[SWIGLU ? i : 0], cs[i], sw1) * i8_silu(x);
+                            i8_put(o, x);
+                        }
                     }
                 }
             }
@@ -352,8 +374,8 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
                 mbar_arrive_expect_tx(&sh.full[slot], stage_bytes);
                 if (SWIGLU) {
 #pragma unroll
-                    for (int b = 0; b < 8; ++b)
-                        i8_load_3d(st + b * 16 * I8_KB, &P.map_w, kb * I8_KB, (b & 1) * p.N + ch0 + (b >> 1) * 16, 0, &sh.full[slot]);
+                    for (int b = 0; b < 2; ++b)           // 64 gate rows, then the 64 matching up rows
+                        i8_load_3d(st + b * 64 * I8_KB, &P.map_w, kb * I8_KB, b * p.N + ch0, 0, &sh.full[slot]);
                 } else {
                     i8_load_3d(st, &P.map_w, kb * I8_KB, ch0, 0, &sh.full[slot]);
                 }
@@ -415,13 +437,13 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
             const int t = i / QUADS, c = (i % QUADS) * 4, ch = ch0 + c;
             if (ch >= p.N) continue;
             int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
-            const uint32_t at = base + (uint32_t)(t * 128 + (SWIGLU ? (c >> 4) * 32 + (c & 15) : c)) * 4;
+            const uint32_t at = base + (uint32_t)(t * 128 + c) * 4;
             for (int r = 0; r < split; ++r) {
                 const uint32_t a = i8_cluster_addr(at, r);
                 const int4 x = i8_ld_peer(a);
                 s0[0] += x.x; s0[1] += x.y; s0[2] += x.z; s0[3] += x.w;
                 if (SWIGLU) {
-                    const int4 y = i8_ld_peer(a + 64);
+                    const int4 y = i8_ld_peer(a + 64 * 4);
                     s1[0] += y.x; s1[1] += y.y; s1[2] += y.z; s1[3] += y.w;
                 }
             }
@@ -482,33 +504,57 @@ bool i8_tc_ok(const I8Problem& p) {
 
 constexpr size_t I8P_SMEM = 227 * 1024;
 
-template <bool SWIGLU>
+// Tokens per item.  Grouped: from the average rows per expert (the counts are on the device).  Dense: the size whose last
+// round of items over the SMs wastes least -- a k-block costs the larger of 4 U (tensor pipe) and 512 + 2 U cycles
+// (ingest), an item of more than 128 tokens its epilogue on top (about 20 cycles a token).
+static int i8_tokens(const I8Problem& p, int kblocks, int ctiles) {
+    if (p.offsets) {
+        const long long per = p.M / p.E;
+        return per <= 32 ? 64 : per <= 128 || kblocks < 16 ? 128 : I8P_TOKENS;
+    }
+    int best = 128;
+    long long least = -1;
+    for (int u = 64; u <= I8P_TOKENS; u += 32) {
+        const long long rounds = ((p.M + u - 1LL) / u * ctiles + tc_sm_count() - 1) / tc_sm_count();
+        const int kb = 4 * u > 512 + 2 * u ? 4 * u : 512 + 2 * u;
+        const long long cost = rounds * ((long long)kblocks * kb + (u > 128 ? 20 * u : 0));
+        if (least < 0 || cost <= least) { least = cost; best = u; }
+    }
+    return best;
+}
+
+template <bool SWIGLU, typename O_>
 static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
     I8TcParams P;
     memset(&P, 0, sizeof(P));
     P.p = p;
     P.kblocks = (p.K + I8_KB - 1) / I8_KB;
-    P.ctiles = SWIGLU ? (p.N + 63) / 64 : (p.N + 127) / 128;
-    // Few rows per expert: items of at most 64 tokens, so that the stages hold more weight bytes in flight.
-    P.tokens = p.E > 1 && (long long)p.M <= 32LL * p.E ? 64 : I8P_TOKENS;
-    const size_t stage = I8_A_BYTES + (size_t)P.tokens * I8_KB;
+    P.ctiles = SWIGLU ? (p.N + 127) / 128 : (p.N + I8P_ROWS - 1) / I8P_ROWS;
+    P.tokens = i8_tokens(p, P.kblocks, P.ctiles);
+    const size_t stage = 2 * I8_A_BYTES + (size_t)P.tokens * I8_KB;
     const size_t rest = sizeof(I8Shared) + 2 * ((size_t)p.E + 1) * sizeof(int) + 1024;
     P.stages = I8P_MAX_STAGES;
     while (P.stages > 2 && P.stages * stage + rest > I8P_SMEM) --P.stages;
     const size_t smem = P.stages * stage + rest;
     if (smem > I8P_SMEM) return VMOE_ERR_LIMIT;
     int rc;
-    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 16 : 128))) return rc;
+    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 128 : I8P_ROWS))) return rc;
     if ((rc = i8_map_a(&P.map_a64, p, I8_BOX_BIG))) return rc;
     if ((rc = i8_map_a(&P.map_a16, p, I8_BOX_SMALL))) return rc;
     // one CTA per SM (tc_sm_count), but no more than there can be items
     const long long blocks = ((long long)p.M + P.tokens - 1) / P.tokens + (p.E > 1 ? (p.E < p.M ? p.E : p.M) : 0);
     const long long items = blocks * P.ctiles;
     const unsigned grid = (unsigned)(items < tc_sm_count() ? items : tc_sm_count());
-    if (cudaFuncSetAttribute(i8_tc_kernel<SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8P_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
-    return cuda_status(launch_pdl(i8_tc_kernel<SWIGLU>, grid, (unsigned)I8P_THREADS, smem, st, P));
+    if (cudaFuncSetAttribute(i8_tc_kernel<SWIGLU, O_>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8P_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    return cuda_status(launch_pdl(i8_tc_kernel<SWIGLU, O_>, grid, (unsigned)I8P_THREADS, smem, st, P));
 }
-int launch_i8_tc(const I8Problem& p, cudaStream_t st) { return p.swiglu ? launch_i8_tc_t<true>(p, st) : launch_i8_tc_t<false>(p, st); }
+int launch_i8_tc(const I8Problem& p, cudaStream_t st) {
+    if (p.swiglu)
+        return p.out_dtype == VMOE_F32 ? launch_i8_tc_t<true, float>(p, st) : p.out_dtype == VMOE_BF16 ? launch_i8_tc_t<true, __nv_bfloat16>(p, st)
+                                                                                                         : launch_i8_tc_t<true, __half>(p, st);
+    return p.out_dtype == VMOE_F32 ? launch_i8_tc_t<false, float>(p, st) : p.out_dtype == VMOE_BF16 ? launch_i8_tc_t<false, __nv_bfloat16>(p, st)
+                                                                                                      : launch_i8_tc_t<false, __half>(p, st);
+}
 
 template <bool SWIGLU>
 static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
@@ -536,7 +582,7 @@ static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
     // cluster holds, while that one waits for its own cluster, could otherwise wait in a circle.
     if (smem < I8S_SMEM_LEAST) smem = I8S_SMEM_LEAST;
     int rc;
-    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 16 : 128))) return rc;
+    if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 64 : 128))) return rc;
     if ((rc = i8_map_a(&P.map_a64, p, (uint32_t)P.tokens))) return rc;
     if (cudaFuncSetAttribute(i8_split_kernel<SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8S_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};

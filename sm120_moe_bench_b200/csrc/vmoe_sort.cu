@@ -88,10 +88,12 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     for (int e = tid; e < E; e += threads) {
         int all = 0, front = 0;
         if (MANY) {
-            for (int r = 0; r < ctas; ++r) {
-                const int n = counts[(size_t)r * E + e];
-                all += n;
-                if (r < rank) front += n;
+            for (int r0 = 0; r0 < ctas; r0 += 8) {            // eight loads in flight
+                int n[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
             }
         } else {
             for (int w = 0; w < warps; ++w) all += count[(size_t)w * E + e];
