@@ -368,6 +368,28 @@ int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, in
                      int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
                      int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream);
 
+/* x [M, K] (bf16 / fp16 / f32) quantised row by row, times w [N, K] (swiglu: [2 N, K]): one launch for up to eight rows,
+ * else two, the codes in `scratch` (16-byte aligned, vmoe_int8_linear_scratch_bytes). */
+size_t vmoe_int8_linear_scratch_bytes(int32_t M, int32_t K);
+int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, const int8_t* w, int64_t w_stride, const float* w_scale,
+                     int32_t N, int32_t K, int32_t swiglu, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
+                     size_t scratch_bytes, void* stream);
+
+/* Rows of codes of any alignment, copied to rows that start on 16-byte boundaries (out and out_stride multiples of 16;
+ * columns from K to the next multiple of 16 become zero). */
+int vmoe_int8_pack(const int8_t* q, int64_t q_stride, int64_t rows, int32_t K, int8_t* out, int64_t out_stride, void* stream);
+
+/* The expert layer on 8-bit weights: plan, quantise into expert order, w13 with silu(gate) * up, quantise, w2, weighted
+ * sum.  Rows between the products are f32.  w13 [E, 2 N, K] (gate rows first), w2 [E, K, N]; topk_ids, topk_weights [M, T];
+ * expert_map as in vmoe_plan_tokens.  Six or seven launches; scratch 16-byte aligned, of
+ * vmoe_int8_experts_scratch_bytes (0: sizes beyond the limits of vmoe_plan_tokens). */
+size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N);
+int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K, int32_t N,
+                      const int32_t* topk_ids, const float* topk_weights, const int32_t* expert_map, int32_t map_len,
+                      const int8_t* w13, int64_t w13_stride, int64_t w13_expert_stride, const float* w13_scale,
+                      const int8_t* w2, int64_t w2_stride, int64_t w2_expert_stride, const float* w2_scale,
+                      void* out, int64_t out_stride, int32_t out_dtype, void* scratch, size_t scratch_bytes, void* stream);
+
 /* Status word of the 8-bit products on the current device: VMOE_OK, or VMOE_ERR_TIMEOUT when a bounded wait inside one of
  * them ran out since the last reading (that product's output is not complete).  Synchronises the stream, clears the word. */
 int vmoe_int8_read_status(void* stream);

@@ -4,38 +4,11 @@
 namespace vmoe {
 
 // ---------------------------------------------------------------------------------
-// Row quantiser: scale = max|x| / 127, code = rint(127 x / max|x|), ties to even -- the code of the exact quotient, not of
-// a rounded one.  y = x * RN(127 / max|x|) is off by at most 127 * 2^-23 < 2e-5, so only vectors with a y within 1e-4 of a
-// border between two codes are decided in 64 bits.  A row of zeros has scale 0 and codes 0; a row with an infinity or a NaN has
-// scale NaN and codes 0, so that its outputs are NaN and no other row's are.
-// WPR warps per row, eight per CTA.  With row_of_pair a row is a token and its codes go to the token's T sorted rows.
-// A thread keeps up to four vectors of the row in registers, so that rows of up to 4 * 32 * WPR vectors are read once.
-// Rounding adds 1.5 * 2^23: the sum's low byte is the code, and taking the constant off again gives the rounded value.
+// Rows to codes (the arithmetic: I8RowScale).  WPR warps per row, eight per CTA; a thread keeps up to four vectors of the
+// row in registers, so that rows of up to 4 * 32 * WPR vectors are read once.  With row_of_pair a row is a token and its
+// codes go to the token's T sorted rows.
 // ---------------------------------------------------------------------------------
-constexpr float I8_ROUND = 12582912.f;
 constexpr int I8_KEPT = 4;
-
-template <typename R>
-__device__ __forceinline__ void i8_codes(const R& v, float up, float inv, float amax, uint32_t (&w)[2]) {
-    float t[R::N], far = 0.f;
-#pragma unroll
-    for (int k = 0; k < R::N; ++k) {
-        const float y = v.get(k) * up * inv;
-        t[k] = y + I8_ROUND;
-        far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
-    }
-    if (far > 0.5f - 1e-4f) {                            // next to a border
-#pragma unroll
-        for (int k = 0; k < R::N; ++k) t[k] = I8_ROUND + (float)rint(127.0 * (double)(v.get(k) * up) / (double)amax);
-    }
-#pragma unroll
-    for (int h = 0; h < (R::N + 3) / 4; ++h) {
-        uint32_t b[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) b[k] = 4 * h + k < R::N ? __float_as_uint(t[4 * h + k < R::N ? 4 * h + k : 0]) : 0u;
-        w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    }
-}
 
 template <typename T_, int VB, int WPR>
 __global__ void __launch_bounds__(256)
@@ -76,21 +49,16 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
         for (int w = 0; w < WPR; ++w) top = max(top, s_max[warp / WPR * WPR + w]);
     }
     if (!on) return;
-    const bool finite = top < 0x7f800000u;
-    float amax = __uint_as_float(top);
-    const float scale = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
-    const float up = amax < 0x1p-100f ? 0x1p100f : 1.f;  // keeps 127 / max|x| in range; exact
-    amax *= up;
-    const float inv = finite && amax > 0.f ? 127.f / amax : 0.f;
+    const I8RowScale rs(top);
     const int copies = row_of_pair ? T : 1;
     if (part == 0)
         for (int t = 0; t < copies; ++t) {
             const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
-            if (r >= 0) scales[r] = scale;
+            if (r >= 0) scales[r] = rs.scale;
         }
     auto put = [&](const R& v, int c) {
         uint32_t w[2] = {0, 0};
-        if (inv > 0.f) i8_codes(v, up, inv, amax, w);
+        rs.codes(v, w);
         for (int t = 0; t < copies; ++t) {
             const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
             if (r < 0) continue;
@@ -201,6 +169,78 @@ static int launch_i8_tile(const I8Problem& p, cudaStream_t st) {
                                 : cudaLaunchKernelEx(&cfg, i8_tile_kernel<false>, p, (int)aa, (int)aw));
 }
 
+// Rows of any alignment to rows that start on 16-byte boundaries (columns behind K become zero).
+__global__ void __launch_bounds__(256)
+i8_pack_kernel(const int8_t* q, long long q_stride, long long rows, int K, int8_t* out, long long out_stride) {
+    pdl_begin();
+    const int vecs = (K + 15) / 16;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * vecs) return;
+    const long long r = i / vecs;
+    const int k = (int)(i - r * vecs) * 16;
+    const int8_t* src = q + r * q_stride + k;
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = i8_word(src, 4 * j, K - k, ((uintptr_t)src & 3) == 0);
+    // the row's last vector may have no room for its zeros
+    int8_t* dst = out + r * out_stride + k;
+    if (k + 16 <= out_stride) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else
+        for (int j = 0; k + j < K; ++j) dst[j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
+}
+
+static int i8_pitch(int K) { return (K + 15) / 16 * 16; }
+static size_t i8_align(size_t n) { return (n + 255) & ~(size_t)255; }
+
+static int i8_problem(I8Problem* p, const int8_t* a, long long a_stride, const float* a_scale, int M, const int8_t* w, long long w_stride,
+                      long long w_expert_stride, const float* w_scale, int N, int K, int E, const int32_t* expert_offsets, int swiglu,
+                      int zero_tail, void* out, long long out_stride, int out_dtype) {
+    if (M < 0 || N <= 0 || K < 0 || E <= 0 || out_dtype < VMOE_BF16 || out_dtype > VMOE_F32) return VMOE_ERR_SHAPE;
+    if (a_stride < 0 || w_stride < 0 || w_expert_stride < 0 || out_stride < N || (!expert_offsets && E != 1)) return VMOE_ERR_SHAPE;
+    if (K > I8_MAX_K || E > 65535 || N > (1 << 30)) return VMOE_ERR_LIMIT;
+    if (M == 0) return VMOE_OK;
+    if (!w_scale || !out || (K > 0 && !w)) return VMOE_ERR_NULL;
+    if ((uintptr_t)out & (out_dtype == VMOE_F32 ? 3 : 1)) return VMOE_ERR_ALIGN;
+    p->a = a; p->a_stride = M == 1 ? i8_pitch(K) : a_stride; p->a_scale = a_scale;      // the stride of a single row says nothing
+    p->wrows = swiglu ? 2 * N : N;
+    p->w = w; p->w_stride = p->wrows == 1 ? i8_pitch(K) : w_stride; p->w_expert_stride = w_expert_stride; p->w_scale = w_scale;
+    p->out = out; p->out_stride = out_stride; p->offsets = expert_offsets;
+    p->M = M; p->N = N; p->K = K; p->E = E; p->swiglu = swiglu; p->out_dtype = out_dtype; p->zero_tail = zero_tail;
+    return VMOE_OK;
+}
+
+// The kernel of a product, by its sizes and the alignment of its operands.
+static int i8_product(const I8Problem& p, cudaStream_t st) {
+    if (i8_gemv_ok(p)) return launch_i8_gemv(p, nullptr, 0, 0, st);
+    if (!i8_tc_ok(p) || p.E > I8_TC_MAX_EXPERTS) return launch_i8_tile(p, st);
+    if (!p.offsets) {
+        const long long items = (p.M + 127LL) / 128 * ((p.N + (p.swiglu ? 127LL : 255LL)) / (p.swiglu ? 128 : 256));
+        if (items < 148) return launch_i8_split(p, st);
+    }
+    return launch_i8_tc(p, st);
+}
+
+struct I8ExpertsScratch { size_t offsets, row_of_pair, pair_of_row, counts, counts_bytes, scale, q1, h, q2, y, total; };
+// false: sizes the plan does not take.  The f32 rows of the second product (y) take the place of the first one's operands.
+static bool i8_experts_scratch(int M, int T, int E, int K, int N, I8ExpertsScratch* s) {
+    if (M < 0 || T <= 0 || T > MAX_TOPK || E <= 0 || E > 8192 || K <= 0 || N <= 0 || (long long)M * T > 0x7fffffffLL - 1024) return false;
+    const size_t P = (size_t)M * T;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += i8_align(bytes); return here; };
+    s->offsets = take(((size_t)E + 1) * 4);
+    s->row_of_pair = take(P * 4);
+    s->pair_of_row = take(P * 4);
+    s->counts_bytes = vmoe_plan_scratch_bytes(M, T, E);
+    s->counts = take(s->counts_bytes);
+    s->scale = take(P * 4);
+    s->q2 = take(P * i8_pitch(N));
+    s->y = s->q1 = take(P * i8_pitch(K));
+    s->h = take(P * N * 4);
+    const size_t y_end = s->y + i8_align(P * K * 4);
+    s->total = at > y_end ? at : y_end;
+    return true;
+}
+
 }  // namespace vmoe
 
 using namespace vmoe;
@@ -243,26 +283,91 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
 int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, int32_t M, const int8_t* w, int64_t w_stride,
                      int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
                      int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream) {
-    if (M < 0 || N <= 0 || K < 0 || E <= 0 || out_dtype < VMOE_BF16 || out_dtype > VMOE_F32) return VMOE_ERR_SHAPE;
-    if (a_stride < 0 || w_stride < 0 || w_expert_stride < 0 || out_stride < N || (!expert_offsets && E != 1)) return VMOE_ERR_SHAPE;
-    if (K > I8_MAX_K || E > 65535 || N > (1 << 30)) return VMOE_ERR_LIMIT;
-    if (M == 0) return VMOE_OK;
-    if (!a_scale || !w_scale || !out || (K > 0 && (!a || !w))) return VMOE_ERR_NULL;
-    if ((uintptr_t)out & (out_dtype == VMOE_F32 ? 3 : 1)) return VMOE_ERR_ALIGN;
     I8Problem p;
-    p.a = a; p.a_stride = a_stride; p.a_scale = a_scale;
-    p.w = w; p.w_stride = w_stride; p.w_expert_stride = w_expert_stride; p.w_scale = w_scale;
-    p.out = out; p.out_stride = out_stride; p.offsets = expert_offsets;
-    p.M = M; p.N = N; p.K = K; p.E = E; p.wrows = swiglu ? 2 * N : N; p.swiglu = swiglu; p.out_dtype = out_dtype; p.zero_tail = zero_tail;
-    if (M == 1) p.a_stride = (K + 15) / 16 * 16;             // the stride of a single row says nothing
-    if (p.wrows == 1) p.w_stride = (K + 15) / 16 * 16;
+    const int rc = i8_problem(&p, a, a_stride, a_scale, M, w, w_stride, w_expert_stride, w_scale, N, K, E, expert_offsets, swiglu,
+                              zero_tail, out, out_stride, out_dtype);
+    if (rc || M == 0) return rc;
+    if (!a_scale || (K > 0 && !a)) return VMOE_ERR_NULL;
+    return i8_product(p, static_cast<cudaStream_t>(stream));
+}
+
+size_t vmoe_int8_linear_scratch_bytes(int32_t M, int32_t K) {
+    if (M <= 0 || K < 0 || K > I8_MAX_K) return 0;
+    return i8_align((size_t)M * i8_pitch(K)) + (size_t)M * sizeof(float);
+}
+
+int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, const int8_t* w, int64_t w_stride, const float* w_scale,
+                     int32_t N, int32_t K, int32_t swiglu, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
+                     size_t scratch_bytes, void* stream) {
+    if (dtype < VMOE_BF16 || dtype > VMOE_F32 || x_stride < 0) return VMOE_ERR_SHAPE;
+    uint8_t* const base = static_cast<uint8_t*>(scratch);
+    I8Problem p;
+    const int pitch = i8_pitch(K > 0 && K <= I8_MAX_K ? K : 0);
+    int rc = i8_problem(&p, nullptr, pitch, nullptr, M, w, w_stride, 0, w_scale, N, K, 1, nullptr, swiglu, 0, out, out_stride, out_dtype);
+    if (rc || M == 0) return rc;
+    if (K > 0 && !x) return VMOE_ERR_NULL;
+    const long long el = dtype == VMOE_F32 ? 4 : 2;
+    if ((uintptr_t)x & (el - 1)) return VMOE_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!i8_tc_ok(p) || E > I8_TC_MAX_EXPERTS) return launch_i8_tile(p, st);
-    if (!expert_offsets) {
-        const long long items = (M + 127LL) / 128 * ((N + (swiglu ? 127LL : 255LL)) / (swiglu ? 128 : 256));
-        if (items < 148) return launch_i8_split(p, st);
-    }
-    return launch_i8_tc(p, st);
+    if (i8_gemv_ok(p)) return launch_i8_gemv(p, x, x_stride * el, dtype, st);
+    if (!scratch || scratch_bytes < vmoe_int8_linear_scratch_bytes(M, K)) return VMOE_ERR_WORKSPACE;
+    if ((uintptr_t)scratch & 15) return VMOE_ERR_ALIGN;
+    int8_t* q = reinterpret_cast<int8_t*>(base);
+    float* scale = reinterpret_cast<float*>(base + i8_align((size_t)M * pitch));
+    if ((rc = vmoe_int8_quantize(x, x_stride, dtype, M, K, 0, nullptr, nullptr, q, pitch, scale, stream))) return rc;
+    p.a = q; p.a_scale = scale;
+    return i8_product(p, st);
+}
+
+int vmoe_int8_pack(const int8_t* q, int64_t q_stride, int64_t rows, int32_t K, int8_t* out, int64_t out_stride, void* stream) {
+    if (rows < 0 || K < 0 || q_stride < 0 || out_stride < K) return VMOE_ERR_SHAPE;
+    if (rows == 0 || K == 0) return VMOE_OK;
+    if (!q || !out) return VMOE_ERR_NULL;
+    if (((uintptr_t)out | (unsigned long long)out_stride) & 15) return VMOE_ERR_ALIGN;
+    const long long blocks = (rows * ((K + 15) / 16) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return VMOE_ERR_LIMIT;
+    return cuda_status(launch_pdl(i8_pack_kernel, (unsigned)blocks, 256u, 0, static_cast<cudaStream_t>(stream), q, (long long)q_stride,
+                                  (long long)rows, K, out, (long long)out_stride));
+}
+
+size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N) {
+    I8ExpertsScratch s;
+    return i8_experts_scratch(M, T, E, K, N, &s) ? s.total : 0;
+}
+
+int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K, int32_t N,
+                      const int32_t* topk_ids, const float* topk_weights, const int32_t* expert_map, int32_t map_len,
+                      const int8_t* w13, int64_t w13_stride, int64_t w13_expert_stride, const float* w13_scale,
+                      const int8_t* w2, int64_t w2_stride, int64_t w2_expert_stride, const float* w2_scale,
+                      void* out, int64_t out_stride, int32_t out_dtype, void* scratch, size_t scratch_bytes, void* stream) {
+    if (dtype < VMOE_BF16 || dtype > VMOE_F32 || x_stride < 0 || K <= 0 || N <= 0) return VMOE_ERR_SHAPE;
+    if (M < 0 || T <= 0 || E <= 0) return VMOE_ERR_SHAPE;
+    if (K > I8_MAX_K || N > I8_MAX_K) return VMOE_ERR_LIMIT;
+    I8ExpertsScratch L;
+    if (!i8_experts_scratch(M, T, E, K, N, &L)) return VMOE_ERR_LIMIT;
+    if (M == 0) return VMOE_OK;
+    if (!x || !topk_ids || !topk_weights || !w13 || !w2 || !w13_scale || !w2_scale || !out) return VMOE_ERR_NULL;
+    if (!scratch || scratch_bytes < L.total) return VMOE_ERR_WORKSPACE;
+    if ((uintptr_t)scratch & 15) return VMOE_ERR_ALIGN;
+    uint8_t* const b = static_cast<uint8_t*>(scratch);
+    int32_t* offsets = reinterpret_cast<int32_t*>(b + L.offsets);
+    int32_t* row_of_pair = reinterpret_cast<int32_t*>(b + L.row_of_pair);
+    float* scale = reinterpret_cast<float*>(b + L.scale);
+    int8_t* q1 = reinterpret_cast<int8_t*>(b + L.q1);
+    float* h = reinterpret_cast<float*>(b + L.h);
+    int8_t* q2 = reinterpret_cast<int8_t*>(b + L.q2);
+    float* y = reinterpret_cast<float*>(b + L.y);
+    const int P = M * T;
+    int rc;
+    if ((rc = vmoe_plan_tokens(topk_ids, expert_map, map_len, M, T, E, offsets, row_of_pair, reinterpret_cast<int32_t*>(b + L.pair_of_row),
+                               b + L.counts, L.counts_bytes, stream))) return rc;
+    if ((rc = vmoe_int8_quantize(x, x_stride, dtype, M, K, T, row_of_pair, nullptr, q1, i8_pitch(K), scale, stream))) return rc;
+    if ((rc = vmoe_int8_matmul(q1, i8_pitch(K), scale, P, w13, w13_stride, w13_expert_stride, w13_scale, N, K, E, offsets, 1, 0, h, N, VMOE_F32,
+                               stream))) return rc;
+    if ((rc = vmoe_int8_quantize(h, N, VMOE_F32, P, N, 0, nullptr, offsets + E, q2, i8_pitch(N), scale, stream))) return rc;
+    if ((rc = vmoe_int8_matmul(q2, i8_pitch(N), scale, P, w2, w2_stride, w2_expert_stride, w2_scale, K, N, E, offsets, 0, 0, y, K, VMOE_F32,
+                               stream))) return rc;
+    return vmoe_unsort_tokens(y, K, VMOE_F32, M, T, K, row_of_pair, topk_weights, out, out_stride, out_dtype, stream);
 }
 
 }  // extern "C"

@@ -29,6 +29,67 @@ __device__ __forceinline__ void i8_store(void* out, long long at, int dtype, flo
     else static_cast<__half*>(out)[at] = __float2half_rn(v);
 }
 
+// ---------------------------------------------------------------------------------
+// Row quantiser: scale = max|x| / 127, code = rint(127 x / max|x|), ties to even -- the code of the exact quotient, not of
+// a rounded one.  inv = 127 * RN(1 / max|x|) and y = x * inv carry three roundings, so y is off by less than 127 * 3 * 2^-24 <
+// 2.3e-5: only vectors with a y within 2.5e-5 of a border between two codes are decided in 64 bits.  A row of zeros has
+// scale 0 and codes 0; a row with an infinity or a NaN has scale NaN and codes 0, so that its outputs are NaN and no other
+// row's are.  Rounding adds 1.5 * 2^23: the sum's low byte is the code, and taking the constant off again gives the
+// rounded value.
+// ---------------------------------------------------------------------------------
+constexpr float I8_ROUND = 12582912.f;
+constexpr float I8_BORDER = 0.5f - 2.5e-5f;
+
+struct I8RowScale {
+    float scale, amax, up, inv;          // inv = 0: every code is 0
+    // top: the largest magnitude of the row as an integer, which orders NaN > infinity > finite
+    __device__ __forceinline__ explicit I8RowScale(uint32_t top) {
+        const bool finite = top < 0x7f800000u;
+        amax = __uint_as_float(top);
+        // by rcp.rn and a correction, exact for this divisor (Divider) while nothing underflows
+        scale = !finite ? __uint_as_float(0x7fc00000u) : amax >= 0x1p-100f ? Divider(127.f)(amax) : amax / 127.f;
+        up = amax < 0x1p-100f ? 0x1p100f : amax > 0x1p100f ? 0x1p-100f : 1.f;     // keeps 1 / max|x| a normal number; exact
+        amax *= up;
+        float r;
+        asm("rcp.rn.f32 %0, %1;" : "=f"(r) : "f"(amax));
+        inv = finite && amax > 0.f ? 127.f * r : 0.f;
+    }
+    __device__ __forceinline__ float exact(float x) const { return (float)rint(127.0 * (double)(x * up) / (double)amax); }
+    __device__ __forceinline__ int code(float x) const {
+        if (inv == 0.f) return 0;
+        const float y = x * up * inv, r = rintf(y);
+        return (int)(fabsf(y - r) > I8_BORDER ? exact(x) : r);
+    }
+    // the codes of a vector, four to a word
+    template <typename R>
+    __device__ __forceinline__ void codes(const R& v, uint32_t (&w)[2]) const {
+        if (inv == 0.f) { w[0] = w[1] = 0; return; }
+        float t[R::N], far = 0.f;
+#pragma unroll
+        for (int k = 0; k < R::N; ++k) {
+            const float y = v.get(k) * up * inv;
+            t[k] = y + I8_ROUND;
+            far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
+        }
+        if (far > I8_BORDER) {
+#pragma unroll
+            for (int k = 0; k < R::N; ++k) t[k] = I8_ROUND + exact(v.get(k));
+        }
+#pragma unroll
+        for (int h = 0; h < (R::N + 3) / 4; ++h) {
+            uint32_t b[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) b[k] = 4 * h + k < R::N ? __float_as_uint(t[4 * h + k < R::N ? 4 * h + k : 0]) : 0u;
+            w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+        }
+    }
+};
+
+// A few rows (vmoe_int8_gemv.cu): x, when not NULL, holds them as bf16 / fp16 / f32 and p.a is not read.
+constexpr int I8_GEMV_ROWS = 8;
+bool i8_gemv_ok(const I8Problem& p);
+int  launch_i8_gemv(const I8Problem& p, const void* x, long long x_stride_bytes, int x_dtype, cudaStream_t st);
+
 // tensor-core kernels (vmoe_int8_tc.cu)
 constexpr int I8_TC_MAX_EXPERTS = 16384;                 // their tables lie in shared memory
 bool i8_tc_ok(const I8Problem& p);                       // addresses and strides are multiples of 16 bytes

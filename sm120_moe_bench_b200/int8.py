@@ -12,28 +12,23 @@ while gradients are enabled.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
-from ._lib import check, lib
-from .token_sort import DTYPE_CODES, TokenPlan, _on, _unsort, check_out, check_rows, plan_tokens
+from ._lib import lib
+from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_TOPK, TokenPlan, check_out, check_rows, launch
 
 MAX_K = 131071
 
 
-@dataclass(frozen=True, eq=False)
 class Int8Rows:
     """Rows of 8-bit codes ``q`` int8 ``[..., rows, K]`` and a scale each, ``scale`` f32 ``[..., rows]``: row = q * scale.
 
     A row's codes lie next to each other; rows (and the matrices of several experts) may have any stride.  Where address
     and strides are multiples of 16 bytes the tensor cores read them as they are; ``quantize_int8`` makes them so."""
 
-    q: torch.Tensor
-    scale: torch.Tensor
+    __slots__ = ("q", "scale")
 
-    def __post_init__(self):
-        q, scale = self.q, self.scale
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         if not q.is_cuda or q.dtype != torch.int8 or q.dim() not in (2, 3):
             raise ValueError("q must be an int8 CUDA tensor [rows, K] or [experts, rows, K]")
         if scale.dtype != torch.float32 or scale.device != q.device or scale.shape != q.shape[:-1] or not scale.is_contiguous():
@@ -42,6 +37,8 @@ class Int8Rows:
             raise ValueError("the codes of a row must lie next to each other")
         if q.shape[-1] > MAX_K:
             raise ValueError(f"rows of at most {MAX_K} codes")
+        self.q = q
+        self.scale = scale
 
     def dequantize(self) -> torch.Tensor:
         """f32 values."""
@@ -60,15 +57,14 @@ def _codes(rows: int, K: int, device) -> torch.Tensor:
     return q if pitch == K else q[:, :K]
 
 
-def _quantize(x, plan: TokenPlan | None = None, live: torch.Tensor | None = None):
+def _quantize(x, plan: TokenPlan | None = None):
     M, K = x.shape
     rows = M if plan is None else plan.rows
     q = _codes(rows, K, x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with _on(x.device) as stream:
-        check(lib.vmoe_int8_quantize(x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, K, 0 if plan is None else plan.topk,
-                                     None if plan is None else plan.row_of_pair.data_ptr(), None if live is None else live.data_ptr(),
-                                     q.data_ptr(), max(q.stride(0), K), scale.data_ptr(), stream), "vmoe_int8_quantize")
+    launch(x.device, "vmoe_int8_quantize", lib.vmoe_int8_quantize, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, K,
+           0 if plan is None else plan.topk, None if plan is None else plan.row_of_pair.data_ptr(), None, q.data_ptr(),
+           max(q.stride(0), K), scale.data_ptr())
     return q, scale
 
 
@@ -94,16 +90,32 @@ def quantize_int8(x: torch.Tensor, plan: TokenPlan | None = None) -> Int8Rows:
     return Int8Rows(*_quantize(x, plan))
 
 
-def _matmul(q, scale, w: Int8Rows, N: int, offsets, swiglu: bool, zero_tail: bool, out):
-    M, K = q.shape
-    wq = w.q
-    grouped = wq.dim() == 3
-    with _on(q.device) as stream:
-        check(lib.vmoe_int8_matmul(q.data_ptr(), q.stride(0), scale.data_ptr(), M, wq.data_ptr(), wq.stride(-2),
-                                   wq.stride(0) if grouped else 0, w.scale.data_ptr(), N, K, wq.shape[0] if grouped else 1,
-                                   None if offsets is None else offsets.data_ptr(), swiglu, zero_tail, out.data_ptr(),
-                                   max(out.stride(0), N), DTYPE_CODES[out.dtype], stream), "vmoe_int8_matmul")
-    return out
+def _aligned(q: torch.Tensor) -> bool:
+    """Whether the tensor cores can read these rows as they are."""
+    return (q.data_ptr() | q.stride(-2) | (q.stride(0) if q.dim() == 3 else 0)) % 16 == 0
+
+
+def _pack(q: torch.Tensor) -> torch.Tensor:
+    """The same codes in rows that start on 16-byte boundaries."""
+    K = q.shape[-1]
+    pitch = (K + 15) // 16 * 16
+    out = torch.empty((*q.shape[:-1], pitch), dtype=torch.int8, device=q.device)
+    if q.dim() == 3 and q.stride(0) != q.shape[1] * q.stride(1):
+        parts = zip(q, out)                               # matrices with gaps between them
+    else:
+        parts = ((q, out),)
+    for src, dst in parts:
+        launch(q.device, "vmoe_int8_pack", lib.vmoe_int8_pack, src.data_ptr(), src.stride(-2), src.numel() // K, K, dst.data_ptr(), pitch)
+    return out[..., :K]
+
+
+def _operand(w: Int8Rows, rows: int) -> torch.Tensor:
+    """The codes of the weights for a product with ``rows`` rows: packed first where that pays.  The kernel for unaligned rows does
+    about 80 TOPS on them; packing moves twice the weights' bytes and the tensor cores do the rest, which pays from about 13
+    rows per matrix."""
+    q = w.q
+    experts = q.shape[0] if q.dim() == 3 else 1
+    return q if q.shape[-1] == 0 or rows < 16 * experts or _aligned(q) else _pack(q)
 
 
 def int8_status(device: torch.device | str | int = "cuda") -> int:
@@ -151,7 +163,15 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
         if out.device != a.q.device or out.shape[1] != N:
             raise ValueError(f"out must have {N} columns on {a.q.device}")
         _no_grad(out, "out")
-    return _matmul(a.q, a.scale, w, N, None if plan is None else plan.expert_offsets, swiglu, out is None, y)
+    M, K = a.q.shape
+    aq, wq = a.q, _operand(w, M)
+    if M >= 16 and K and not _aligned(aq) and (wq is not w.q or _aligned(wq)):
+        aq = _pack(aq)
+    launch(aq.device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, aq.data_ptr(), aq.stride(0), a.scale.data_ptr(), M, wq.data_ptr(),
+           wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, 1 if plan is None else plan.num_experts,
+           None if plan is None else plan.expert_offsets.data_ptr(), swiglu, out is None, y.data_ptr(), max(y.stride(0), N),
+           DTYPE_CODES[y.dtype])
+    return y
 
 
 def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -166,8 +186,16 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
         if out.dtype != x.dtype or out.shape[1] != N or (x.shape[0] > 1 and out.stride(0) < N):
             raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
         _no_grad(out, "out")
-    q, scale = _quantize(x)
-    return _matmul(q, scale, w, N, None, swiglu, False, out)
+    M, K = x.shape
+    wq = _operand(w, M)
+    # a few rows are quantised inside the product
+    inside = M <= 8 and K <= 8192 and (wq.data_ptr() | wq.stride(0)) % 4 == 0
+    need = 0 if inside else lib.vmoe_int8_linear_scratch_bytes(M, K)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    launch(x.device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, wq.data_ptr(),
+           wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), max(out.stride(0), N), DTYPE_CODES[out.dtype],
+           scratch.data_ptr() if need else None, need)
+    return out
 
 
 def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
@@ -179,6 +207,8 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
     everything between is f32, and the sum is rounded once to the type of ``x``.  ``expert_map`` as in ``plan_tokens``."""
     _no_grad(x, "x")
     _no_grad(topk_weights, "topk_weights")
+    if topk_ids.dim() != 2:
+        raise ValueError("topk_ids must be an int32 tensor [tokens, choices]")
     check_rows(x, "x", topk_ids.shape[0], topk_ids.device)
     if w13.q.dim() != 3 or w2.q.dim() != 3:
         raise ValueError("w13 and w2 hold one matrix per expert")
@@ -189,12 +219,21 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
     if topk_weights.dtype != torch.float32 or topk_weights.shape != topk_ids.shape or topk_weights.device != x.device \
             or not topk_weights.is_contiguous():
         raise ValueError("topk_weights must be a contiguous float32 tensor of the shape of topk_ids")
-    plan = plan_tokens(topk_ids, E, expert_map)
-    kept = plan.expert_offsets[E:]
-    q, scale = _quantize(x, plan)
-    h = torch.empty(plan.rows, N, dtype=torch.float32, device=x.device)
-    _matmul(q, scale, w13, N, plan.expert_offsets, True, False, h)
-    q, scale = _quantize(h, None, kept)
-    y = torch.empty(plan.rows, K, dtype=torch.float32, device=x.device)
-    _matmul(q, scale, w2, K, plan.expert_offsets, False, False, y)
-    return _unsort(y, plan, topk_weights, torch.empty_like(x, memory_format=torch.contiguous_format))
+    if topk_ids.dtype != torch.int32 or not topk_ids.is_contiguous():
+        raise ValueError("topk_ids must be a contiguous int32 tensor [tokens, choices]")
+    M, T = topk_ids.shape
+    if not 1 <= T <= MAX_TOPK or E > MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_TOPK} choices per token and at most {MAX_EXPERTS} experts, got {T} and {E}")
+    if expert_map is not None and (expert_map.device != x.device or expert_map.dtype != torch.int32 or expert_map.dim() != 1
+                                   or not expert_map.is_contiguous() or expert_map.numel() == 0):
+        raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids, not empty")
+    q13, q2 = _operand(w13, M * T), _operand(w2, M * T)
+    out = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    need = lib.vmoe_int8_experts_scratch_bytes(M, T, E, K, N)
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+    launch(x.device, "vmoe_int8_experts", lib.vmoe_int8_experts, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, T, E, K, N,
+           topk_ids.data_ptr(), topk_weights.data_ptr(), None if expert_map is None else expert_map.data_ptr(),
+           0 if expert_map is None else expert_map.numel(), q13.data_ptr(), q13.stride(1), q13.stride(0), w13.scale.data_ptr(),
+           q2.data_ptr(), q2.stride(1), q2.stride(0), w2.scale.data_ptr(), out.data_ptr(), K, DTYPE_CODES[out.dtype], scratch.data_ptr(),
+           need)
+    return out

@@ -56,3 +56,38 @@ def test_host_tensors_are_refused():
         vm.quantize_int8(torch.zeros(4, 16))
     with pytest.raises(ValueError, match="gradient"):
         vm.quantize_int8(torch.zeros(4, 16, requires_grad=True))
+
+
+def test_linear_pack_and_experts_checks():
+    lib, keep = _lib(), _buf()
+    b = ctypes.addressof(keep) & ~15
+    assert lib.vmoe_int8_linear_scratch_bytes(0, 64) == 0 and lib.vmoe_int8_linear_scratch_bytes(3, 131072) == 0
+    assert lib.vmoe_int8_linear_scratch_bytes(9, 100) >= 9 * 112 + 36
+
+    def linear(x=b, xs=16, dtype=0, M=16, w=b, ws=16, sw=b, N=8, K=16, out=b, os_=8, to=0, scratch=b, bytes_=4096):
+        return lib.vmoe_int8_linear(x, xs, dtype, M, w, ws, sw, N, K, 0, out, os_, to, scratch, bytes_, None)
+
+    assert linear(M=0) == 0
+    assert linear(dtype=3) == 2 and linear(xs=-1) == 2 and linear(M=-1) == 2 and linear(N=0) == 2 and linear(os_=7) == 2 and linear(K=131072) == 8
+    assert linear(x=None) == 1 and linear(w=None) == 1 and linear(sw=None) == 1 and linear(out=None) == 1
+    assert linear(x=b + 1) == 3 and linear(scratch=b + 8) == 3
+    assert linear(scratch=None) == 4 and linear(bytes_=16) == 4
+
+    pack = lambda q=b, qs=20, rows=3, K=20, out=b, os_=32: lib.vmoe_int8_pack(q, qs, rows, K, out, os_, None)
+    assert pack(rows=0) == 0 and pack(K=0) == 0
+    assert pack(rows=-1) == 2 and pack(os_=16) == 2 and pack(q=None) == 1 and pack(out=None) == 1 and pack(os_=24) == 3 and pack(out=b + 4) == 3
+
+    size = lib.vmoe_int8_experts_scratch_bytes
+    assert size(4, 17, 8, 64, 32) == 0 and size(4, 2, 8193, 64, 32) == 0 and size(2 ** 28, 16, 8, 64, 32) == 0
+    assert size(64, 10, 512, 4096, 1024) >= 640 * 4096 * 4
+
+    def experts(x=b, dtype=0, M=4, T=2, E=4, K=32, N=16, ids=b, wt=b, w13=b, s13=b, w2=b, s2=b, out=b, scratch=b, bytes_=1 << 40):
+        return lib.vmoe_int8_experts(x, K, dtype, M, T, E, K, N, ids, wt, None, 0, w13, K, 2 * N * K, s13, w2, N, N * K, s2, out, K, 0,
+                                     scratch, bytes_, None)
+
+    assert experts(M=0) == 0
+    assert experts(dtype=3) == 2 and experts(M=-1) == 2 and experts(K=0) == 2 and experts(N=0) == 2 and experts(E=0) == 2
+    assert experts(K=131072) == 8 and experts(T=17) == 8 and experts(E=8193) == 8
+    for name in ("x", "ids", "wt", "w13", "s13", "w2", "s2", "out"):
+        assert experts(**{name: None}) == 1, name
+    assert experts(scratch=None) == 4 and experts(bytes_=64) == 4 and experts(scratch=b + 8) == 3
