@@ -10,11 +10,12 @@ namespace vmoe {
 // ---------------------------------------------------------------------------------
 constexpr int I8_KEPT = 4;
 
-template <typename T_, int VB, int WPR>
+template <typename T_, int VB, int WPR, bool SORTED>
 __global__ void __launch_bounds__(256)
 i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vecs, int T, const int32_t* row_of_pair,
                    const int32_t* live, int8_t* q, long long q_stride, float* scales) {
     using R = RowVec<T_, VB>;
+    constexpr int STEP = WPR * 32;
     __shared__ uint32_t s_max[8];
     pdl_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -22,26 +23,22 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
     const int part = (warp % WPR) * 32 + lane;
     const bool on = m < rows && (!live || m < *live);
     const uint8_t* src = x + m * x_stride;
-    uint32_t top = 0;                                    // magnitudes ordered as integers: NaN > infinity > finite
+    uint32_t top = 0;
     R keep[I8_KEPT];
     if (on) {
 #pragma unroll
         for (int i = 0; i < I8_KEPT; ++i)
-            if (part + i * WPR * 32 < vecs) keep[i].load(src, part + i * WPR * 32);
+            if (part + i * STEP < vecs) keep[i].load(src, part + i * STEP);
 #pragma unroll
         for (int i = 0; i < I8_KEPT; ++i)
-            if (part + i * WPR * 32 < vecs) {
-#pragma unroll
-                for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(keep[i].get(k)) & 0x7fffffffu);
-            }
-        for (int c = part + I8_KEPT * WPR * 32; c < vecs; c += WPR * 32) {
+            if (part + i * STEP < vecs) top = keep[i].join(top);
+        for (int c = part + I8_KEPT * STEP; c < vecs; c += STEP) {
             R v;
             v.load(src, c);
-#pragma unroll
-            for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(v.get(k)) & 0x7fffffffu);
+            top = v.join(top);
         }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    top = __reduce_max_sync(0xffffffffu, R::magnitude(top));
     if (WPR > 1) {
         if (lane == 0) s_max[warp] = top;
         __syncthreads();
@@ -50,33 +47,48 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
     }
     if (!on) return;
     const I8RowScale rs(top);
-    const int copies = row_of_pair ? T : 1;
-    if (part == 0)
-        for (int t = 0; t < copies; ++t) {
-            const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
-            if (r >= 0) scales[r] = rs.scale;
-        }
+    const int32_t* rp = SORTED ? row_of_pair + m * T : nullptr;
+    if (SORTED) {
+        for (int t = part; t < T; t += STEP)
+            if (rp[t] >= 0) scales[rp[t]] = rs.scale;
+    } else if (part == 0) {
+        scales[m] = rs.scale;
+    }
+    auto store = [&](long long r, int c, const uint32_t (&w)[2]) {
+        int8_t* dst = q + r * q_stride + (long long)c * R::N;
+        if (R::N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+        else if (R::N == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+        else if (R::N == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w[0];
+        else *dst = (int8_t)w[0];
+    };
     auto put = [&](const R& v, int c) {
-        uint32_t w[2] = {0, 0};
+        uint32_t w[2];
         rs.codes(v, w);
-        for (int t = 0; t < copies; ++t) {
-            const long long r = row_of_pair ? row_of_pair[m * T + t] : m;
-            if (r < 0) continue;
-            int8_t* dst = q + r * q_stride + (long long)c * R::N;
-            if (R::N == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-            else if (R::N == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
-            else if (R::N == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)w[0];
-            else *dst = (int8_t)w[0];
+        if (SORTED) {
+            for (int t = 0; t < T; ++t)
+                if (rp[t] >= 0) store(rp[t], c, w);
+        } else {
+            store(m, c, w);
         }
     };
 #pragma unroll
     for (int i = 0; i < I8_KEPT; ++i)
-        if (part + i * WPR * 32 < vecs) put(keep[i], part + i * WPR * 32);
-    for (int c = part + I8_KEPT * WPR * 32; c < vecs; c += WPR * 32) {
+        if (part + i * STEP < vecs) put(keep[i], part + i * STEP);
+    for (int c = part + I8_KEPT * STEP; c < vecs; c += STEP) {
         R v;
         v.load(src, c);
         put(v, c);
     }
+}
+
+template <typename T_, int VB, int WPR>
+static int launch_quantize_rows(const void* x, long long xs, long long rows, int vecs, int T, const int32_t* row_of_pair, const int32_t* live,
+                                int8_t* q, long long q_stride, float* scales, cudaStream_t st) {
+    const unsigned grid = (unsigned)((rows + 8 / WPR - 1) / (8 / WPR));
+    const auto a = static_cast<const uint8_t*>(x);
+    return cuda_status(row_of_pair
+        ? launch_pdl(i8_quantize_kernel<T_, VB, WPR, true>, grid, 256u, 0, st, a, xs, rows, vecs, T, row_of_pair, live, q, q_stride, scales)
+        : launch_pdl(i8_quantize_kernel<T_, VB, WPR, false>, grid, 256u, 0, st, a, xs, rows, vecs, T, row_of_pair, live, q, q_stride, scales));
 }
 
 // ---------------------------------------------------------------------------------
@@ -264,19 +276,11 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
     return with_rows(dtype, vb, [&](auto r) {
         using R = decltype(r);
         const int vecs = K / R::N;
-        const auto a = static_cast<const uint8_t*>(x);
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        if (vecs <= 64)
-            return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 1>, (unsigned)((rows + 7LL) / 8), 256u, 0, st, a, xs,
-                                          (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
-        if (vecs <= 256)
-            return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 2>, (unsigned)((rows + 3LL) / 4), 256u, 0, st, a, xs,
-                                          (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
-        if (vecs <= 512)
-            return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 4>, (unsigned)((rows + 1LL) / 2), 256u, 0, st, a, xs,
-                                          (long long)rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales));
-        return cuda_status(launch_pdl(i8_quantize_kernel<typename R::T, R::BYTES, 8>, (unsigned)rows, 256u, 0, st, a, xs, (long long)rows,
-                                      vecs, T, row_of_pair, live_rows, q, q_stride, scales));
+        // four vectors a thread, and no fewer than two rows a CTA while they fit
+        if (vecs <= 128) return launch_quantize_rows<typename R::T, R::BYTES, 1>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        if (vecs <= 512) return launch_quantize_rows<typename R::T, R::BYTES, 4>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        return launch_quantize_rows<typename R::T, R::BYTES, 8>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
     });
 }
 

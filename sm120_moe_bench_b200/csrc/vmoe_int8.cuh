@@ -40,6 +40,9 @@ __device__ __forceinline__ void i8_store(void* out, long long at, int dtype, flo
 constexpr float I8_ROUND = 12582912.f;
 constexpr float I8_BORDER = 0.5f - 2.5e-5f;
 
+// (kept out of line: a rare path with long 64-bit divisions)
+static __device__ __noinline__ float i8_exact_code(float x, float amax) { return (float)rint(127.0 * (double)x / (double)amax); }
+
 struct I8RowScale {
     float scale, amax, up, inv;          // inv = 0: every code is 0
     // top: the largest magnitude of the row as an integer, which orders NaN > infinity > finite
@@ -54,7 +57,9 @@ struct I8RowScale {
         asm("rcp.rn.f32 %0, %1;" : "=f"(r) : "f"(amax));
         inv = finite && amax > 0.f ? 127.f * r : 0.f;
     }
-    __device__ __forceinline__ float exact(float x) const { return (float)rint(127.0 * (double)(x * up) / (double)amax); }
+    // neither a row of zeros nor one that needs `up`: almost every row
+    __device__ __forceinline__ bool plain() const { return up == 1.f && inv != 0.f; }
+    __device__ __forceinline__ float exact(float x) const { return i8_exact_code(x * up, amax); }
     __device__ __forceinline__ int code(float x) const {
         if (inv == 0.f) return 0;
         const float y = x * up * inv, r = rintf(y);
@@ -63,11 +68,17 @@ struct I8RowScale {
     // the codes of a vector, four to a word
     template <typename R>
     __device__ __forceinline__ void codes(const R& v, uint32_t (&w)[2]) const {
-        if (inv == 0.f) { w[0] = w[1] = 0; return; }
+        if (plain()) put<R, true>(v, w);
+        else if (inv != 0.f) put<R, false>(v, w);
+        else w[0] = w[1] = 0;
+    }
+private:
+    template <typename R, bool PLAIN>
+    __device__ __forceinline__ void put(const R& v, uint32_t (&w)[2]) const {
         float t[R::N], far = 0.f;
 #pragma unroll
         for (int k = 0; k < R::N; ++k) {
-            const float y = v.get(k) * up * inv;
+            const float y = (PLAIN ? v.get(k) : v.get(k) * up) * inv;
             t[k] = y + I8_ROUND;
             far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
         }

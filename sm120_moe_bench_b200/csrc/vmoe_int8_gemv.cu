@@ -52,17 +52,13 @@ __device__ __forceinline__ void i8_row_codes_vec(const T_* x, int K, int pitch, 
         if (tid + i * I8G_THREADS < vecs) keep[i].load(x, tid + i * I8G_THREADS);
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
-        if (tid + i * I8G_THREADS < vecs) {
-#pragma unroll
-            for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(keep[i].get(k)) & 0x7fffffffu);
-        }
+        if (tid + i * I8G_THREADS < vecs) top = keep[i].join(top);
     for (int c = tid + KEPT * I8G_THREADS; c < vecs; c += I8G_THREADS) {
         R v;
         v.load(x, c);
-#pragma unroll
-        for (int k = 0; k < R::N; ++k) top = max(top, __float_as_uint(v.get(k)) & 0x7fffffffu);
+        top = v.join(top);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    top = __reduce_max_sync(0xffffffffu, R::magnitude(top));
     __syncthreads();
     if ((tid & 31) == 0) s_max[tid >> 5] = top;
     __syncthreads();

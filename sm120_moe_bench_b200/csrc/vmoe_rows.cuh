@@ -29,6 +29,25 @@ struct RowVec {
     __device__ __forceinline__ void load(const void* row, long long c) { raw = static_cast<const Raw*>(row)[c]; }
     __device__ __forceinline__ void store(void* row, long long c) const { static_cast<Raw*>(row)[c] = raw; }
     __device__ __forceinline__ float get(int k) const { return elem_float(reinterpret_cast<const T_*>(half)[k]); }
+    // Largest magnitude, ordered as integers (NaN > infinity > finite), joined to `top`; with 16-bit elements two at a time,
+    // and `top` holds two 16-bit maxima until magnitude() takes the larger as an f32.
+    __device__ __forceinline__ uint32_t join(uint32_t top) const {
+        if constexpr (sizeof(T_) == 4) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) top = max(top, __float_as_uint(get(k)) & 0x7fffffffu);
+        } else if constexpr (BYTES >= 4) {
+#pragma unroll
+            for (int k = 0; k < BYTES / 4; ++k) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(half)[k] & 0x7fff7fffu);
+        } else {
+            top = __vmaxu2(top, half[0] & 0x7fffu);
+        }
+        return top;
+    }
+    __device__ static __forceinline__ uint32_t magnitude(uint32_t top) {
+        if constexpr (sizeof(T_) == 4) return top;
+        const uint16_t m = (uint16_t)max(top & 0xffffu, top >> 16);
+        return __float_as_uint(elem_float(*reinterpret_cast<const T_*>(&m))) & 0x7fffffffu;
+    }
     __device__ __forceinline__ void set(int k, float v) { elem_store(reinterpret_cast<T_*>(half)[k], v); }
 };
 

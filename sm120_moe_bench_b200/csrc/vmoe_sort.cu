@@ -25,7 +25,8 @@ namespace vmoe {
 // ---------------------------------------------------------------------------------
 constexpr int PLAN_MAX_EXPERTS = 8192;
 constexpr int PLAN_ONE_CTA_PAIRS = 4096;
-constexpr int PLAN_PAIRS_PER_CTA = 2048;
+constexpr int PLAN_PAIRS_PER_CTA = 4096;
+constexpr int PLAN_KEPT = 4;                 // experts of a lane's first pairs stay in registers between the passes
 constexpr int PLAN_MAX_CTAS = 64;
 constexpr int PLAN_SMEM = 200 * 1024;
 
@@ -76,24 +77,26 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     int* mine = count + (size_t)warp * E;
     const long long first = ((long long)rank * warps + warp) * run;
     const long long end = min(first + run, (long long)P);
-    {
-        int e = plan_expert(ids, expert_map, map_len, E, first + lane, end);
-        for (long long b = first; b < end; b += 32) {
-            const int next = plan_expert(ids, expert_map, map_len, E, b + 32 + lane, end);
-            if (e >= 0) atomicAdd(&mine[e], 1);
-            e = next;
-        }
+    int kept_e[PLAN_KEPT];
+#pragma unroll
+    for (int i = 0; i < PLAN_KEPT; ++i) kept_e[i] = plan_expert(ids, expert_map, map_len, E, first + 32 * i + lane, end);
+#pragma unroll
+    for (int i = 0; i < PLAN_KEPT; ++i)
+        if (kept_e[i] >= 0) atomicAdd(&mine[kept_e[i]], 1);
+    for (long long b = first + 32 * PLAN_KEPT; b < end; b += 32) {
+        const int e = plan_expert(ids, expert_map, map_len, E, b + lane, end);
+        if (e >= 0) atomicAdd(&mine[e], 1);
     }
     __syncthreads();
     for (int e = tid; e < E; e += threads) {
         int all = 0, front = 0;
         if (MANY) {
-            for (int r0 = 0; r0 < ctas; r0 += 8) {            // eight loads in flight
-                int n[8];
+            for (int r0 = 0; r0 < ctas; r0 += 16) {           // sixteen loads in flight
+                int n[16];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
+                for (int k = 0; k < 16; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
+                for (int k = 0; k < 16; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
             }
         } else {
             for (int w = 0; w < warps; ++w) all += count[(size_t)w * E + e];
@@ -138,24 +141,45 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
         for (int w = 0; w < warps; ++w) { const int n = count[(size_t)w * E + e]; count[(size_t)w * E + e] = row; row += n; }
     }
     __syncthreads();
-    {
-        int e = plan_expert(ids, expert_map, map_len, E, first + lane, end);
-        for (long long b = first; b < end; b += 32) {
-            const int next = plan_expert(ids, expert_map, map_len, E, b + 32 + lane, end);
-            const uint32_t same = __match_any_sync(0xffffffffu, e);
-            const int rank_in = __popc(same & ((1u << lane) - 1));
-            const int row = e >= 0 ? mine[e] + rank_in : -1;
-            __syncwarp();
-            if (e >= 0 && rank_in == 0) mine[e] += __popc(same);
-            __syncwarp();
-            if (b + lane < end) {
-                row_of_pair[b + lane] = row;
-                if (row >= 0) pair_of_row[row] = (int)(b + lane);
-            }
-            e = next;
+    auto place = [&](long long p, int e) {               // one pair per lane, the whole warp
+        const uint32_t same = __match_any_sync(0xffffffffu, e);
+        const int rank_in = __popc(same & ((1u << lane) - 1));
+        const int row = e >= 0 ? mine[e] + rank_in : -1;
+        __syncwarp();
+        if (e >= 0 && rank_in == 0) mine[e] += __popc(same);
+        __syncwarp();
+        if (p < end) {
+            row_of_pair[p] = row;
+            if (row >= 0) pair_of_row[row] = (int)p;
         }
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < PLAN_KEPT; ++i)
+        if (first + 32 * i < end) place(first + 32 * i + lane, kept_e[i]);
+    for (long long b = first + 32 * PLAN_KEPT; b < end; b += 32) place(b + lane, plan_expert(ids, expert_map, map_len, E, b + lane, end));
     for (long long r = (long long)kept + rank * threads + tid; r < P; r += (long long)ctas * threads) pair_of_row[r] = -1;
+}
+
+// i = m * vecs + c
+__device__ __forceinline__ void row_and_vector(long long i, long long vecs, long long& m, long long& c) {
+    if (i <= 0xffffffffLL && vecs <= 0xffffffffLL) {
+        const uint32_t q = (uint32_t)i / (uint32_t)vecs;
+        m = q;
+        c = (uint32_t)i - q * (uint32_t)vecs;
+    } else {
+        m = i / vecs;
+        c = i - m * vecs;
+    }
+}
+
+// Rows from `first` on become zero: a warp per row, all warps of the grid in turn.
+template <typename V>
+__device__ __forceinline__ void zero_rows(uint8_t* rows, long long stride, long long first, long long end, long long vecs) {
+    const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
+    for (long long r = first + (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < end; r += warps) {
+        V* row = reinterpret_cast<V*>(rows + r * stride);
+        for (long long c = threadIdx.x & 31; c < vecs; c += 32) row[c] = V{};
+    }
 }
 
 // ---------------------------------------------------------------------------------
@@ -170,9 +194,11 @@ __global__ void __launch_bounds__(256)
 sort_kernel(const uint8_t* x, long long x_stride, uint8_t* rows, long long rows_stride, long long vecs,
             int M, int T, const int32_t* row_of_pair, const int32_t* kept, int zero_tail) {
     pdl_begin();
+    if (zero_tail) zero_rows<V>(rows, rows_stride, *kept, (long long)M * T, vecs);
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)M * vecs;
     if (i >= all) return;
-    const long long m = i / vecs, c = i - m * vecs;
+    long long m, c;
+    row_and_vector(i, vecs, m, c);
     const V v = reinterpret_cast<const V*>(x + m * x_stride)[c];
     const int32_t* rp = row_of_pair + m * T;
     for (int t0 = 0; t0 < T; t0 += SORT_BATCH) {
@@ -183,9 +209,6 @@ sort_kernel(const uint8_t* x, long long x_stride, uint8_t* rows, long long rows_
         for (int j = 0; j < SORT_BATCH; ++j)
             if (r[j] >= 0) reinterpret_cast<V*>(rows + r[j] * rows_stride)[c] = v;
     }
-    if (zero_tail)
-        for (long long j = (long long)*kept * vecs + i; j < all * T; j += all)
-            reinterpret_cast<V*>(rows + (j / vecs) * rows_stride)[j % vecs] = V{};
 }
 
 // ---------------------------------------------------------------------------------
@@ -202,7 +225,8 @@ unsort_kernel(const uint8_t* rows, long long rows_stride, uint8_t* out, long lon
     pdl_begin();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long long)M * vecs) return;
-    const long long m = i / vecs, c = i - m * vecs;
+    long long m, c;
+    row_and_vector(i, vecs, m, c);
     float acc[R::N];
 #pragma unroll
     for (int k = 0; k < R::N; ++k) acc[k] = 0.f;
@@ -302,12 +326,7 @@ unsort_grad_kernel(const uint8_t* dy, long long dy_stride, const uint8_t* rows, 
             dw[mm * T + t] = d;
         }
     }
-    if (drows) {       // rows nobody owns
-        using V = typename R::Raw;
-        const long long all = (long long)M * T * vecs, step = (long long)gridDim.x * 256;
-        for (long long j = (long long)*kept * vecs + (long long)blockIdx.x * 256 + threadIdx.x; j < all; j += step)
-            reinterpret_cast<V*>(drows + (j / vecs) * drows_stride)[j % vecs] = V{};
-    }
+    if (drows) zero_rows<typename R::Raw>(drows, drows_stride, *kept, (long long)M * T, vecs);      // rows nobody owns
 }
 
 static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_len, int M, int T, int E, int32_t* offsets,

@@ -63,7 +63,7 @@ def _quantize(x, plan: TokenPlan | None = None):
     q = _codes(rows, K, x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
     launch(x.device, "vmoe_int8_quantize", lib.vmoe_int8_quantize, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, K,
-           0 if plan is None else plan.topk, None if plan is None else plan.row_of_pair.data_ptr(), None, q.data_ptr(),
+           0 if plan is None else plan.topk, None if plan is None else plan._rows_ptr, None, q.data_ptr(),
            max(q.stride(0), K), scale.data_ptr())
     return q, scale
 
@@ -84,7 +84,7 @@ def quantize_int8(x: torch.Tensor, plan: TokenPlan | None = None) -> Int8Rows:
         E, N, K = x.shape
         flat = quantize_int8(x.view(E * N, K))
         return Int8Rows(flat.q.as_strided((E, N, K), (N * flat.q.stride(0), flat.q.stride(0), 1)), flat.scale.view(E, N))
-    check_rows(x, "x", None if plan is None else plan.tokens, None if plan is None else plan.expert_offsets.device)
+    check_rows(x, "x", None if plan is None else plan.tokens, None if plan is None else plan.device)
     if x.shape[1] > MAX_K:
         raise ValueError(f"rows of at most {MAX_K} elements")
     return Int8Rows(*_quantize(x, plan))
@@ -151,8 +151,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
     holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``, ``[M, N]``."""
     if a.q.dim() != 2:
         raise ValueError("a must be rows [M, K]")
-    if plan is not None and (a.q.shape[0] != plan.rows or plan.expert_offsets.device != a.q.device):
-        raise ValueError(f"the plan has {plan.rows} rows on {plan.expert_offsets.device}, a {a.q.shape[0]} on {a.q.device}")
+    if plan is not None and (a.q.shape[0] != plan.rows or plan.device != a.q.device):
+        raise ValueError(f"the plan has {plan.rows} rows on {plan.device}, a {a.q.shape[0]} on {a.q.device}")
     N = _out_columns(w, a.q.shape[1], a.q.device, swiglu, None if plan is None else plan.num_experts)
     if out is None:
         if out_dtype not in DTYPE_CODES:
@@ -169,7 +169,7 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
         aq = _pack(aq)
     launch(aq.device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, aq.data_ptr(), aq.stride(0), a.scale.data_ptr(), M, wq.data_ptr(),
            wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, 1 if plan is None else plan.num_experts,
-           None if plan is None else plan.expert_offsets.data_ptr(), swiglu, out is None, y.data_ptr(), max(y.stride(0), N),
+           None if plan is None else plan._offsets_ptr, swiglu, out is None, y.data_ptr(), max(y.stride(0), N),
            DTYPE_CODES[y.dtype])
     return y
 

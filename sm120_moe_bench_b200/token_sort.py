@@ -23,6 +23,7 @@ from ._lib import check, lib
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK = 16
 MAX_EXPERTS = 8192
+ONE_CTA_PAIRS = 4096      # up to here the plan needs no scratch (vmoe_plan_scratch_bytes is 0)
 
 
 # The driver-level handle of a device's current stream and the current device's index, without the wrapper objects that
@@ -75,25 +76,49 @@ class TokenPlan:
     ``expert_offsets`` int32 ``[E + 1]``: rows of expert e are ``expert_offsets[e] .. expert_offsets[e + 1] - 1``;
     ``row_of_pair`` int32 ``[M, T]``, -1 = dropped; ``pair_of_row`` int32 ``[M * T]``, -1 behind the last kept row."""
 
-    __slots__ = ("expert_offsets", "row_of_pair", "pair_of_row", "num_experts")
+    __slots__ = ("tokens", "topk", "rows", "num_experts", "device", "_buf", "_offsets", "_rows", "_pairs", "_offsets_ptr", "_rows_ptr")
 
     def __init__(self, expert_offsets: torch.Tensor, row_of_pair: torch.Tensor, pair_of_row: torch.Tensor, num_experts: int):
-        self.expert_offsets = expert_offsets
-        self.row_of_pair = row_of_pair
-        self.pair_of_row = pair_of_row
+        self.tokens, self.topk = row_of_pair.shape
+        self.rows = self.tokens * self.topk
         self.num_experts = num_experts
+        self.device = row_of_pair.device
+        for t, n, name in ((expert_offsets, num_experts + 1, "expert_offsets"), (row_of_pair, self.rows, "row_of_pair"),
+                           (pair_of_row, self.rows, "pair_of_row")):
+            if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous() or t.device != self.device:
+                raise ValueError(f"{name} must be a contiguous int32 tensor of {n} elements, on the device of the others")
+        self._buf, self._offsets, self._rows, self._pairs = None, expert_offsets, row_of_pair, pair_of_row
+        self._offsets_ptr, self._rows_ptr = expert_offsets.data_ptr(), row_of_pair.data_ptr()
+
+    @classmethod
+    def _over(cls, buf: torch.Tensor, tokens: int, topk: int, num_experts: int) -> "TokenPlan":
+        """The three tables one behind another in ``buf``; views of them are made when they are asked for."""
+        self = cls.__new__(cls)
+        self.tokens, self.topk, self.rows, self.num_experts, self.device = tokens, topk, tokens * topk, num_experts, buf.device
+        self._buf, self._offsets, self._rows, self._pairs = buf, None, None, None
+        self._offsets_ptr = buf.data_ptr()
+        self._rows_ptr = self._offsets_ptr + 4 * (num_experts + 1)
+        return self
 
     @property
-    def tokens(self) -> int:
-        return self.row_of_pair.shape[0]
+    def expert_offsets(self) -> torch.Tensor:
+        if self._offsets is None:
+            self._offsets = self._buf[:self.num_experts + 1]
+        return self._offsets
 
     @property
-    def topk(self) -> int:
-        return self.row_of_pair.shape[1]
+    def row_of_pair(self) -> torch.Tensor:
+        if self._rows is None:
+            at = self.num_experts + 1
+            self._rows = self._buf[at:at + self.rows].view(self.tokens, self.topk)
+        return self._rows
 
     @property
-    def rows(self) -> int:
-        return self.pair_of_row.shape[0]
+    def pair_of_row(self) -> torch.Tensor:
+        if self._pairs is None:
+            at = self.num_experts + 1 + self.rows
+            self._pairs = self._buf[at:at + self.rows]
+        return self._pairs
 
 
 def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tensor | None = None) -> TokenPlan:
@@ -118,31 +143,31 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
             raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids")
         if expert_map.numel() == 0:
             raise ValueError("expert_map is empty")
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    row_of_pair = torch.empty(M, T, dtype=torch.int32, device=dev)
-    pair_of_row = torch.empty(M * T, dtype=torch.int32, device=dev)
-    need = lib.vmoe_plan_scratch_bytes(M, T, num_experts)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    P = M * T
+    need = 0 if P <= ONE_CTA_PAIRS else lib.vmoe_plan_scratch_bytes(M, T, num_experts)
+    buf = torch.empty(num_experts + 1 + 2 * P + need // 4, dtype=torch.int32, device=dev)
+    plan = TokenPlan._over(buf, M, T, num_experts)
+    rows = plan._rows_ptr
     launch(dev, "vmoe_plan_tokens", lib.vmoe_plan_tokens, topk_ids.data_ptr(), None if expert_map is None else expert_map.data_ptr(),
-           0 if expert_map is None else expert_map.numel(), M, T, num_experts, offsets.data_ptr(), row_of_pair.data_ptr(),
-           pair_of_row.data_ptr(), scratch.data_ptr() if need else None, need)
-    return TokenPlan(offsets, row_of_pair, pair_of_row, num_experts)
+           0 if expert_map is None else expert_map.numel(), M, T, num_experts, plan._offsets_ptr, rows, rows + 4 * P,
+           rows + 8 * P if need else None, need)
+    return plan
 
 
 def _sort(x, plan: TokenPlan, out=None):
     K = x.shape[1]
-    rows = torch.empty((plan.rows, K), dtype=x.dtype, device=x.device) if out is None else out
+    rows = x.new_empty((plan.rows, K)) if out is None else out
     launch(x.device, "vmoe_sort_tokens", lib.vmoe_sort_tokens, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], plan.tokens, plan.topk,
-           plan.num_experts, K, plan.expert_offsets.data_ptr(), plan.row_of_pair.data_ptr(), out is None, rows.data_ptr(),
+           plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr, out is None, rows.data_ptr(),
            max(rows.stride(0), K))
     return rows
 
 
 def _unsort(rows, plan: TokenPlan, weights=None, out=None):
     K = rows.shape[1]
-    y = torch.empty((plan.tokens, K), dtype=rows.dtype, device=rows.device) if out is None else out
+    y = rows.new_empty((plan.tokens, K)) if out is None else out
     launch(rows.device, "vmoe_unsort_tokens", lib.vmoe_unsort_tokens, rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype],
-           plan.tokens, plan.topk, K, plan.row_of_pair.data_ptr(), None if weights is None else weights.data_ptr(), y.data_ptr(),
+           plan.tokens, plan.topk, K, plan._rows_ptr, None if weights is None else weights.data_ptr(), y.data_ptr(),
            max(y.stride(0), K), DTYPE_CODES[y.dtype])
     return y
 
@@ -177,11 +202,11 @@ class _UnsortTokens(torch.autograd.Function):
         rows, weights = ctx.saved_tensors
         plan, grad = ctx.plan, _dense_rows(grad)
         M, T, K = plan.tokens, plan.topk, rows.shape[1]
-        drows = torch.empty(plan.rows, K, dtype=rows.dtype, device=rows.device) if ctx.needs_input_grad[0] else None
+        drows = rows.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
         dw = torch.empty(M, T, dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[2] else None
         launch(rows.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0), rows.data_ptr(),
-               rows.stride(0), DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan.expert_offsets.data_ptr(),
-               plan.row_of_pair.data_ptr(), None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(),
+               rows.stride(0), DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
+               None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(),
                K, None if dw is None else dw.data_ptr())
         return drows, None, dw
 
@@ -189,7 +214,7 @@ class _UnsortTokens(torch.autograd.Function):
 def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = None) -> torch.Tensor:
     """``rows[r] = x[token of row r]``: the token rows ``[M, K]`` in expert order, ``[M * T, K]``.  Differentiable in ``x``
     (a token's gradient is the sum over its rows) unless ``out`` is given."""
-    check_rows(x, "x", plan.tokens, plan.expert_offsets.device)
+    check_rows(x, "x", plan.tokens, plan.device)
     if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
@@ -202,7 +227,7 @@ def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = Non
 def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """``out[m] = sum_t weights[m, t] * rows[row of (m, t)]``: rows ``[M * T, K]`` in expert order back to tokens ``[M, K]``.
     ``weights`` f32 ``[M, T]`` (None = 1).  Differentiable in ``rows`` and ``weights`` unless ``out`` is given."""
-    check_rows(rows, "rows", plan.rows, plan.expert_offsets.device)
+    check_rows(rows, "rows", plan.rows, plan.device)
     if weights is not None:
         if weights.device != rows.device or weights.dtype != torch.float32 or tuple(weights.shape) != (plan.tokens, plan.topk):
             raise ValueError(f"weights must be a float32 tensor [{plan.tokens}, {plan.topk}] on the device of rows")
