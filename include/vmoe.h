@@ -363,27 +363,29 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
  * expert_offsets [E + 1] (vmoe_plan_tokens; NULL = dense, E = 1): rows expert_offsets[e] .. use w[e] and w_scale[e]; rows
  * behind expert_offsets[E] are set to zero when zero_tail != 0, else left as they were.
  * swiglu != 0: w has 2 N rows per expert, the N gate rows first, and out = silu(gate) * up.
- * Operands whose addresses and strides are multiples of 16 bytes take the tensor cores. */
+ * Operands whose addresses and strides are multiples of 16 bytes take the tensor cores.  Others are packed into scratch
+ * first (16-byte aligned, vmoe_int8_pack_bytes with weight_rows = N, or 2 N with swiglu) when it is there; without it
+ * (NULL) they are read where they are, which costs less only for a few rows per weight matrix. */
+size_t vmoe_int8_pack_bytes(int32_t M, int32_t weight_rows, int32_t K, int32_t E);
 int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, int32_t M, const int8_t* w, int64_t w_stride,
                      int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
-                     int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream);
+                     int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
+                     size_t scratch_bytes, void* stream);
 
 /* x [M, K] (bf16 / fp16 / f32) quantised row by row, times w [N, K] (swiglu: [2 N, K]): one launch for up to eight rows,
- * else two, the codes in `scratch` (16-byte aligned, vmoe_int8_linear_scratch_bytes). */
+ * else two, the codes in `scratch` (16-byte aligned, vmoe_int8_linear_scratch_bytes); vmoe_int8_pack_bytes(M, weight rows,
+ * K, 1) more let weights of any alignment be packed in a third launch. */
 size_t vmoe_int8_linear_scratch_bytes(int32_t M, int32_t K);
 int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, const int8_t* w, int64_t w_stride, const float* w_scale,
                      int32_t N, int32_t K, int32_t swiglu, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
                      size_t scratch_bytes, void* stream);
 
-/* Rows of codes of any alignment, copied to rows that start on 16-byte boundaries (out and out_stride multiples of 16;
- * columns from K to the next multiple of 16 become zero). */
-int vmoe_int8_pack(const int8_t* q, int64_t q_stride, int64_t rows, int32_t K, int8_t* out, int64_t out_stride, void* stream);
-
 /* The expert layer on 8-bit weights: plan, quantise into expert order, w13 with silu(gate) * up, quantise, w2, weighted
  * sum.  Rows between the products are f32.  w13 [E, 2 N, K] (gate rows first), w2 [E, K, N]; topk_ids, topk_weights [M, T];
  * expert_map as in vmoe_plan_tokens.  Six or seven launches; scratch 16-byte aligned, of
- * vmoe_int8_experts_scratch_bytes (0: sizes beyond the limits of vmoe_plan_tokens). */
-size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N);
+ * vmoe_int8_experts_scratch_bytes (0: sizes beyond the limits of vmoe_plan_tokens), with room to pack weights of any
+ * alignment when pack != 0. */
+size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N, int32_t pack);
 int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K, int32_t N,
                       const int32_t* topk_ids, const float* topk_weights, const int32_t* expert_map, int32_t map_len,
                       const int8_t* w13, int64_t w13_stride, int64_t w13_expert_stride, const float* w13_scale,

@@ -96,12 +96,12 @@ SIGNATURES = {
                                           _P, _P, _P, _P, C.c_int64, _P, _P]),
     "vmoe_int8_quantize": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P, _P]),
     "vmoe_int8_matmul": (C.c_int, [_P, C.c_int64, _P, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P,
-                                   C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P]),
+                                   C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P, C.c_size_t, _P]),
+    "vmoe_int8_pack_bytes": (C.c_size_t, [C.c_int32] * 4),
     "vmoe_int8_linear_scratch_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
     "vmoe_int8_linear": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64,
                                    C.c_int32, _P, C.c_size_t, _P]),
-    "vmoe_int8_pack": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int32, _P, C.c_int64, _P]),
-    "vmoe_int8_experts_scratch_bytes": (C.c_size_t, [C.c_int32] * 5),
+    "vmoe_int8_experts_scratch_bytes": (C.c_size_t, [C.c_int32] * 6),
     "vmoe_int8_experts": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, C.c_int32,
                                     _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, C.c_int32, _P, C.c_size_t,
                                     _P]),

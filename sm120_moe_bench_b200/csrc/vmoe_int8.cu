@@ -181,24 +181,35 @@ static int launch_i8_tile(const I8Problem& p, cudaStream_t st) {
                                 : cudaLaunchKernelEx(&cfg, i8_tile_kernel<false>, p, (int)aa, (int)aw));
 }
 
-// Rows of any alignment to rows that start on 16-byte boundaries (columns behind K become zero).
+// Both operands of a product, rows of any alignment, to rows that start on 16-byte boundaries: one thread per 16 codes,
+// first those of a [M], then those of w [E][wrows].  Columns behind K become zero.
 __global__ void __launch_bounds__(256)
-i8_pack_kernel(const int8_t* q, long long q_stride, long long rows, int K, int8_t* out, long long out_stride) {
+i8_pack_kernel(const I8Problem p, int pack_a, int8_t* a, int8_t* w) {
     pdl_begin();
-    const int vecs = (K + 15) / 16;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= rows * vecs) return;
-    const long long r = i / vecs;
-    const int k = (int)(i - r * vecs) * 16;
-    const int8_t* src = q + r * q_stride + k;
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = i8_word(src, 4 * j, K - k, ((uintptr_t)src & 3) == 0);
-    // the row's last vector may have no room for its zeros
-    int8_t* dst = out + r * out_stride + k;
-    if (k + 16 <= out_stride) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    else
-        for (int j = 0; k + j < K; ++j) dst[j] = (int8_t)(w[j >> 2] >> (8 * (j & 3)));
+    const int K = p.K, vecs = (K + 15) / 16;
+    const long long in_a = pack_a ? (long long)p.M * vecs : 0;
+    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int8_t* src;
+    int8_t* dst;
+    int k;
+    if (i < in_a) {
+        const long long r = i / vecs;
+        k = (int)(i - r * vecs) * 16;
+        src = p.a + r * p.a_stride + k;
+        dst = a + r * vecs * 16 + k;
+    } else {
+        i -= in_a;
+        const long long r = i / vecs, e = r / p.wrows;
+        if (!w || e >= p.E) return;
+        k = (int)(i - r * vecs) * 16;
+        src = p.w + e * p.w_expert_stride + (r - e * p.wrows) * p.w_stride + k;
+        dst = w + r * vecs * 16 + k;
+    }
+    const bool aligned = ((uintptr_t)src & 3) == 0;
+    uint4 v;
+    v.x = i8_word(src, 0, K - k, aligned); v.y = i8_word(src, 4, K - k, aligned);
+    v.z = i8_word(src, 8, K - k, aligned); v.w = i8_word(src, 12, K - k, aligned);
+    *reinterpret_cast<uint4*>(dst) = v;
 }
 
 static int i8_pitch(int K) { return (K + 15) / 16 * 16; }
@@ -232,9 +243,35 @@ static int i8_product(const I8Problem& p, cudaStream_t st) {
     return launch_i8_tc(p, st);
 }
 
-struct I8ExpertsScratch { size_t offsets, row_of_pair, pair_of_row, counts, counts_bytes, scale, q1, h, q2, y, total; };
+static size_t i8_pack_bytes(long long M, long long wrows, int K, int E) {
+    return i8_align((size_t)M * i8_pitch(K)) + (size_t)E * wrows * i8_pitch(K);
+}
+
+// The product of operands of any alignment: with room for it, unaligned ones are packed first.  The kernel that reads them
+// where they are does about 80 TOPS; packing moves twice the operands' bytes and the tensor cores do the rest, which
+// pays from about 13 rows per weight matrix.
+static int i8_product_any(I8Problem p, void* room, size_t bytes, cudaStream_t st) {
+    if (room && p.M > 0 && p.K > 0 && p.E <= I8_TC_MAX_EXPERTS && !i8_gemv_ok(p) && !i8_tc_ok(p) &&
+        bytes >= i8_pack_bytes(p.M, p.wrows, p.K, p.E) && !((uintptr_t)room & 15)) {
+        I8Problem q = p;
+        int8_t* a = static_cast<int8_t*>(room);
+        int8_t* w = a + i8_align((size_t)p.M * i8_pitch(p.K));
+        const bool pack_a = (((uintptr_t)p.a | (unsigned long long)p.a_stride) & 15) != 0 || p.a_stride < p.K;
+        if (pack_a) { q.a = a; q.a_stride = i8_pitch(p.K); }
+        const bool pack_w = !i8_tc_ok(q);
+        if (pack_w) { q.w = w; q.w_stride = i8_pitch(p.K); q.w_expert_stride = (long long)p.wrows * i8_pitch(p.K); }
+        const long long vecs = (long long)(i8_pitch(p.K) / 16) * ((pack_a ? p.M : 0) + (pack_w ? (long long)p.E * p.wrows : 0));
+        if ((vecs + 255) / 256 > 0x7fffffffLL) return VMOE_ERR_LIMIT;
+        if (launch_pdl(i8_pack_kernel, (unsigned)((vecs + 255) / 256), 256u, 0, st, p, (int)pack_a, a, pack_w ? w : (int8_t*)nullptr) != cudaSuccess)
+            return VMOE_ERR_CUDA;
+        p = q;
+    }
+    return i8_product(p, st);
+}
+
+struct I8ExpertsScratch { size_t offsets, row_of_pair, pair_of_row, counts, counts_bytes, scale, q1, h, q2, y, room13, room2, room13_bytes, room2_bytes, total; };
 // false: sizes the plan does not take.  The f32 rows of the second product (y) take the place of the first one's operands.
-static bool i8_experts_scratch(int M, int T, int E, int K, int N, I8ExpertsScratch* s) {
+static bool i8_experts_scratch(int M, int T, int E, int K, int N, int pack, I8ExpertsScratch* s) {
     if (M < 0 || T <= 0 || T > MAX_TOPK || E <= 0 || E > 8192 || K <= 0 || N <= 0 || (long long)M * T > 0x7fffffffLL - 1024) return false;
     const size_t P = (size_t)M * T;
     size_t at = 0;
@@ -249,7 +286,11 @@ static bool i8_experts_scratch(int M, int T, int E, int K, int N, I8ExpertsScrat
     s->y = s->q1 = take(P * i8_pitch(K));
     s->h = take(P * N * 4);
     const size_t y_end = s->y + i8_align(P * K * 4);
-    s->total = at > y_end ? at : y_end;
+    if (at < y_end) at = y_end;
+    s->room13_bytes = pack ? i8_pack_bytes(P, 2LL * N, K, E) : 0;      // the rows are packed already; only the weights may be copied
+    s->room2_bytes = pack ? i8_pack_bytes(P, K, N, E) : 0;
+    s->room13 = s->room2 = take(s->room13_bytes > s->room2_bytes ? s->room13_bytes : s->room2_bytes);
+    s->total = at;
     return true;
 }
 
@@ -279,25 +320,31 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         // four vectors a thread, and no fewer than two rows a CTA while they fit
         if (vecs <= 128) return launch_quantize_rows<typename R::T, R::BYTES, 1>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        if (vecs <= 256) return launch_quantize_rows<typename R::T, R::BYTES, 2>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
         if (vecs <= 512) return launch_quantize_rows<typename R::T, R::BYTES, 4>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
         return launch_quantize_rows<typename R::T, R::BYTES, 8>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
     });
 }
 
+size_t vmoe_int8_pack_bytes(int32_t M, int32_t weight_rows, int32_t K, int32_t E) {
+    return M <= 0 || weight_rows <= 0 || K <= 0 || E <= 0 || K > I8_MAX_K ? 0 : i8_pack_bytes(M, weight_rows, K, E);
+}
+
 int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, int32_t M, const int8_t* w, int64_t w_stride,
                      int64_t w_expert_stride, const float* w_scale, int32_t N, int32_t K, int32_t E, const int32_t* expert_offsets,
-                     int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* stream) {
+                     int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
+                     size_t scratch_bytes, void* stream) {
     I8Problem p;
     const int rc = i8_problem(&p, a, a_stride, a_scale, M, w, w_stride, w_expert_stride, w_scale, N, K, E, expert_offsets, swiglu,
                               zero_tail, out, out_stride, out_dtype);
     if (rc || M == 0) return rc;
     if (!a_scale || (K > 0 && !a)) return VMOE_ERR_NULL;
-    return i8_product(p, static_cast<cudaStream_t>(stream));
+    return i8_product_any(p, scratch, scratch_bytes, static_cast<cudaStream_t>(stream));
 }
 
 size_t vmoe_int8_linear_scratch_bytes(int32_t M, int32_t K) {
     if (M <= 0 || K < 0 || K > I8_MAX_K) return 0;
-    return i8_align((size_t)M * i8_pitch(K)) + (size_t)M * sizeof(float);
+    return i8_align((size_t)M * i8_pitch(K)) + i8_align((size_t)M * sizeof(float));
 }
 
 int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, const int8_t* w, int64_t w_stride, const float* w_scale,
@@ -314,29 +361,19 @@ int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
     if ((uintptr_t)x & (el - 1)) return VMOE_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (i8_gemv_ok(p)) return launch_i8_gemv(p, x, x_stride * el, dtype, st);
-    if (!scratch || scratch_bytes < vmoe_int8_linear_scratch_bytes(M, K)) return VMOE_ERR_WORKSPACE;
+    const size_t need = vmoe_int8_linear_scratch_bytes(M, K);
+    if (!scratch || scratch_bytes < need) return VMOE_ERR_WORKSPACE;
     if ((uintptr_t)scratch & 15) return VMOE_ERR_ALIGN;
     int8_t* q = reinterpret_cast<int8_t*>(base);
     float* scale = reinterpret_cast<float*>(base + i8_align((size_t)M * pitch));
     if ((rc = vmoe_int8_quantize(x, x_stride, dtype, M, K, 0, nullptr, nullptr, q, pitch, scale, stream))) return rc;
     p.a = q; p.a_scale = scale;
-    return i8_product(p, st);
+    return i8_product_any(p, base + need, scratch_bytes - need, st);
 }
 
-int vmoe_int8_pack(const int8_t* q, int64_t q_stride, int64_t rows, int32_t K, int8_t* out, int64_t out_stride, void* stream) {
-    if (rows < 0 || K < 0 || q_stride < 0 || out_stride < K) return VMOE_ERR_SHAPE;
-    if (rows == 0 || K == 0) return VMOE_OK;
-    if (!q || !out) return VMOE_ERR_NULL;
-    if (((uintptr_t)out | (unsigned long long)out_stride) & 15) return VMOE_ERR_ALIGN;
-    const long long blocks = (rows * ((K + 15) / 16) + 255) / 256;
-    if (blocks > 0x7fffffffLL) return VMOE_ERR_LIMIT;
-    return cuda_status(launch_pdl(i8_pack_kernel, (unsigned)blocks, 256u, 0, static_cast<cudaStream_t>(stream), q, (long long)q_stride,
-                                  (long long)rows, K, out, (long long)out_stride));
-}
-
-size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N) {
+size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N, int32_t pack) {
     I8ExpertsScratch s;
-    return i8_experts_scratch(M, T, E, K, N, &s) ? s.total : 0;
+    return i8_experts_scratch(M, T, E, K, N, pack, &s) ? s.total : 0;
 }
 
 int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M, int32_t T, int32_t E, int32_t K, int32_t N,
@@ -348,7 +385,9 @@ int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M,
     if (M < 0 || T <= 0 || E <= 0) return VMOE_ERR_SHAPE;
     if (K > I8_MAX_K || N > I8_MAX_K) return VMOE_ERR_LIMIT;
     I8ExpertsScratch L;
-    if (!i8_experts_scratch(M, T, E, K, N, &L)) return VMOE_ERR_LIMIT;
+    if (!i8_experts_scratch(M, T, E, K, N, 1, &L)) return VMOE_ERR_LIMIT;
+    const bool pack = scratch_bytes >= L.total;
+    if (!pack) i8_experts_scratch(M, T, E, K, N, 0, &L);
     if (M == 0) return VMOE_OK;
     if (!x || !topk_ids || !topk_weights || !w13 || !w2 || !w13_scale || !w2_scale || !out) return VMOE_ERR_NULL;
     if (!scratch || scratch_bytes < L.total) return VMOE_ERR_WORKSPACE;
@@ -361,16 +400,17 @@ int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M,
     float* h = reinterpret_cast<float*>(b + L.h);
     int8_t* q2 = reinterpret_cast<int8_t*>(b + L.q2);
     float* y = reinterpret_cast<float*>(b + L.y);
+    void* room = pack ? b + L.room13 : nullptr;
     const int P = M * T;
     int rc;
     if ((rc = vmoe_plan_tokens(topk_ids, expert_map, map_len, M, T, E, offsets, row_of_pair, reinterpret_cast<int32_t*>(b + L.pair_of_row),
                                b + L.counts, L.counts_bytes, stream))) return rc;
     if ((rc = vmoe_int8_quantize(x, x_stride, dtype, M, K, T, row_of_pair, nullptr, q1, i8_pitch(K), scale, stream))) return rc;
     if ((rc = vmoe_int8_matmul(q1, i8_pitch(K), scale, P, w13, w13_stride, w13_expert_stride, w13_scale, N, K, E, offsets, 1, 0, h, N, VMOE_F32,
-                               stream))) return rc;
+                               room, L.room13_bytes, stream))) return rc;
     if ((rc = vmoe_int8_quantize(h, N, VMOE_F32, P, N, 0, nullptr, offsets + E, q2, i8_pitch(N), scale, stream))) return rc;
     if ((rc = vmoe_int8_matmul(q2, i8_pitch(N), scale, P, w2, w2_stride, w2_expert_stride, w2_scale, K, N, E, offsets, 0, 0, y, K, VMOE_F32,
-                               stream))) return rc;
+                               room, L.room2_bytes, stream))) return rc;
     return vmoe_unsort_tokens(y, K, VMOE_F32, M, T, K, row_of_pair, topk_weights, out, out_stride, out_dtype, stream);
 }
 

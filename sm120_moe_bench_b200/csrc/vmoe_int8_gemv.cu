@@ -11,6 +11,8 @@ namespace vmoe {
 constexpr int I8G_THREADS = 256;
 constexpr int I8G_SMEM = 64 * 1024;                       // codes of all rows
 
+// VB = 16: the weights' rows start on 16-byte boundaries.  VB = 4: anywhere; a word is joined from the two aligned ones that
+// hold it, the second of which is read only where the row reaches into it.
 template <int VB> struct I8Word;
 template <> struct I8Word<16> { using type = uint4; };
 template <> struct I8Word<4>  { using type = uint32_t; };
@@ -22,6 +24,14 @@ __device__ __forceinline__ int i8_dot(uint4 a, uint4 b, int s) {
     return __dp4a((int)a.w, (int)b.w, s);
 }
 __device__ __forceinline__ int i8_dot(uint32_t a, uint32_t b, int s) { return __dp4a((int)a, (int)b, s); }
+
+__device__ __forceinline__ uint4 i8_weights(const uint4* row, int c, int, int) { return row[c]; }
+__device__ __forceinline__ uint32_t i8_weights(const uint32_t* row, int c, int shift, int K) {      // shift: the row starts so many bytes into row[0]
+    const uint32_t lo = row[c];
+    if (shift == 0) return lo;
+    const uint32_t hi = 4 * (c + 1) - shift < K ? row[c + 1] : 0u;
+    return __funnelshift_r(lo, hi, 8 * shift);
+}
 
 // One row into shared memory: its codes (padded with zeros to `pitch`) and scale, by the whole CTA.
 template <typename T_>
@@ -106,15 +116,20 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
     const int K = p.K, pitch = (K + 15) & ~15, words = (K + VB - 1) / VB;
     const bool on = n < p.N;
     const W* w[SETS];
+    int shift[SETS];
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) w[s] = reinterpret_cast<const W*>(p.w + (long long)(s * p.N + (on ? n : 0)) * p.w_stride);
+    for (int s = 0; s < SETS; ++s) {
+        const uintptr_t at = (uintptr_t)(p.w + (long long)(s * p.N + (on ? n : 0)) * p.w_stride);
+        shift[s] = VB == 4 ? (int)(at & 3) : 0;
+        w[s] = reinterpret_cast<const W*>(at - shift[s]);
+    }
     W have[SETS][AHEAD];
 #pragma unroll
     for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             have[s][i] = W{};
-            if (lane + 32 * i < words) have[s][i] = w[s][lane + 32 * i];
+            if (lane + 32 * i < words) have[s][i] = i8_weights(w[s], lane + 32 * i, shift[s], K);
         }
     for (int m = 0; m < p.M; ++m) {
         uint8_t* dst = codes + (size_t)m * pitch;
@@ -154,7 +169,7 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int c = c0 + 32 * AHEAD + lane + 32 * i;
-                if (c < words) have[s][i] = w[s][c];
+                if (c < words) have[s][i] = i8_weights(w[s], c, shift[s], K);
             }
     }
     float mine = 0.f;
@@ -169,9 +184,7 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
 }
 
 bool i8_gemv_ok(const I8Problem& p) {
-    const unsigned long long all = (unsigned long long)(uintptr_t)p.w | (unsigned long long)p.w_stride;
-    return p.E == 1 && !p.offsets && p.M <= I8_GEMV_ROWS && p.K > 0 && all % 4 == 0 && p.w_stride >= p.K &&
-           (long long)p.M * ((p.K + 15) & ~15) <= I8G_SMEM;
+    return p.E == 1 && !p.offsets && p.M <= I8_GEMV_ROWS && p.K > 0 && p.w_stride >= p.K && (long long)p.M * ((p.K + 15) & ~15) <= I8G_SMEM;
 }
 
 template <int VB, int ROWS, bool SWIGLU>

@@ -95,27 +95,10 @@ def _aligned(q: torch.Tensor) -> bool:
     return (q.data_ptr() | q.stride(-2) | (q.stride(0) if q.dim() == 3 else 0)) % 16 == 0
 
 
-def _pack(q: torch.Tensor) -> torch.Tensor:
-    """The same codes in rows that start on 16-byte boundaries."""
-    K = q.shape[-1]
-    pitch = (K + 15) // 16 * 16
-    out = torch.empty((*q.shape[:-1], pitch), dtype=torch.int8, device=q.device)
-    if q.dim() == 3 and q.stride(0) != q.shape[1] * q.stride(1):
-        parts = zip(q, out)                               # matrices with gaps between them
-    else:
-        parts = ((q, out),)
-    for src, dst in parts:
-        launch(q.device, "vmoe_int8_pack", lib.vmoe_int8_pack, src.data_ptr(), src.stride(-2), src.numel() // K, K, dst.data_ptr(), pitch)
-    return out[..., :K]
-
-
-def _operand(w: Int8Rows, rows: int) -> torch.Tensor:
-    """The codes of the weights for a product with ``rows`` rows: packed first where that pays.  The kernel for unaligned rows does
-    about 80 TOPS on them; packing moves twice the weights' bytes and the tensor cores do the rest, which pays from about 13
-    rows per matrix."""
-    q = w.q
-    experts = q.shape[0] if q.dim() == 3 else 1
-    return q if q.shape[-1] == 0 or rows < 16 * experts or _aligned(q) else _pack(q)
+def _packs(w: Int8Rows, rows: int) -> bool:
+    """Whether unaligned weights are worth a copy for a product with this many rows (the reason stands at the C side's
+    ``i8_product_any``).  Up to eight rows of a single matrix have a kernel of their own that reads them anywhere."""
+    return rows > 8 if w.q.dim() == 2 else rows >= 16 * w.q.shape[0]
 
 
 def int8_status(device: torch.device | str | int = "cuda") -> int:
@@ -164,13 +147,13 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
             raise ValueError(f"out must have {N} columns on {a.q.device}")
         _no_grad(out, "out")
     M, K = a.q.shape
-    aq, wq = a.q, _operand(w, M)
-    if M >= 16 and K and not _aligned(aq) and (wq is not w.q or _aligned(wq)):
-        aq = _pack(aq)
+    aq, wq = a.q, w.q
+    E = 1 if plan is None else plan.num_experts
+    need = 0 if (_aligned(aq) and _aligned(wq)) or not _packs(w, M) else lib.vmoe_int8_pack_bytes(M, wq.shape[-2], K, E)
+    scratch = torch.empty(need, dtype=torch.uint8, device=aq.device) if need else None
     launch(aq.device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, aq.data_ptr(), aq.stride(0), a.scale.data_ptr(), M, wq.data_ptr(),
-           wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, 1 if plan is None else plan.num_experts,
-           None if plan is None else plan._offsets_ptr, swiglu, out is None, y.data_ptr(), max(y.stride(0), N),
-           DTYPE_CODES[y.dtype])
+           wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, E, None if plan is None else plan._offsets_ptr,
+           swiglu, out is None, y.data_ptr(), max(y.stride(0), N), DTYPE_CODES[y.dtype], scratch.data_ptr() if need else None, need)
     return y
 
 
@@ -187,10 +170,12 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
             raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
         _no_grad(out, "out")
     M, K = x.shape
-    wq = _operand(w, M)
-    # a few rows are quantised inside the product
-    inside = M <= 8 and K <= 8192 and (wq.data_ptr() | wq.stride(0)) % 4 == 0
-    need = 0 if inside else lib.vmoe_int8_linear_scratch_bytes(M, K)
+    wq = w.q
+    need = 0
+    if M > 8 or not 0 < K <= 8192 or wq.stride(0) < K:    # else the rows are quantised inside the product
+        need = lib.vmoe_int8_linear_scratch_bytes(M, K)
+        if not _aligned(wq) and _packs(w, M):
+            need += lib.vmoe_int8_pack_bytes(M, wq.shape[0], K, 1)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     launch(x.device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, wq.data_ptr(),
            wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), max(out.stride(0), N), DTYPE_CODES[out.dtype],
@@ -227,9 +212,10 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
     if expert_map is not None and (expert_map.device != x.device or expert_map.dtype != torch.int32 or expert_map.dim() != 1
                                    or not expert_map.is_contiguous() or expert_map.numel() == 0):
         raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids, not empty")
-    q13, q2 = _operand(w13, M * T), _operand(w2, M * T)
+    q13, q2 = w13.q, w2.q
+    pack = not (_aligned(q13) and _aligned(q2)) and _packs(w13, M * T)
     out = torch.empty((M, K), dtype=x.dtype, device=x.device)
-    need = lib.vmoe_int8_experts_scratch_bytes(M, T, E, K, N)
+    need = lib.vmoe_int8_experts_scratch_bytes(M, T, E, K, N, pack)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
     launch(x.device, "vmoe_int8_experts", lib.vmoe_int8_experts, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, T, E, K, N,
            topk_ids.data_ptr(), topk_weights.data_ptr(), None if expert_map is None else expert_map.data_ptr(),

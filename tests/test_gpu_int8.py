@@ -152,6 +152,48 @@ def test_product_of_unaligned_rows(M, N, K, pa, pw):
     check_product(vm.int8_matmul(odd, w), exact_product(odd, w))
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 8])
+@pytest.mark.parametrize("K", [1, 5, 127, 1001, 4098, 9001])
+def test_few_rows_of_any_alignment(M, K):
+    import sm120_moe_bench_b200 as vm
+    for skew in range(5):
+        q = torch.randint(-128, 128, (61 * (K + skew) + skew,), generator=gen(64 + skew), device="cuda", dtype=torch.int8)
+        w = vm.Int8Rows(q[skew:].view(61, K + skew)[:, :K], torch.rand(61, generator=gen(65), device="cuda"))
+        a = random_rows(vm, (M, K), 66)
+        check_product(vm.int8_matmul(a, w, out_dtype=torch.float32), exact_product(a, w))
+        half = vm.Int8Rows(w.q[:60], w.scale[:60])
+        check_swiglu(vm.int8_matmul(a, half, swiglu=True, out_dtype=torch.float32), exact_product(a, half), 30)
+        x = torch.randn(M, K, generator=gen(67), device="cuda").half()
+        assert torch.equal(vm.int8_linear(x, w), vm.int8_matmul(vm.quantize_int8(x), w, out_dtype=torch.float16))
+
+
+def test_broadcast_rows():
+    import sm120_moe_bench_b200 as vm
+    for M in (3, 40):
+        a, w = random_rows(vm, (1, 64), 68), random_rows(vm, (1, 64), 70)
+        many = vm.Int8Rows(a.q.expand(M, 64), a.scale.expand(M).contiguous())
+        wide = vm.Int8Rows(w.q.expand(50, 64), w.scale.expand(50).contiguous())
+        for l, r in ((many, wide), (many, random_rows(vm, (50, 64), 72)), (random_rows(vm, (M, 64), 74), wide)):
+            check_product(vm.int8_matmul(l, r, out_dtype=torch.float32), exact_product(l, r))
+        x = torch.randn(M, 64, generator=gen(76), device="cuda")
+        check_product(vm.int8_linear(x, wide), exact_product(vm.quantize_int8(x), wide))
+        nothing = vm.Int8Rows(torch.zeros(7, 0, dtype=torch.int8, device="cuda"), torch.ones(7, device="cuda"))
+        assert torch.equal(vm.int8_linear(torch.zeros(M, 0, device="cuda"), nothing), torch.zeros(M, 7, device="cuda"))
+
+
+def test_expert_layer_with_unaligned_weights():
+    import sm120_moe_bench_b200 as vm
+    E, K, N, T = 3, 200, 72, 2
+    w13, w2 = random_rows(vm, (E, 2 * N, K), 77, K + 3), random_rows(vm, (E, K, N), 79, N + 1)
+    a13 = vm.Int8Rows(torch.nn.functional.pad(w13.q, (0, 8))[..., :K], w13.scale)
+    a2 = vm.Int8Rows(torch.nn.functional.pad(w2.q, (0, 8))[..., :N], w2.scale)
+    for M in (2, 12, 30, 200):
+        x = torch.randn(M, K, generator=gen(81), device="cuda").bfloat16()
+        ids = torch.randint(0, E, (M, T), generator=gen(82), device="cuda", dtype=torch.int32)
+        wt = torch.rand(M, T, generator=gen(83), device="cuda")
+        assert torch.equal(vm.int8_experts(x, w13, w2, ids, wt), vm.int8_experts(x, a13, a2, ids, wt))
+
+
 def test_product_at_the_ends_of_the_integers():
     import sm120_moe_bench_b200 as vm
     for M in (1, 20, 140):

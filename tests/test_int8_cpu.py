@@ -36,7 +36,7 @@ def test_matmul_checks():
     b = ctypes.addressof(keep) & ~15
 
     def matmul(a=b, sa=b, M=4, w=b, sw=b, N=8, K=16, E=1, off=None, out=b, os_=8, dtype=0, ast=16, wst=16, est=0):
-        return lib.vmoe_int8_matmul(a, ast, sa, M, w, wst, est, sw, N, K, E, off, 0, 0, out, os_, dtype, None)
+        return lib.vmoe_int8_matmul(a, ast, sa, M, w, wst, est, sw, N, K, E, off, 0, 0, out, os_, dtype, None, 0, None)
 
     assert matmul(M=0) == 0
     assert matmul(M=-1) == 2 and matmul(N=0) == 2 and matmul(K=-1) == 2 and matmul(E=0) == 2 and matmul(dtype=3) == 2
@@ -58,7 +58,7 @@ def test_host_tensors_are_refused():
         vm.quantize_int8(torch.zeros(4, 16, requires_grad=True))
 
 
-def test_linear_pack_and_experts_checks():
+def test_linear_and_experts_checks():
     lib, keep = _lib(), _buf()
     b = ctypes.addressof(keep) & ~15
     assert lib.vmoe_int8_linear_scratch_bytes(0, 64) == 0 and lib.vmoe_int8_linear_scratch_bytes(3, 131072) == 0
@@ -73,13 +73,12 @@ def test_linear_pack_and_experts_checks():
     assert linear(x=b + 1) == 3 and linear(scratch=b + 8) == 3
     assert linear(scratch=None) == 4 and linear(bytes_=16) == 4
 
-    pack = lambda q=b, qs=20, rows=3, K=20, out=b, os_=32: lib.vmoe_int8_pack(q, qs, rows, K, out, os_, None)
-    assert pack(rows=0) == 0 and pack(K=0) == 0
-    assert pack(rows=-1) == 2 and pack(os_=16) == 2 and pack(q=None) == 1 and pack(out=None) == 1 and pack(os_=24) == 3 and pack(out=b + 4) == 3
+    assert lib.vmoe_int8_pack_bytes(0, 8, 20, 1) == 0 and lib.vmoe_int8_pack_bytes(3, 8, 20, 2) >= 3 * 32 + 2 * 8 * 32
 
     size = lib.vmoe_int8_experts_scratch_bytes
-    assert size(4, 17, 8, 64, 32) == 0 and size(4, 2, 8193, 64, 32) == 0 and size(2 ** 28, 16, 8, 64, 32) == 0
-    assert size(64, 10, 512, 4096, 1024) >= 640 * 4096 * 4
+    assert size(4, 17, 8, 64, 32, 0) == 0 and size(4, 2, 8193, 64, 32, 0) == 0 and size(2 ** 28, 16, 8, 64, 32, 0) == 0
+    assert size(64, 10, 512, 4096, 1024, 0) >= 640 * 4096 * 4
+    assert size(64, 10, 512, 4096, 1024, 1) >= size(64, 10, 512, 4096, 1024, 0) + 512 * 2048 * 4096
 
     def experts(x=b, dtype=0, M=4, T=2, E=4, K=32, N=16, ids=b, wt=b, w13=b, s13=b, w2=b, s2=b, out=b, scratch=b, bytes_=1 << 40):
         return lib.vmoe_int8_experts(x, K, dtype, M, T, E, K, N, ids, wt, None, 0, w13, K, 2 * N * K, s13, w2, N, N * K, s2, out, K, 0,
