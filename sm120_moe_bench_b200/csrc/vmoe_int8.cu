@@ -4,14 +4,14 @@
 namespace vmoe {
 
 // ---------------------------------------------------------------------------------
-// Rows to codes (the arithmetic: I8RowScale).  WPR warps per row, eight per CTA; a thread keeps up to four vectors of the
-// row in registers, so that rows of up to 4 * 32 * WPR vectors are read once.  With row_of_pair a row is a token and its
+// Rows to codes (the arithmetic: I8RowScale).  WPR warps per row, eight per CTA; a thread keeps up to eight vectors of the
+// row in registers, so that rows of up to 8 * 32 * WPR vectors are read once.  With row_of_pair a row is a token and its
 // codes go to the token's T sorted rows.
 // ---------------------------------------------------------------------------------
-constexpr int I8_KEPT = 4;
+constexpr int I8_KEPT = 8;
 
 template <typename T_, int VB, int WPR, bool SORTED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 4)
 i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vecs, int T, const int32_t* row_of_pair,
                    const int32_t* live, int8_t* q, long long q_stride, float* scales) {
     using R = RowVec<T_, VB>;
@@ -318,10 +318,12 @@ int vmoe_int8_quantize(const void* x, int64_t x_stride, int32_t dtype, int32_t r
         using R = decltype(r);
         const int vecs = K / R::N;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        // four vectors a thread, and no fewer than two rows a CTA while they fit
-        if (vecs <= 128) return launch_quantize_rows<typename R::T, R::BYTES, 1>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
-        if (vecs <= 256) return launch_quantize_rows<typename R::T, R::BYTES, 2>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
-        if (vecs <= 512) return launch_quantize_rows<typename R::T, R::BYTES, 4>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        // Many rows: eight vectors a thread, so that the row's own work (its largest magnitude, its scale) is spread over
+        // them.  Few rows: as many warps a row as find a vector for each lane.
+        const bool many = rows >= 2048;
+        if (vecs <= (many ? 256 : 32)) return launch_quantize_rows<typename R::T, R::BYTES, 1>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        if (vecs <= (many ? 512 : 64)) return launch_quantize_rows<typename R::T, R::BYTES, 2>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
+        if (vecs <= (many ? 1024 : 128)) return launch_quantize_rows<typename R::T, R::BYTES, 4>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
         return launch_quantize_rows<typename R::T, R::BYTES, 8>(x, xs, rows, vecs, T, row_of_pair, live_rows, q, q_stride, scales, st);
     });
 }

@@ -31,11 +31,15 @@ __device__ __forceinline__ void i8_store(void* out, long long at, int dtype, flo
 
 // ---------------------------------------------------------------------------------
 // Row quantiser: scale = max|x| / 127, code = rint(127 x / max|x|), ties to even -- the code of the exact quotient, not of
-// a rounded one.  inv = 127 * RN(1 / max|x|) and y = x * inv carry three roundings, so y is off by less than 127 * 3 * 2^-24 <
-// 2.3e-5: only vectors with a y within 2.5e-5 of a border between two codes are decided in 64 bits.  A row of zeros has
-// scale 0 and codes 0; a row with an infinity or a NaN has scale NaN and codes 0, so that its outputs are NaN and no other
-// row's are.  Rounding adds 1.5 * 2^23: the sum's low byte is the code, and taking the constant off again gives the
-// rounded value.
+// a rounded one.  A row of zeros has scale 0 and codes 0; a row with an infinity or a NaN has scale NaN and codes 0, so that
+// its outputs are NaN and no other row's are.  Rounding adds 1.5 * 2^23: the sum's low byte is the code.
+//   16-bit elements: n = 127 x is exact in f32 (7 + 11 bits), q = n * RN(1 / max|x|) with one correction q + (n - q max|x|) r is
+//   the correctly rounded quotient, exact at a tie; a quotient that is no tie is at least y / (254 * 2047) away from one
+//   (its numerator is a whole number of units), f32's half step y * 2^-24 is less, so rounding q rounds the quotient.
+//   f32 elements: inv = 127 * RN(1 / max|x|) and y = x * inv carry three roundings, so y is off by less than
+//   127 * 3 * 2^-24 < 2.3e-5; vectors with a y within 2.5e-5 of a border between two codes are decided in 64 bits.
+// Rows whose largest magnitude is below 2^-100 or above 2^100 are decided in 64 bits throughout: 1 / max|x| and the
+// residual stay normal numbers otherwise.
 // ---------------------------------------------------------------------------------
 constexpr float I8_ROUND = 12582912.f;
 constexpr float I8_BORDER = 0.5f - 2.5e-5f;
@@ -44,45 +48,46 @@ constexpr float I8_BORDER = 0.5f - 2.5e-5f;
 static __device__ __noinline__ float i8_exact_code(float x, float amax) { return (float)rint(127.0 * (double)x / (double)amax); }
 
 struct I8RowScale {
-    float scale, amax, up, inv;          // inv = 0: every code is 0
+    float scale, amax, r, inv;           // r = RN(1 / amax), inv = 127 r; plain: these are good for the whole row
+    bool plain;
     // top: the largest magnitude of the row as an integer, which orders NaN > infinity > finite
     __device__ __forceinline__ explicit I8RowScale(uint32_t top) {
-        const bool finite = top < 0x7f800000u;
         amax = __uint_as_float(top);
+        plain = amax >= 0x1p-100f && amax <= 0x1p100f;
         // by rcp.rn and a correction, exact for this divisor (Divider) while nothing underflows
-        scale = !finite ? __uint_as_float(0x7fc00000u) : amax >= 0x1p-100f ? Divider(127.f)(amax) : amax / 127.f;
-        up = amax < 0x1p-100f ? 0x1p100f : amax > 0x1p100f ? 0x1p-100f : 1.f;     // keeps 1 / max|x| a normal number; exact
-        amax *= up;
-        float r;
+        scale = plain ? Divider(127.f)(amax) : top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : amax / 127.f;
         asm("rcp.rn.f32 %0, %1;" : "=f"(r) : "f"(amax));
-        inv = finite && amax > 0.f ? 127.f * r : 0.f;
+        inv = 127.f * r;
     }
-    // neither a row of zeros nor one that needs `up`: almost every row
-    __device__ __forceinline__ bool plain() const { return up == 1.f && inv != 0.f; }
-    __device__ __forceinline__ float exact(float x) const { return i8_exact_code(x * up, amax); }
+    __device__ __forceinline__ float exact(float x) const {
+        return amax > 0.f && amax < __uint_as_float(0x7f800000u) ? i8_exact_code(x, amax) : 0.f;
+    }
     __device__ __forceinline__ int code(float x) const {
-        if (inv == 0.f) return 0;
-        const float y = x * up * inv, r = rintf(y);
-        return (int)(fabsf(y - r) > I8_BORDER ? exact(x) : r);
+        const float y = x * inv, t = rintf(y);
+        return (int)(plain && fabsf(y - t) < I8_BORDER ? t : exact(x));
     }
     // the codes of a vector, four to a word
     template <typename R>
     __device__ __forceinline__ void codes(const R& v, uint32_t (&w)[2]) const {
-        if (plain()) put<R, true>(v, w);
-        else if (inv != 0.f) put<R, false>(v, w);
-        else w[0] = w[1] = 0;
-    }
-private:
-    template <typename R, bool PLAIN>
-    __device__ __forceinline__ void put(const R& v, uint32_t (&w)[2]) const {
-        float t[R::N], far = 0.f;
+        float t[R::N];
+        bool good = plain;
+        if constexpr (sizeof(typename R::T) == 2) {
 #pragma unroll
-        for (int k = 0; k < R::N; ++k) {
-            const float y = (PLAIN ? v.get(k) : v.get(k) * up) * inv;
-            t[k] = y + I8_ROUND;
-            far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
+            for (int k = 0; k < R::N; ++k) {
+                const float n = 127.f * v.get(k), q = n * r;
+                t[k] = fmaf(fmaf(-amax, q, n), r, q) + I8_ROUND;
+            }
+        } else {
+            float far = 0.f;
+#pragma unroll
+            for (int k = 0; k < R::N; ++k) {
+                const float y = v.get(k) * inv;
+                t[k] = y + I8_ROUND;
+                far = fmaxf(far, fabsf(y - (t[k] - I8_ROUND)));
+            }
+            good = good && far < I8_BORDER;
         }
-        if (far > I8_BORDER) {
+        if (!good) {
 #pragma unroll
             for (int k = 0; k < R::N; ++k) t[k] = I8_ROUND + exact(v.get(k));
         }

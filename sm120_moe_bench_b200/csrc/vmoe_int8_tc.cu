@@ -67,7 +67,7 @@ struct I8Shared {
     int abort_flag;
     int blocks;                                           // token blocks of all experts
     int pad;
-    float row_scale[I8P_EPI_WARPS][I8P_TOKENS / 2];       // of the item in hand, each epilogue warp its own tokens
+    alignas(16) float row_scale[I8P_EPI_WARPS][I8P_TOKENS / 2];       // of the item in hand, each epilogue warp its own tokens
 };
 
 struct I8TcParams {
@@ -266,7 +266,9 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
             const uint32_t tacc = tmem + buf * I8P_TOKENS + ((uint32_t)(quad * 32) << 16);
             for (int k = sub, slot = 0; k < units; k += 4, slot += 16) {
                 const int c = (SWIGLU ? k : k >> 1) * 16, left = u.rows - c;
-                const float* cs = rs + slot;
+                float cs[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(cs + i) = *reinterpret_cast<const float4*>(rs + slot + i);
                 uint32_t v[16], v2[SWIGLU ? 16 : 1];
                 __syncwarp();
                 if (SWIGLU) {

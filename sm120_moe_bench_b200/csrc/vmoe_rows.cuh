@@ -3,6 +3,8 @@
 
 #include "vmoe_common.cuh"
 
+#include <type_traits>
+
 namespace vmoe {
 
 template <int BYTES> struct RawVec;
@@ -29,23 +31,27 @@ struct RowVec {
     __device__ __forceinline__ void load(const void* row, long long c) { raw = static_cast<const Raw*>(row)[c]; }
     __device__ __forceinline__ void store(void* row, long long c) const { static_cast<Raw*>(row)[c] = raw; }
     __device__ __forceinline__ float get(int k) const { return elem_float(reinterpret_cast<const T_*>(half)[k]); }
-    // Largest magnitude, ordered as integers (NaN > infinity > finite), joined to `top`; with 16-bit elements two at a time,
-    // and `top` holds two 16-bit maxima until magnitude() takes the larger as an f32.
+    // Largest magnitude so far, joined with this vector's; a NaN stays.  16-bit elements are compared two at a time: `top`
+    // then holds two of them.  magnitude(top) is the result as an f32's bits.
     __device__ __forceinline__ uint32_t join(uint32_t top) const {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(half);
         if constexpr (sizeof(T_) == 4) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) top = max(top, __float_as_uint(get(k)) & 0x7fffffffu);
-        } else if constexpr (BYTES >= 4) {
-#pragma unroll
-            for (int k = 0; k < BYTES / 4; ++k) top = __vmaxu2(top, reinterpret_cast<const uint32_t*>(half)[k] & 0x7fff7fffu);
+            for (int k = 0; k < N; ++k)
+                asm("max.NaN.f32 %0, %1, %2;" : "=r"(top) : "r"(top), "r"(w[k] & 0x7fffffffu));
         } else {
-            top = __vmaxu2(top, half[0] & 0x7fffu);
+#pragma unroll
+            for (int k = 0; k < (BYTES + 3) / 4; ++k) {
+                const uint32_t v = (BYTES >= 4 ? w[k] : half[0]) & 0x7fff7fffu;
+                if constexpr (std::is_same<T_, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(top) : "r"(top), "r"(v));
+                else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(top) : "r"(top), "r"(v));
+            }
         }
         return top;
     }
     __device__ static __forceinline__ uint32_t magnitude(uint32_t top) {
-        if constexpr (sizeof(T_) == 4) return top;
-        const uint16_t m = (uint16_t)max(top & 0xffffu, top >> 16);
+        if constexpr (sizeof(T_) == 4) return top & 0x7fffffffu;
+        const uint16_t m = (uint16_t)max(top & 0x7fffu, (top >> 16) & 0x7fffu);      // ordered as integers: NaN > infinity > finite
         return __float_as_uint(elem_float(*reinterpret_cast<const T_*>(&m))) & 0x7fffffffu;
     }
     __device__ __forceinline__ void set(int k, float v) { elem_store(reinterpret_cast<T_*>(half)[k], v); }

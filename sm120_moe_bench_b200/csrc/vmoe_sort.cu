@@ -80,6 +80,20 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     int kept_e[PLAN_KEPT];
 #pragma unroll
     for (int i = 0; i < PLAN_KEPT; ++i) kept_e[i] = plan_expert(ids, expert_map, map_len, E, first + 32 * i + lane, end);
+    if (MANY) {                               // the other CTAs' counts, while the ids are on their way
+        for (int e = tid; e < E; e += threads) {
+            int all = 0, front = 0;
+            for (int r0 = 0; r0 < ctas; r0 += 16) {           // sixteen loads in flight
+                int n[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
+            }
+            start[e] = all;
+            before[e] = front;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < PLAN_KEPT; ++i)
         if (kept_e[i] >= 0) atomicAdd(&mine[kept_e[i]], 1);
@@ -88,23 +102,16 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
         if (e >= 0) atomicAdd(&mine[e], 1);
     }
     __syncthreads();
-    for (int e = tid; e < E; e += threads) {
-        int all = 0, front = 0;
-        if (MANY) {
-            for (int r0 = 0; r0 < ctas; r0 += 16) {           // sixteen loads in flight
-                int n[16];
-#pragma unroll
-                for (int k = 0; k < 16; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
-            }
-        } else {
+    if (!MANY) {
+        for (int e = tid; e < E; e += threads) {
+            int all = 0;
+#pragma unroll 8
             for (int w = 0; w < warps; ++w) all += count[(size_t)w * E + e];
+            start[e] = all;
+            before[e] = 0;
         }
-        start[e] = all;
-        before[e] = front;
+        __syncthreads();
     }
-    __syncthreads();
     // exclusive prefix over the experts: every thread a contiguous run of them
     const int per = (E + threads - 1) / threads;
     int sum = 0;
@@ -138,7 +145,14 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     __syncthreads();
     for (int e = tid; e < E; e += threads) {
         int row = start[e];
-        for (int w = 0; w < warps; ++w) { const int n = count[(size_t)w * E + e]; count[(size_t)w * E + e] = row; row += n; }
+        for (int w0 = 0; w0 < warps; w0 += 8) {               // eight loads in flight
+            int n[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) n[k] = w0 + k < warps ? count[(size_t)(w0 + k) * E + e] : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (w0 + k < warps) { count[(size_t)(w0 + k) * E + e] = row; row += n[k]; }
+        }
     }
     __syncthreads();
     auto place = [&](long long p, int e) {               // one pair per lane, the whole warp
