@@ -1,10 +1,13 @@
-// The 8-bit product for a few rows (decode of one to eight tokens), in one launch: the rows are quantised inside.
+// The 8-bit product for a few rows (decode of one to eight tokens), in one launch: the rows are quantised inside.  One token,
+// N = 2048, K = 4096: 4.3 us (8.4 MB of weights: 2 TB/s, a launch alone is 2 us); N = 8192: 9.3 us (3.6 TB/s).
 //
-// Bound by reading the weights once, and at these sizes by latency: a warp owns one channel (with swiglu its gate and up
-// rows), requests the first 4 KB of it before anything else, and quantises the rows -- every CTA for itself, 8 KB from
-// L2 -- while they are on their way.  Codes lie in shared memory; four products per dp4a, integer sums joined by one
-// warp reduction, so the result is the other kernels' bit for bit.
+// Bound by reading the weights once, and at these sizes by latency: a warp requests the first 4 KB of its first channel
+// (with swiglu of its gate and up rows) before anything else and quantises the rows -- every CTA for itself, 8 KB from L2
+// -- while they are on their way; from then on each vector it uses is replaced at once by the one that comes next, of the
+// same channel or of the warp's next one.  Codes lie in shared memory; four products per dp4a, integer sums joined by
+// one warp reduction, so the result is the other kernels' bit for bit.
 #include "vmoe_int8.cuh"
+#include "vmoe_tc_common.cuh"
 
 namespace vmoe {
 
@@ -33,78 +36,102 @@ __device__ __forceinline__ uint32_t i8_weights(const uint32_t* row, int c, int s
     return __funnelshift_r(lo, hi, 8 * shift);
 }
 
-// One row into shared memory: its codes (padded with zeros to `pitch`) and scale, by the whole CTA.
-template <typename T_>
-__device__ __forceinline__ void i8_row_codes(const T_* x, int K, int pitch, uint8_t* codes, float* scale, uint32_t* s_max) {
-    const int tid = threadIdx.x;
-    uint32_t top = 0;
-    for (int k = tid; k < K; k += I8G_THREADS) top = max(top, __float_as_uint(elem_float(x[k])) & 0x7fffffffu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    __syncthreads();                                      // the row before has been read out of s_max
-    if ((tid & 31) == 0) s_max[tid >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < I8G_THREADS / 32; ++w) top = max(top, s_max[w]);
-    const I8RowScale r(top);
-    if (tid == 0) *scale = r.scale;
-    for (int k = tid; k < pitch; k += I8G_THREADS) codes[k] = k < K ? (uint8_t)r.code(elem_float(x[k])) : 0;
-}
-// The same for rows of whole 16-byte vectors.
-template <typename T_>
-__device__ __forceinline__ void i8_row_codes_vec(const T_* x, int K, int pitch, uint8_t* codes, float* scale, uint32_t* s_max) {
+// The rows into shared memory as codes (padded with zeros to `pitch`) and scales, all at once: the CTA's warps share the
+// ROWS rows out.  Rows of whole 16-byte vectors; a thread keeps up to eight of its vectors between the two passes.
+template <typename T_, int ROWS>
+__device__ __forceinline__ void i8_rows_vec(const uint8_t* x, long long x_stride, int M, int K, int pitch, uint8_t* codes, float* scales, uint32_t* s_max) {
     using R = RowVec<T_, 16>;
-    const int tid = threadIdx.x, vecs = K / R::N;
-    constexpr int KEPT = 4;
+    constexpr int WPR = 8 / ROWS, STEP = WPR * 32, KEPT = 8;
+    const int warp = threadIdx.x >> 5, m = warp / WPR, part = (warp % WPR) * 32 + (threadIdx.x & 31), vecs = K / R::N;
+    const uint8_t* src = x + m * x_stride;
     uint32_t top = 0;
     R keep[KEPT];
+    if (m < M) {
 #pragma unroll
-    for (int i = 0; i < KEPT; ++i)
-        if (tid + i * I8G_THREADS < vecs) keep[i].load(x, tid + i * I8G_THREADS);
+        for (int i = 0; i < KEPT; ++i)
+            if (part + i * STEP < vecs) keep[i].load(src, part + i * STEP);
 #pragma unroll
-    for (int i = 0; i < KEPT; ++i)
-        if (tid + i * I8G_THREADS < vecs) top = keep[i].join(top);
-    for (int c = tid + KEPT * I8G_THREADS; c < vecs; c += I8G_THREADS) {
-        R v;
-        v.load(x, c);
-        top = v.join(top);
+        for (int i = 0; i < KEPT; ++i)
+            if (part + i * STEP < vecs) top = keep[i].join(top);
+        for (int c = part + KEPT * STEP; c < vecs; c += STEP) {
+            R v;
+            v.load(src, c);
+            top = v.join(top);
+        }
     }
     top = __reduce_max_sync(0xffffffffu, R::magnitude(top));
+    if ((threadIdx.x & 31) == 0) s_max[warp] = top;
     __syncthreads();
-    if ((tid & 31) == 0) s_max[tid >> 5] = top;
-    __syncthreads();
+    if (m >= M) return;
 #pragma unroll
-    for (int w = 0; w < I8G_THREADS / 32; ++w) top = max(top, s_max[w]);
+    for (int w = 0; w < WPR; ++w) top = max(top, s_max[m * WPR + w]);
     const I8RowScale r(top);
-    if (tid == 0) *scale = r.scale;
+    uint8_t* dst = codes + (size_t)m * pitch;
+    if (part == 0) scales[m] = r.scale;
     auto put = [&](const R& v, int c) {
         uint32_t w[2] = {0, 0};
         r.codes(v, w);
-        if (R::N == 8) *reinterpret_cast<uint2*>(codes + c * 8) = make_uint2(w[0], w[1]);
-        else *reinterpret_cast<uint32_t*>(codes + c * 4) = w[0];
+        if (R::N == 8) *reinterpret_cast<uint2*>(dst + c * 8) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(dst + c * 4) = w[0];
     };
 #pragma unroll
     for (int i = 0; i < KEPT; ++i)
-        if (tid + i * I8G_THREADS < vecs) put(keep[i], tid + i * I8G_THREADS);
-    for (int c = tid + KEPT * I8G_THREADS; c < vecs; c += I8G_THREADS) {
+        if (part + i * STEP < vecs) put(keep[i], part + i * STEP);
+    for (int c = part + KEPT * STEP; c < vecs; c += STEP) {
         R v;
-        v.load(x, c);
+        v.load(src, c);
         put(v, c);
     }
-    for (int k = K + tid; k < pitch; k += I8G_THREADS) codes[k] = 0;
+    for (int k = K + part; k < pitch; k += STEP) dst[k] = 0;
 }
-__device__ __forceinline__ void i8_row_copy(const int8_t* a, int K, int pitch, uint8_t* codes) {
-    const int tid = threadIdx.x;
-    if (((uintptr_t)a & 15) == 0) {
-        for (int k = tid * 16; k < K / 16 * 16; k += I8G_THREADS * 16) *reinterpret_cast<uint4*>(codes + k) = *reinterpret_cast<const uint4*>(a + k);
-        for (int k = K / 16 * 16 + tid; k < pitch; k += I8G_THREADS) codes[k] = k < K ? (uint8_t)a[k] : 0;
-    } else {
-        for (int k = tid; k < pitch; k += I8G_THREADS) codes[k] = k < K ? (uint8_t)a[k] : 0;
+// The same for rows of any length and alignment.
+template <typename T_, int ROWS>
+__device__ __forceinline__ void i8_rows(const uint8_t* x, long long x_stride, int M, int K, int pitch, uint8_t* codes, float* scales, uint32_t* s_max) {
+    constexpr int WPR = 8 / ROWS, STEP = WPR * 32;
+    const int warp = threadIdx.x >> 5, m = warp / WPR, part = (warp % WPR) * 32 + (threadIdx.x & 31);
+    const T_* src = reinterpret_cast<const T_*>(x + m * x_stride);
+    uint32_t top = 0;
+    if (m < M) {
+#pragma unroll 4
+        for (int k = part; k < K; k += STEP) top = max(top, __float_as_uint(elem_float(src[k])) & 0x7fffffffu);
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) s_max[warp] = top;
+    __syncthreads();
+    if (m >= M) return;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) top = max(top, s_max[m * WPR + w]);
+    const I8RowScale r(top);
+    uint8_t* dst = codes + (size_t)m * pitch;
+    if (part == 0) scales[m] = r.scale;
+#pragma unroll 4
+    for (int k = part; k < pitch; k += STEP) dst[k] = k < K ? (uint8_t)r.code(elem_float(src[k])) : 0;
+}
+// Rows that are codes already.
+__device__ __forceinline__ void i8_rows_copy(const int8_t* a, long long a_stride, int M, int K, int pitch, uint8_t* codes) {
+    const int vecs = pitch / 16;
+    const bool aligned = (((uintptr_t)a | (unsigned long long)a_stride) & 15) == 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < M * vecs; i += I8G_THREADS) {
+        const int m = i / vecs, k = (i - m * vecs) * 16;
+        const int8_t* src = a + m * a_stride + k;
+        uint4 v;
+        if (aligned && k + 16 <= K) {
+            v = *reinterpret_cast<const uint4*>(src);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (k + j < K) w[j >> 2] |= (uint32_t)(uint8_t)src[j] << (8 * (j & 3));
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        *reinterpret_cast<uint4*>(codes + (size_t)m * pitch + k) = v;
     }
 }
 
 // x_dtype < 0: p.a / p.a_scale hold the rows; else x does.
 template <int VB, int ROWS, bool SWIGLU>
-__global__ void __launch_bounds__(I8G_THREADS)
+__global__ void __launch_bounds__(I8G_THREADS, 2)
 i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dtype, int x_vec) {
     using W = typename I8Word<VB>::type;
     constexpr int AHEAD = VB == 16 ? 8 : 16, SETS = SWIGLU ? 2 : 1;
@@ -112,87 +139,102 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
     __shared__ uint32_t s_max[I8G_THREADS / 32];
     __shared__ float s_scale[ROWS];
     pdl_begin();
-    const int lane = threadIdx.x & 31, n = blockIdx.x * (I8G_THREADS / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, stride = gridDim.x * (I8G_THREADS / 32);
+    int n = blockIdx.x * (I8G_THREADS / 32) + (threadIdx.x >> 5);
     const int K = p.K, pitch = (K + 15) & ~15, words = (K + VB - 1) / VB;
-    const bool on = n < p.N;
     const W* w[SETS];
     int shift[SETS];
+    float scale[SETS] = {};                               // of the channel whose vectors come next: requested with them
+    auto channel = [&](int c) {
 #pragma unroll
-    for (int s = 0; s < SETS; ++s) {
-        const uintptr_t at = (uintptr_t)(p.w + (long long)(s * p.N + (on ? n : 0)) * p.w_stride);
-        shift[s] = VB == 4 ? (int)(at & 3) : 0;
-        w[s] = reinterpret_cast<const W*>(at - shift[s]);
-    }
+        for (int s = 0; s < SETS; ++s) {
+            scale[s] = p.w_scale[s * p.N + c];
+            const uintptr_t at = (uintptr_t)(p.w + (long long)(s * p.N + c) * p.w_stride);
+            shift[s] = VB == 4 ? (int)(at & 3) : 0;
+            w[s] = reinterpret_cast<const W*>(at - shift[s]);
+        }
+    };
     W have[SETS][AHEAD];
+    if (n < p.N) channel(n);
 #pragma unroll
     for (int s = 0; s < SETS; ++s)
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             have[s][i] = W{};
-            if (lane + 32 * i < words) have[s][i] = i8_weights(w[s], lane + 32 * i, shift[s], K);
+            if (n < p.N && lane + 32 * i < words) have[s][i] = i8_weights(w[s], lane + 32 * i, shift[s], K);
         }
-    for (int m = 0; m < p.M; ++m) {
-        uint8_t* dst = codes + (size_t)m * pitch;
-        if (x_dtype < 0) {
-            i8_row_copy(p.a + m * p.a_stride, K, pitch, dst);
-            if (threadIdx.x == 0) s_scale[m] = p.a_scale[m];
-        } else {
-            const uint8_t* src = x + m * x_stride;
-#define VMOE_I8_ROW(T) (x_vec ? i8_row_codes_vec(reinterpret_cast<const T*>(src), K, pitch, dst, &s_scale[m], s_max) \
-                              : i8_row_codes(reinterpret_cast<const T*>(src), K, pitch, dst, &s_scale[m], s_max))
-            if (x_dtype == VMOE_BF16) VMOE_I8_ROW(__nv_bfloat16);
-            else if (x_dtype == VMOE_F16) VMOE_I8_ROW(__half);
-            else VMOE_I8_ROW(float);
-#undef VMOE_I8_ROW
-        }
+    if (x_dtype < 0) {
+        i8_rows_copy(p.a, p.a_stride, p.M, K, pitch, codes);
+        if (threadIdx.x < p.M) s_scale[threadIdx.x] = p.a_scale[threadIdx.x];
+    } else {
+#define VMOE_I8_ROWS(T) (x_vec ? i8_rows_vec<T, ROWS>(x, x_stride, p.M, K, pitch, codes, s_scale, s_max) \
+                               : i8_rows<T, ROWS>(x, x_stride, p.M, K, pitch, codes, s_scale, s_max))
+        if (x_dtype == VMOE_BF16) VMOE_I8_ROWS(__nv_bfloat16);
+        else if (x_dtype == VMOE_F16) VMOE_I8_ROWS(__half);
+        else VMOE_I8_ROWS(float);
+#undef VMOE_I8_ROWS
     }
     __syncthreads();
-    if (!on) return;
-    int acc[SETS][ROWS] = {};
-    for (int c0 = 0; c0 < words; c0 += 32 * AHEAD) {
+    for (; n < p.N; n += stride) {
+        int acc[SETS][ROWS] = {};
+        float sw[SETS];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            const int c = c0 + lane + 32 * i;
-            if (c < words) {
-                // bytes behind K meet zero codes
+        for (int s = 0; s < SETS; ++s) sw[s] = scale[s];
+        for (int c0 = 0; c0 < words; c0 += 32 * AHEAD) {
+            const bool last = c0 + 32 * AHEAD >= words;
+            const int next = last ? 0 : c0 + 32 * AHEAD;
+            const bool more = !last || n + stride < p.N;
+            if (last && more) channel(n + stride);
 #pragma unroll
-                for (int m = 0; m < ROWS; ++m) {
-                    if (m >= p.M) break;
-                    const W a = *reinterpret_cast<const W*>(codes + (size_t)m * pitch + (size_t)c * VB);
+            for (int i = 0; i < AHEAD; ++i) {
+                const int c = c0 + lane + 32 * i;
+                if (c < words) {
+                    // bytes behind K meet zero codes
 #pragma unroll
-                    for (int s = 0; s < SETS; ++s) acc[s][m] = i8_dot(have[s][i], a, acc[s][m]);
+                    for (int m = 0; m < ROWS; ++m) {
+                        if (m >= p.M) break;
+                        const W a = *reinterpret_cast<const W*>(codes + (size_t)m * pitch + (size_t)c * VB);
+#pragma unroll
+                        for (int s = 0; s < SETS; ++s) acc[s][m] = i8_dot(have[s][i], a, acc[s][m]);
+                    }
+                }
+                const int cn = next + lane + 32 * i;
+                if (more && cn < words) {
+#pragma unroll
+                    for (int s = 0; s < SETS; ++s) have[s][i] = i8_weights(w[s], cn, shift[s], K);
                 }
             }
         }
+        float mine = 0.f;
 #pragma unroll
-        for (int s = 0; s < SETS; ++s)
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int c = c0 + 32 * AHEAD + lane + 32 * i;
-                if (c < words) have[s][i] = i8_weights(w[s], c, shift[s], K);
-            }
+        for (int m = 0; m < ROWS; ++m) {
+            if (m >= p.M) break;
+            float v = i8_scaled(__reduce_add_sync(0xffffffffu, acc[0][m]), s_scale[m], sw[0]);
+            if (SWIGLU) v = i8_scaled(__reduce_add_sync(0xffffffffu, acc[SETS - 1][m]), s_scale[m], sw[SETS - 1]) * i8_silu(v);
+            if (lane == m) mine = v;
+        }
+        if (lane < p.M) i8_store(p.out, lane * p.out_stride + n, p.out_dtype, mine);
     }
-    float mine = 0.f;
-#pragma unroll
-    for (int m = 0; m < ROWS; ++m) {
-        if (m >= p.M) break;
-        float v = i8_scaled(__reduce_add_sync(0xffffffffu, acc[0][m]), s_scale[m], p.w_scale[n]);
-        if (SWIGLU) v = i8_scaled(__reduce_add_sync(0xffffffffu, acc[SETS - 1][m]), s_scale[m], p.w_scale[p.N + n]) * i8_silu(v);
-        if (lane == m) mine = v;
-    }
-    if (lane < p.M) i8_store(p.out, lane * p.out_stride + n, p.out_dtype, mine);
 }
 
+// Measured against quantiser + tensor-core product (K = 4096, us): N = 2048, 1 / 4 / 8 rows 4.3 / 6.3 / 9.4 against 12;
+// N = 4096, 1 / 4 / 6 rows 6.4 / 9.0 / 11.9 against 10; N = 8192, 1 / 4 / 6 rows 9.3 / 13.2 / 17.2 against 12.8.  So up to four
+// rows, up to eight of weights of at most 8 MB; rows the tensor cores could only read after packing up to eight.
 bool i8_gemv_ok(const I8Problem& p) {
-    return p.E == 1 && !p.offsets && p.M <= I8_GEMV_ROWS && p.K > 0 && p.w_stride >= p.K && (long long)p.M * ((p.K + 15) & ~15) <= I8G_SMEM;
+    if (p.E != 1 || p.offsets || p.M > I8_GEMV_ROWS || p.K <= 0 || p.w_stride < p.K) return false;
+    if ((long long)p.M * ((p.K + 15) & ~15) > I8G_SMEM) return false;
+    return p.M <= 4 || (long long)p.wrows * p.K <= (8 << 20) || (((uintptr_t)p.w | (unsigned long long)p.w_stride) & 15) != 0;
 }
 
 template <int VB, int ROWS, bool SWIGLU>
 static int launch_gemv(const I8Problem& p, const void* x, long long x_stride, int x_dtype, int x_vec, cudaStream_t st) {
     const size_t smem = (size_t)p.M * ((p.K + 15) & ~15);
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(i8_gemv_kernel<VB, ROWS, SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8G_SMEM) != cudaSuccess)
-        return VMOE_ERR_CUDA;
-    return cuda_status(launch_pdl(i8_gemv_kernel<VB, ROWS, SWIGLU>, (unsigned)((p.N + 7) / 8), (unsigned)I8G_THREADS, smem, st, p,
+    static SmemAllowed done;
+    if (allow_smem(i8_gemv_kernel<VB, ROWS, SWIGLU>, I8G_SMEM, done) != cudaSuccess) return VMOE_ERR_CUDA;
+    // two CTAs an SM, every warp the same number of channels
+    const long long warps = 2LL * tc_sm_count() * (I8G_THREADS / 32), rounds = (p.N + warps - 1) / warps;
+    const unsigned grid = (unsigned)((p.N + rounds * (I8G_THREADS / 32) - 1) / (rounds * (I8G_THREADS / 32)));
+    return cuda_status(launch_pdl(i8_gemv_kernel<VB, ROWS, SWIGLU>, grid, (unsigned)I8G_THREADS, smem, st, p,
                                   static_cast<const uint8_t*>(x), x_stride, x_dtype, x_vec));
 }
 template <int VB, bool SWIGLU>

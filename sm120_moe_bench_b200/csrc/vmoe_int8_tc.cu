@@ -506,13 +506,15 @@ bool i8_tc_ok(const I8Problem& p) {
 
 constexpr size_t I8P_SMEM = 227 * 1024;
 
-// Tokens per item.  Grouped: from the average rows per expert (the counts are on the device).  Dense: the size whose last
-// round of items over the SMs wastes least -- a k-block costs the larger of 4 U (tensor pipe) and 512 + 2 U cycles
-// (ingest), an item of more than 128 tokens its epilogue on top (about 20 cycles a token).
+// Tokens per item.  Grouped: from the average rows per expert (the counts are on the device); 64 experts, N = 1024, K = 4096,
+// items of 64 / 128 / 256 tokens: 16 rows each 46 / 47 / 48 us, 100 rows 64 / 56 / 57, 160 rows 85 / 75 / 66, 320 rows
+// 134 / 111 / 103.  Dense: the size whose last round of items over the SMs wastes least -- a k-block costs the larger of 4 U
+// (tensor pipe) and 512 + 2 U cycles (ingest), an item of more than 128 tokens its epilogue on top (about 20 cycles a
+// token); 8192 x 4096 x 4096: 224 tokens (the choice) 92.5 us, 128 107, 192 101, 256 97.
 static int i8_tokens(const I8Problem& p, int kblocks, int ctiles) {
     if (p.offsets) {
         const long long per = p.M / p.E;
-        return per <= 32 ? 64 : per <= 128 || kblocks < 16 ? 128 : I8P_TOKENS;
+        return per <= 32 ? 64 : per <= 128 ? 128 : I8P_TOKENS;
     }
     int best = 128;
     long long least = -1;
@@ -547,7 +549,8 @@ static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
     const long long blocks = ((long long)p.M + P.tokens - 1) / P.tokens + (p.E > 1 ? (p.E < p.M ? p.E : p.M) : 0);
     const long long items = blocks * P.ctiles;
     const unsigned grid = (unsigned)(items < tc_sm_count() ? items : tc_sm_count());
-    if (cudaFuncSetAttribute(i8_tc_kernel<SWIGLU, O_>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)I8P_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    static SmemAllowed done;
+    if (allow_smem(i8_tc_kernel<SWIGLU, O_>, I8P_SMEM, done) != cudaSuccess) return VMOE_ERR_CUDA;
     return cuda_status(launch_pdl(i8_tc_kernel<SWIGLU, O_>, grid, (unsigned)I8P_THREADS, smem, st, P));
 }
 int launch_i8_tc(const I8Problem& p, cudaStream_t st) {
@@ -586,7 +589,8 @@ static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
     int rc;
     if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 64 : 128))) return rc;
     if ((rc = i8_map_a(&P.map_a64, p, (uint32_t)P.tokens))) return rc;
-    if (cudaFuncSetAttribute(i8_split_kernel<SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8S_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    static SmemAllowed done;
+    if (allow_smem(i8_split_kernel<SWIGLU>, I8S_SMEM, done) != cudaSuccess) return VMOE_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)split, (unsigned)P.ctiles, (unsigned)ttiles); cfg.blockDim = dim3(I8S_THREADS);
     cfg.dynamicSmemBytes = smem; cfg.stream = st;

@@ -63,6 +63,18 @@ inline int vector_bytes(uintptr_t addresses, long long lengths) {
     return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
+// More than 48 KB of dynamic shared memory have to be allowed once per device and kernel; `done` is the caller's, one for each.
+struct SmemAllowed { bool on[64] = {}; };
+template <typename F>
+inline cudaError_t allow_smem(F* kernel, size_t bytes, SmemAllowed& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && done.on[dev])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.on[dev] = true;
+    return e;
+}
+
 // f(RowTag) for the wanted type and width
 template <typename T_, int BYTES_>
 struct RowTag {

@@ -354,11 +354,13 @@ static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_le
     run = (run + 31) / 32 * 32;
     const size_t smem = (size_t)4 * E * (warps + 2);
     if (ctas == 1) {
-        if (cudaFuncSetAttribute(plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+        static SmemAllowed one;
+        if (allow_smem(plan_kernel<false>, PLAN_SMEM, one) != cudaSuccess) return VMOE_ERR_CUDA;
         return cuda_status(launch_pdl(plan_kernel<false>, 1u, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
                                       (const int32_t*)nullptr, offsets, row_of_pair, pair_of_row));
     }
-    if (cudaFuncSetAttribute(plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PLAN_SMEM) != cudaSuccess) return VMOE_ERR_CUDA;
+    static SmemAllowed many;
+    if (allow_smem(plan_kernel<true>, PLAN_SMEM, many) != cudaSuccess) return VMOE_ERR_CUDA;
     const cudaError_t e = launch_pdl(plan_count_kernel, (unsigned)ctas, 1024u, (size_t)4 * E, st, ids, expert_map, map_len, P, E, run * warps, scratch);
     if (e != cudaSuccess) return VMOE_ERR_CUDA;
     return cuda_status(launch_pdl(plan_kernel<true>, (unsigned)ctas, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,

@@ -96,9 +96,10 @@ def _aligned(q: torch.Tensor) -> bool:
 
 
 def _packs(w: Int8Rows, rows: int) -> bool:
-    """Whether unaligned weights are worth a copy for a product with this many rows (the reason stands at the C side's
-    ``i8_product_any``).  Up to eight rows of a single matrix have a kernel of their own that reads them anywhere."""
-    return rows > 8 if w.q.dim() == 2 else rows >= 16 * w.q.shape[0]
+    """Whether unaligned weights are worth a copy for a product with this many rows (figures at the C side's
+    ``i8_product_any``): not below one row per matrix, since the copy reads every matrix, nor for the few rows of a dense
+    product whose kernel reads weights at any alignment."""
+    return rows > 8 if w.q.dim() == 2 else rows >= w.q.shape[0]
 
 
 def int8_status(device: torch.device | str | int = "cuda") -> int:
@@ -172,7 +173,7 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
     M, K = x.shape
     wq = w.q
     need = 0
-    if M > 8 or not 0 < K <= 8192 or wq.stride(0) < K:    # else the rows are quantised inside the product
+    if M > 4 or not 0 < K <= 8192 or wq.stride(0) < K:    # else the rows are quantised inside the product
         need = lib.vmoe_int8_linear_scratch_bytes(M, K)
         if not _aligned(wq) and _packs(w, M):
             need += lib.vmoe_int8_pack_bytes(M, wq.shape[0], K, 1)
