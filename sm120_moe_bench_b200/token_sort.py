@@ -184,9 +184,26 @@ class _SortTokens(torch.autograd.Function):
         return _sort(x, plan)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        return _unsort(_dense_rows(grad), ctx.plan), None
+        grad = _dense_rows(grad)
+        # with create_graph the gradient is differentiable itself
+        return (unsort_tokens if torch.is_grad_enabled() else _unsort)(grad, ctx.plan), None
+
+
+def _unsort_backward(ctx, grad):
+    rows, weights = ctx.saved_tensors
+    plan, grad = ctx.plan, _dense_rows(grad)
+    M, T, K = plan.tokens, plan.topk, rows.shape[1]
+    drows = rows.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
+    dw = torch.empty((M, T), dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[2] else None
+    launch(rows.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0), rows.data_ptr(),
+           rows.stride(0), DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
+           None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(), K,
+           None if dw is None else dw.data_ptr())
+    return drows, None, dw
+
+
+_unsort_backward_once = torch.autograd.function.once_differentiable(_unsort_backward)
 
 
 class _UnsortTokens(torch.autograd.Function):
@@ -197,18 +214,9 @@ class _UnsortTokens(torch.autograd.Function):
         return _unsort(rows, plan, weights)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        rows, weights = ctx.saved_tensors
-        plan, grad = ctx.plan, _dense_rows(grad)
-        M, T, K = plan.tokens, plan.topk, rows.shape[1]
-        drows = rows.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(M, T, dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[2] else None
-        launch(rows.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0), rows.data_ptr(),
-               rows.stride(0), DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
-               None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(),
-               K, None if dw is None else dw.data_ptr())
-        return drows, None, dw
+        # once_differentiable only matters, and only costs, where a graph of the gradient is asked for
+        return (_unsort_backward_once if torch.is_grad_enabled() else _unsort_backward)(ctx, grad)
 
 
 def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -173,6 +173,23 @@ def test_gradients_against_differences():
                 assert abs(float((a - b) / (2 * step)) - float(d.view(-1)[i])) <= tol
 
 
+def test_gradient_of_the_gradient():
+    import sm120_moe_bench_b200 as vm
+    plan = vm.plan_tokens(ids_of(9, 3, 5, 35), 5)
+    x, g = rows_of(9, 12, torch.float32, 36).requires_grad_(), rows_of(27, 12, torch.float32, 37).requires_grad_()
+    dx, = torch.autograd.grad(vm.sort_tokens(x, plan), x, g, create_graph=True)
+    v = rows_of(9, 12, torch.float32, 38)
+    dg, = torch.autograd.grad(dx, g, v)                    # dx is linear in g: its gradient sorts v
+    assert torch.equal(dg, vm.sort_tokens(v, plan))
+    w = torch.rand(9, 3, device="cuda").requires_grad_()
+    dy = rows_of(9, 12, torch.float32, 39).requires_grad_()
+    y = vm.unsort_tokens(g, plan, w)
+    once = torch.autograd.grad(y, (g, w), dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(once, torch.autograd.grad(vm.unsort_tokens(g, plan, w), (g, w), dy)))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        once[0].sum().backward()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strides_and_alignment(dtype):
     import sm120_moe_bench_b200 as vm
