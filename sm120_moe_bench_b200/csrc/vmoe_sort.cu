@@ -25,9 +25,9 @@ namespace vmoe {
 // ---------------------------------------------------------------------------------
 constexpr int PLAN_MAX_EXPERTS = 8192;
 constexpr int PLAN_ONE_CTA_PAIRS = 4096;
-constexpr int PLAN_PAIRS_PER_CTA = 4096;
+constexpr int PLAN_PAIRS_PER_CTA = 1024;        // 4096: placing them takes 9500 cycles of a CTA's 19700
 constexpr int PLAN_KEPT = 4;                 // experts of a lane's first pairs stay in registers between the passes
-constexpr int PLAN_MAX_CTAS = 64;
+constexpr int PLAN_MAX_CTAS = 148;
 constexpr int PLAN_SMEM = 200 * 1024;
 
 static int plan_ctas(long long pairs) {
@@ -70,7 +70,7 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     int* start = count + (size_t)warps * E;   // [E] all CTAs' pairs, then the first row of this CTA's pairs
     int* before = start + E;                  // [E] pairs of the CTAs in front
     const int rank = (int)blockIdx.x, ctas = (int)gridDim.x;
-    for (int i = tid; i < warps * E; i += threads) count[i] = 0;
+    for (int i = tid; i < (warps + (MANY ? 2 : 0)) * E; i += threads) count[i] = 0;       // start and before lie behind count
     __syncthreads();
     pdl_begin();
 
@@ -80,18 +80,20 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     int kept_e[PLAN_KEPT];
 #pragma unroll
     for (int i = 0; i < PLAN_KEPT; ++i) kept_e[i] = plan_expert(ids, expert_map, map_len, E, first + 32 * i + lane, end);
-    if (MANY) {                               // the other CTAs' counts, while the ids are on their way
-        for (int e = tid; e < E; e += threads) {
+    if (MANY) {                               // the CTAs' counts, while the ids are on their way: `parts` threads per expert
+        const int parts = threads >= 2 * E ? threads / E : 1;
+        for (int i = tid; i < parts * E; i += threads) {
+            const int e = i % E, part = i / E;
             int all = 0, front = 0;
-            for (int r0 = 0; r0 < ctas; r0 += 16) {           // sixteen loads in flight
+            for (int r0 = part; r0 < ctas; r0 += 16 * parts) {           // sixteen loads in flight
                 int n[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) n[k] = r0 + k < ctas ? counts[(size_t)(r0 + k) * E + e] : 0;
+                for (int k = 0; k < 16; ++k) n[k] = r0 + k * parts < ctas ? counts[(size_t)(r0 + k * parts) * E + e] : 0;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) { all += n[k]; front += r0 + k < rank ? n[k] : 0; }
+                for (int k = 0; k < 16; ++k) { all += n[k]; front += r0 + k * parts < rank ? n[k] : 0; }
             }
-            start[e] = all;
-            before[e] = front;
+            atomicAdd(&start[e], all);
+            atomicAdd(&before[e], front);
         }
     }
 #pragma unroll
@@ -196,76 +198,123 @@ __device__ __forceinline__ void zero_rows(uint8_t* rows, long long stride, long 
     }
 }
 
+// Which vectors of which token a thread owns.  U = 1: vector i of all tokens' vectors in a row.  U > 1 (rows that only allow
+// narrow vectors): a warp owns 32 U neighbours of one token, a lane every 32nd of them, so that a thread has as many bytes in
+// flight as with one wide vector.
+template <int U>
+struct Share {
+    long long m, c;
+    bool on;
+    __device__ __forceinline__ Share(long long vecs, int M) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+        if (U == 1) {
+            on = i < (long long)M * vecs;
+            if (on) row_and_vector(i, vecs, m, c);
+        } else {
+            const long long tiles = (vecs + 32 * U - 1) / (32 * U);
+            on = (i >> 5) < M * tiles;
+            if (on) {
+                row_and_vector(i >> 5, tiles, m, c);
+                c = c * 32 * U + (i & 31);
+            }
+        }
+    }
+    __device__ __forceinline__ bool has(int u, long long vecs) const { return U == 1 || c + 32 * u < vecs; }
+};
+static unsigned share_blocks(long long vecs, int M, int U) {
+    const long long threads = U == 1 ? M * vecs : 32 * M * ((vecs + 32 * U - 1) / (32 * U));
+    return (unsigned)((threads + 255) / 256);
+}
+// Narrow vectors: as many as make 16 bytes, where a row has enough of them.
+static constexpr int share_of(int vector_bytes, long long vecs) { return vector_bytes < 16 && vecs >= 64 ? 16 / vector_bytes : 1; }
+
 // ---------------------------------------------------------------------------------
-// Sort: a thread reads one vector of one token and stores it to the token's T rows, so a token is read once and the
+// Sort: a thread reads its vectors of one token and stores them to the token's T rows, so a token is read once and the
 // rest of the traffic is the rows' own writes.  Rows nobody owns (dropped pairs leave them behind the last kept row)
-// are zeroed when the caller wants every row defined.
+// are zeroed when the caller wants every row defined.  Bound by the writes: 8192 x 10 rows of 4096 bf16 6.1 TB/s (0.93 of a
+// copy's); rows of 1021 f32 (4-byte vectors) 3.6 TB/s with one vector a thread, 6.6 (part of it L2) with four.
 // ---------------------------------------------------------------------------------
 constexpr int SORT_BATCH = 4;
 
-template <typename V>
+template <typename V, int U>
 __global__ void __launch_bounds__(256)
 sort_kernel(const uint8_t* x, long long x_stride, uint8_t* rows, long long rows_stride, long long vecs,
             int M, int T, const int32_t* row_of_pair, const int32_t* kept, int zero_tail) {
     pdl_begin();
     if (zero_tail) zero_rows<V>(rows, rows_stride, *kept, (long long)M * T, vecs);
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, all = (long long)M * vecs;
-    if (i >= all) return;
-    long long m, c;
-    row_and_vector(i, vecs, m, c);
-    const V v = reinterpret_cast<const V*>(x + m * x_stride)[c];
-    const int32_t* rp = row_of_pair + m * T;
+    const Share<U> s(vecs, M);
+    if (!s.on) return;
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        if (s.has(u, vecs)) v[u] = reinterpret_cast<const V*>(x + s.m * x_stride)[s.c + 32 * u];
+    const int32_t* rp = row_of_pair + s.m * T;
     for (int t0 = 0; t0 < T; t0 += SORT_BATCH) {
         int r[SORT_BATCH];
 #pragma unroll
         for (int j = 0; j < SORT_BATCH; ++j) r[j] = t0 + j < T ? rp[t0 + j] : -1;
 #pragma unroll
         for (int j = 0; j < SORT_BATCH; ++j)
-            if (r[j] >= 0) reinterpret_cast<V*>(rows + r[j] * rows_stride)[c] = v;
+            if (r[j] >= 0) {
+                V* dst = reinterpret_cast<V*>(rows + r[j] * rows_stride) + s.c;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (s.has(u, vecs)) dst[32 * u] = v[u];
+            }
     }
 }
 
 // ---------------------------------------------------------------------------------
-// Unsort: a thread owns one vector of one token and sums it over the token's pairs in order; four rows are requested
-// at a time.  Rows in f32 may leave as bf16 / fp16: the expert layer's rows stay in f32 until they are summed.
+// Unsort: a thread sums its vectors of one token over the token's pairs in order; BATCH rows are requested at a time.
+// Bound by reading the rows.  BATCH divides T as evenly as up to five rows allow: with 4 for every T, 10 choices of 4096
+// bf16 reach 5.6 TB/s and 8 choices 6.0; with 5, 6.0 and 5.6.  Rows in f32 may leave as bf16 / fp16: the expert layer's
+// rows stay in f32 until they are summed.
 // ---------------------------------------------------------------------------------
-constexpr int UNSORT_BATCH = 4;
-
-template <typename T_, int VB, typename O_>
+template <typename T_, int VB, typename O_, int BATCH, int U>
 __global__ void __launch_bounds__(256)
 unsort_kernel(const uint8_t* rows, long long rows_stride, uint8_t* out, long long out_stride, long long vecs,
               int M, int T, const int32_t* row_of_pair, const float* weights) {
     using R = RowVec<T_, VB>;
     pdl_begin();
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)M * vecs) return;
-    long long m, c;
-    row_and_vector(i, vecs, m, c);
-    float acc[R::N];
+    const Share<U> s(vecs, M);
+    if (!s.on) return;
+    float acc[U][R::N];
 #pragma unroll
-    for (int k = 0; k < R::N; ++k) acc[k] = 0.f;
-    const int32_t* rp = row_of_pair + m * T;
-    for (int t0 = 0; t0 < T; t0 += UNSORT_BATCH) {
-        R v[UNSORT_BATCH];
-        int r[UNSORT_BATCH];
-        float w[UNSORT_BATCH];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < UNSORT_BATCH; ++j) {
+        for (int k = 0; k < R::N; ++k) acc[u][k] = 0.f;
+    const int32_t* rp = row_of_pair + s.m * T;
+    for (int t0 = 0; t0 < T; t0 += BATCH) {
+        R v[BATCH][U];
+        int r[BATCH];
+        float w[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
             r[j] = t0 + j < T ? rp[t0 + j] : -1;
-            w[j] = r[j] >= 0 && weights ? weights[m * T + t0 + j] : 1.f;
-            if (r[j] >= 0) v[j].load(rows + r[j] * rows_stride, c);
-        }
-#pragma unroll
-        for (int j = 0; j < UNSORT_BATCH; ++j)
+            w[j] = r[j] >= 0 && weights ? weights[s.m * T + t0 + j] : 1.f;
             if (r[j] >= 0) {
 #pragma unroll
-                for (int k = 0; k < R::N; ++k) acc[k] = fmaf(w[j], v[j].get(k), acc[k]);
+                for (int u = 0; u < U; ++u)
+                    if (s.has(u, vecs)) v[j][u].load(rows + r[j] * rows_stride, s.c + 32 * u);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j)
+            if (r[j] >= 0) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int k = 0; k < R::N; ++k) acc[u][k] = fmaf(w[j], v[j][u].get(k), acc[u][k]);
             }
     }
-    RowVec<O_, R::N * (int)sizeof(O_)> o;
 #pragma unroll
-    for (int k = 0; k < R::N; ++k) o.set(k, acc[k]);
-    o.store(out + m * out_stride, c);
+    for (int u = 0; u < U; ++u)
+        if (s.has(u, vecs)) {
+            RowVec<O_, R::N * (int)sizeof(O_)> o;
+#pragma unroll
+            for (int k = 0; k < R::N; ++k) o.set(k, acc[u][k]);
+            o.store(out + s.m * out_stride, s.c + 32 * u);
+        }
 }
 
 // ---------------------------------------------------------------------------------
@@ -273,6 +322,8 @@ unsort_kernel(const uint8_t* rows, long long rows_stride, uint8_t* out, long lon
 // dot products with dy[m] and their gradients written in the same pass.  Order of a dot product: a thread's vectors
 // in ascending order, the warp's xor tree, the warps in order.
 // ---------------------------------------------------------------------------------
+constexpr int UNSORT_BATCH = 4;
+
 template <typename T_, int VB, int WPT>
 __global__ void __launch_bounds__(256)
 unsort_grad_kernel(const uint8_t* dy, long long dy_stride, const uint8_t* rows, long long rows_stride,
@@ -295,28 +346,38 @@ unsort_grad_kernel(const uint8_t* dy, long long dy_stride, const uint8_t* rows, 
                 w[j] = r[j] >= 0 && weights ? weights[m * T + t0 + j] : 1.f;
                 dot[j] = 0.f;
             }
-            for (int c = part; c < vecs; c += WPT * 32) {
-                R g, v[UNSORT_BATCH];
-                g.load(dy + m * dy_stride, c);
+            constexpr int U = VB < 16 ? 8 / VB < 2 ? 2 : 8 / VB : 1;         // narrow vectors: several in flight
+            for (int c0 = part; c0 < vecs; c0 += WPT * 32 * U) {
+                R g[U], v[UNSORT_BATCH][U];
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (c0 + WPT * 32 * u < vecs) g[u].load(dy + m * dy_stride, c0 + WPT * 32 * u);
                 if (dw) {
 #pragma unroll
                     for (int j = 0; j < UNSORT_BATCH; ++j)
-                        if (r[j] >= 0) v[j].load(rows + r[j] * rows_stride, c);
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+                            if (r[j] >= 0 && c0 + WPT * 32 * u < vecs) v[j][u].load(rows + r[j] * rows_stride, c0 + WPT * 32 * u);
                 }
 #pragma unroll
-                for (int j = 0; j < UNSORT_BATCH; ++j)
-                    if (r[j] >= 0) {
-                        if (dw) {
+                for (int u = 0; u < U; ++u) {
+                    const int c = c0 + WPT * 32 * u;
+                    if (c >= vecs) break;
 #pragma unroll
-                            for (int k = 0; k < R::N; ++k) dot[j] = fmaf(v[j].get(k), g.get(k), dot[j]);
-                        }
-                        if (drows) {
-                            R o;
+                    for (int j = 0; j < UNSORT_BATCH; ++j)
+                        if (r[j] >= 0) {
+                            if (dw) {
 #pragma unroll
-                            for (int k = 0; k < R::N; ++k) o.set(k, w[j] * g.get(k));
-                            o.store(drows + r[j] * drows_stride, c);
+                                for (int k = 0; k < R::N; ++k) dot[j] = fmaf(v[j][u].get(k), g[u].get(k), dot[j]);
+                            }
+                            if (drows) {
+                                R o;
+#pragma unroll
+                                for (int k = 0; k < R::N; ++k) o.set(k, w[j] * g[u].get(k));
+                                o.store(drows + r[j] * drows_stride, c);
+                            }
                         }
-                    }
+                }
             }
             if (dw) {
 #pragma unroll
@@ -367,7 +428,34 @@ static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_le
                                   (const int32_t*)scratch, offsets, row_of_pair, pair_of_row));
 }
 
-static unsigned blocks_of(long long threads) { return (unsigned)((threads + 255) / 256); }
+template <typename T_, int VB, typename O_>
+static int launch_unsort(const uint8_t* rows, long long rs, uint8_t* out, long long os, long long vecs, int M, int T, const int32_t* rp,
+                         const float* w, cudaStream_t st) {
+    auto go = [&](auto kernel, int U) { return cuda_status(launch_pdl(kernel, share_blocks(vecs, M, U), 256u, 0, st, rows, rs, out, os, vecs, M, T, rp, w)); };
+    if constexpr (VB == 16) {
+        const int batches = (T + 4) / 5;
+        switch ((T + batches - 1) / batches) {
+            case 1: return go(unsort_kernel<T_, VB, O_, 1, 1>, 1);
+            case 2: return go(unsort_kernel<T_, VB, O_, 2, 1>, 1);
+            case 3: return go(unsort_kernel<T_, VB, O_, 3, 1>, 1);
+            case 4: return go(unsort_kernel<T_, VB, O_, 4, 1>, 1);
+            default: return go(unsort_kernel<T_, VB, O_, 5, 1>, 1);
+        }
+    } else {
+        constexpr int U = share_of(VB, 1 << 20);
+        if (share_of(VB, vecs) > 1) return go(unsort_kernel<T_, VB, O_, 4, U>, U);
+        return go(unsort_kernel<T_, VB, O_, 4, 1>, 1);
+    }
+}
+
+template <typename V>
+static int launch_sort(const uint8_t* x, long long xs, uint8_t* rows, long long rs, long long vecs, int M, int T, const int32_t* rp,
+                       const int32_t* kept, int zero_tail, cudaStream_t st) {
+    constexpr int U = share_of(sizeof(V), 1 << 20);
+    auto go = [&](auto kernel, int u) { return cuda_status(launch_pdl(kernel, share_blocks(vecs, M, u), 256u, 0, st, x, xs, rows, rs, vecs, M, T, rp, kept, zero_tail)); };
+    if (share_of(sizeof(V), vecs) > 1) return go(sort_kernel<V, U>, U);
+    return go(sort_kernel<V, 1>, 1);
+}
 
 template <typename T_, int VB>
 static int launch_grad(const void* dy, long long dys, const void* rows, long long rs, void* drows, long long drs, float* dw, int K,
@@ -427,17 +515,14 @@ int vmoe_sort_tokens(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
     if (((uintptr_t)x | (uintptr_t)rows) & (el - 1)) return VMOE_ERR_ALIGN;
     const int vb = vector_bytes((uintptr_t)x | (uintptr_t)rows, xs | rs | K * el);
     const long long vecs = K * el / vb;
-    const unsigned grid = blocks_of((long long)M * vecs);
     const auto a = static_cast<const uint8_t*>(x);
     const auto o = static_cast<uint8_t*>(rows);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e;
     const int32_t* kept = expert_offsets + E;
-    if (vb == 16) e = launch_pdl(sort_kernel<uint4>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
-    else if (vb == 8) e = launch_pdl(sort_kernel<uint2>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
-    else if (vb == 4) e = launch_pdl(sort_kernel<uint32_t>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
-    else e = launch_pdl(sort_kernel<uint16_t>, grid, 256u, 0, st, a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail);
-    return cuda_status(e);
+    if (vb == 16) return launch_sort<uint4>(a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail, st);
+    if (vb == 8) return launch_sort<uint2>(a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail, st);
+    if (vb == 4) return launch_sort<uint32_t>(a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail, st);
+    return launch_sort<uint16_t>(a, xs, o, rs, vecs, M, T, row_of_pair, kept, zero_tail, st);
 }
 
 int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int32_t M, int32_t T, int32_t K,
@@ -462,14 +547,11 @@ int vmoe_unsort_tokens(const void* rows, int64_t rows_stride, int32_t dtype, int
         using R = decltype(r);
         using T_ = typename R::T;
         const long long vecs = (long long)K / R::N;
-        const unsigned grid = blocks_of((long long)M * vecs);
         if constexpr (sizeof(T_) == 4) {
-            if (out_dtype == VMOE_BF16)
-                return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, __nv_bfloat16>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
-            if (out_dtype == VMOE_F16)
-                return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, __half>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
+            if (out_dtype == VMOE_BF16) return launch_unsort<T_, R::BYTES, __nv_bfloat16>(a, rs, o, os, vecs, M, T, row_of_pair, weights, st);
+            if (out_dtype == VMOE_F16) return launch_unsort<T_, R::BYTES, __half>(a, rs, o, os, vecs, M, T, row_of_pair, weights, st);
         }
-        return cuda_status(launch_pdl(unsort_kernel<T_, R::BYTES, T_>, grid, 256u, 0, st, a, rs, o, os, vecs, M, T, row_of_pair, weights));
+        return launch_unsort<T_, R::BYTES, T_>(a, rs, o, os, vecs, M, T, row_of_pair, weights, st);
     });
 }
 
