@@ -47,10 +47,11 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
     }
     if (!on) return;
     const I8RowScale rs(top);
-    const int32_t* rp = SORTED ? row_of_pair + m * T : nullptr;
+    // a sorted row's place; outside the rows there are (a table not made by vmoe_plan_tokens): dropped
+    auto place = [&](int t) { const int r = row_of_pair[m * T + t]; return r < rows * T ? r : -1; };
     if (SORTED) {
         for (int t = part; t < T; t += STEP)
-            if (rp[t] >= 0) scales[rp[t]] = rs.scale;
+            if (place(t) >= 0) scales[place(t)] = rs.scale;
     } else if (part == 0) {
         scales[m] = rs.scale;
     }
@@ -65,8 +66,10 @@ i8_quantize_kernel(const uint8_t* x, long long x_stride, long long rows, int vec
         uint32_t w[2];
         rs.codes(v, w);
         if (SORTED) {
-            for (int t = 0; t < T; ++t)
-                if (rp[t] >= 0) store(rp[t], c, w);
+            for (int t = 0; t < T; ++t) {
+                const int r = place(t);
+                if (r >= 0) store(r, c, w);
+            }
         } else {
             store(m, c, w);
         }
@@ -113,7 +116,7 @@ i8_tile_kernel(const I8Problem p, int aligned_a, int aligned_w) {
     pdl_begin();
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int e = blockIdx.y, n0 = blockIdx.x * I8_TILE;
-    const int first = p.offsets ? p.offsets[e] : 0, end = p.offsets ? p.offsets[e + 1] : p.M;
+    const int first = p.offsets ? max(p.offsets[e], 0) : 0, end = p.offsets ? min(p.offsets[e + 1], p.M) : p.M;
     const int8_t* w = p.w + e * p.w_expert_stride;
     const float* wscale = p.w_scale + (long long)e * p.wrows;
     for (long long m0 = first + (long long)blockIdx.z * I8_TILE; m0 < end; m0 += (long long)gridDim.z * I8_TILE) {
@@ -161,7 +164,7 @@ i8_tile_kernel(const I8Problem p, int aligned_a, int aligned_w) {
     if (p.offsets && p.zero_tail) {
         const long long block = blockIdx.x + (long long)gridDim.x * (blockIdx.y + (long long)gridDim.y * blockIdx.z);
         const long long blocks = (long long)gridDim.x * gridDim.y * gridDim.z;
-        for (long long m = p.offsets[p.E] + block; m < p.M; m += blocks)
+        for (long long m = max(p.offsets[p.E], 0) + block; m < p.M; m += blocks)
             for (int n = tid; n < p.N; n += 256) i8_store(p.out, m * p.out_stride + n, p.out_dtype, 0.f);
     }
 }
@@ -220,7 +223,7 @@ static int i8_problem(I8Problem* p, const int8_t* a, long long a_stride, const f
                       int zero_tail, void* out, long long out_stride, int out_dtype) {
     if (M < 0 || N <= 0 || K < 0 || E <= 0 || out_dtype < VMOE_BF16 || out_dtype > VMOE_F32) return VMOE_ERR_SHAPE;
     if (a_stride < 0 || w_stride < 0 || w_expert_stride < 0 || out_stride < N || (!expert_offsets && E != 1)) return VMOE_ERR_SHAPE;
-    if (K > I8_MAX_K || E > 65535 || N > (1 << 30)) return VMOE_ERR_LIMIT;
+    if (K > I8_MAX_K || E > 65535 || N > (1 << 30) || M > 0x7fffffff - 1024) return VMOE_ERR_LIMIT;
     if (M == 0) return VMOE_OK;
     if (!w_scale || !out || (K > 0 && !w)) return VMOE_ERR_NULL;
     if ((uintptr_t)out & (out_dtype == VMOE_F32 ? 3 : 1)) return VMOE_ERR_ALIGN;

@@ -176,6 +176,12 @@ plan_kernel(const int32_t* ids, const int32_t* expert_map, int map_len, int P, i
     for (long long r = (long long)kept + rank * threads + tid; r < P; r += (long long)ctas * threads) pair_of_row[r] = -1;
 }
 
+// A pair's row, or -1: dropped, or (in a table that vmoe_plan_tokens did not make) outside the rows there are.
+__device__ __forceinline__ int pair_row(const int32_t* row_of_pair, long long pair, long long rows) {
+    const int r = row_of_pair[pair];
+    return r < rows ? r : -1;
+}
+
 // i = m * vecs + c
 __device__ __forceinline__ void row_and_vector(long long i, long long vecs, long long& m, long long& c) {
     if (i <= 0xffffffffLL && vecs <= 0xffffffffLL) {
@@ -192,7 +198,7 @@ __device__ __forceinline__ void row_and_vector(long long i, long long vecs, long
 template <typename V>
 __device__ __forceinline__ void zero_rows(uint8_t* rows, long long stride, long long first, long long end, long long vecs) {
     const long long warps = (long long)gridDim.x * (blockDim.x >> 5);
-    for (long long r = first + (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < end; r += warps) {
+    for (long long r = max(first, 0LL) + (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < end; r += warps) {
         V* row = reinterpret_cast<V*>(rows + r * stride);
         for (long long c = threadIdx.x & 31; c < vecs; c += 32) row[c] = V{};
     }
@@ -222,7 +228,7 @@ struct Share {
     __device__ __forceinline__ bool has(int u, long long vecs) const { return U == 1 || c + 32 * u < vecs; }
 };
 static unsigned share_blocks(long long vecs, int M, int U) {
-    const long long threads = U == 1 ? M * vecs : 32 * M * ((vecs + 32 * U - 1) / (32 * U));
+    const long long threads = U == 1 ? M * vecs : 32LL * M * ((vecs + 32 * U - 1) / (32 * U));
     return (unsigned)((threads + 255) / 256);
 }
 // Narrow vectors: as many as make 16 bytes, where a row has enough of them.
@@ -248,11 +254,11 @@ sort_kernel(const uint8_t* x, long long x_stride, uint8_t* rows, long long rows_
 #pragma unroll
     for (int u = 0; u < U; ++u)
         if (s.has(u, vecs)) v[u] = reinterpret_cast<const V*>(x + s.m * x_stride)[s.c + 32 * u];
-    const int32_t* rp = row_of_pair + s.m * T;
+    const long long pairs = (long long)M * T;
     for (int t0 = 0; t0 < T; t0 += SORT_BATCH) {
         int r[SORT_BATCH];
 #pragma unroll
-        for (int j = 0; j < SORT_BATCH; ++j) r[j] = t0 + j < T ? rp[t0 + j] : -1;
+        for (int j = 0; j < SORT_BATCH; ++j) r[j] = t0 + j < T ? pair_row(row_of_pair, s.m * T + t0 + j, pairs) : -1;
 #pragma unroll
         for (int j = 0; j < SORT_BATCH; ++j)
             if (r[j] >= 0) {
@@ -283,14 +289,14 @@ unsort_kernel(const uint8_t* rows, long long rows_stride, uint8_t* out, long lon
     for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int k = 0; k < R::N; ++k) acc[u][k] = 0.f;
-    const int32_t* rp = row_of_pair + s.m * T;
+    const long long pairs = (long long)M * T;
     for (int t0 = 0; t0 < T; t0 += BATCH) {
         R v[BATCH][U];
         int r[BATCH];
         float w[BATCH];
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
-            r[j] = t0 + j < T ? rp[t0 + j] : -1;
+            r[j] = t0 + j < T ? pair_row(row_of_pair, s.m * T + t0 + j, pairs) : -1;
             w[j] = r[j] >= 0 && weights ? weights[s.m * T + t0 + j] : 1.f;
             if (r[j] >= 0) {
 #pragma unroll
@@ -336,13 +342,13 @@ unsort_grad_kernel(const uint8_t* dy, long long dy_stride, const uint8_t* rows, 
     const long long m = (long long)blockIdx.x * (8 / WPT) + warp / WPT;
     const int part = (warp % WPT) * 32 + lane;
     if (m < M) {
-        const int32_t* rp = row_of_pair + m * T;
+        const long long pairs = (long long)M * T;
         for (int t0 = 0; t0 < T; t0 += UNSORT_BATCH) {
             int r[UNSORT_BATCH];
             float w[UNSORT_BATCH], dot[UNSORT_BATCH];
 #pragma unroll
             for (int j = 0; j < UNSORT_BATCH; ++j) {
-                r[j] = t0 + j < T ? rp[t0 + j] : -1;
+                r[j] = t0 + j < T ? pair_row(row_of_pair, m * T + t0 + j, pairs) : -1;
                 w[j] = r[j] >= 0 && weights ? weights[m * T + t0 + j] : 1.f;
                 dot[j] = 0.f;
             }

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import lib
-from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_TOPK, TokenPlan, check_out, check_rows, launch
+from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, launch
 
 MAX_K = 131071
 
@@ -37,6 +37,8 @@ class Int8Rows:
             raise ValueError("the codes of a row must lie next to each other")
         if q.shape[-1] > MAX_K:
             raise ValueError(f"rows of at most {MAX_K} codes")
+        if q.shape[-2] > MAX_ROWS:
+            raise ValueError(f"at most {MAX_ROWS} rows")
         self.q = q
         self.scale = scale
 

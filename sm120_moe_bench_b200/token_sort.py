@@ -11,10 +11,13 @@ experts, or not local under an ``expert_map``) take part in nothing: they have n
 weights get a zero gradient.  They leave ``M * T - kept`` rows behind the last kept one; these are zero in every tensor
 made here (rows and gradients) and left as they were in a tensor given as ``out``.
 
-A backward pass is captured into a CUDA graph together with its forward pass; eager graphs of the same leaf tensors have
-to be gone by then, as for any operator of torch (a leaf's accumulator stays bound to the stream of the graph that made it).
+A backward pass is captured into a CUDA graph together with its forward pass.  An eager graph of the same leaf tensor has
+to be gone by then (a leaf's accumulator stays bound to the stream of the graph that made it, which the capture must not
+wait for): with one of these operators' graphs still alive the captured call raises.
 """
 from __future__ import annotations
+
+import weakref
 
 import torch
 
@@ -22,6 +25,7 @@ from ._lib import check, lib
 
 DTYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 MAX_TOPK = 16
+MAX_ROWS = 2 ** 31 - 1025    # sizes travel as int32
 MAX_EXPERTS = 8192
 ONE_CTA_PAIRS = 4096      # up to here the plan needs no scratch (vmoe_plan_scratch_bytes is 0)
 
@@ -56,6 +60,8 @@ def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torc
         raise ValueError(f"{name} must have {rows} rows, got {t.shape[0]}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the plan on {device}")
+    if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_ROWS:
+        raise ValueError(f"{name} has a dimension of more than {MAX_ROWS}")
     if t.shape[1] > 1 and t.stride(1) != 1:
         raise ValueError(f"the elements of a row of {name} must lie next to each other")
     return t
@@ -137,6 +143,8 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
         raise ValueError(f"1 to {MAX_TOPK} choices per token, got {T}")
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
+    if M * T > MAX_ROWS:
+        raise ValueError(f"at most {MAX_ROWS} pairs, got {M * T}")
     dev = topk_ids.device
     if expert_map is not None:
         if expert_map.device != dev or expert_map.dtype != torch.int32 or expert_map.dim() != 1 or not expert_map.is_contiguous():
@@ -177,9 +185,21 @@ def _dense_rows(g: torch.Tensor) -> torch.Tensor:
     return g if g.shape[1] <= 1 or g.stride(1) == 1 else g.contiguous()
 
 
+def _note_graph(ctx, leaf: torch.Tensor) -> None:
+    """Leaves a mark of an eager graph on its leaf, and refuses to capture one while another's mark is alive."""
+    if not leaf.is_leaf:
+        return
+    if not torch.cuda.is_current_stream_capturing():
+        leaf._vmoe_graph = weakref.ref(ctx)
+    elif getattr(leaf, "_vmoe_graph", None) is not None and leaf._vmoe_graph() is not None:
+        raise RuntimeError("an eager graph of this leaf tensor is still alive (an output of it is held): drop it before capturing a graph "
+                           "that differentiates the leaf again")
+
+
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
+        _note_graph(ctx, x)
         ctx.plan = plan
         return _sort(x, plan)
 
@@ -209,6 +229,10 @@ _unsort_backward_once = torch.autograd.function.once_differentiable(_unsort_back
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, plan, weights):
+        if rows.requires_grad:
+            _note_graph(ctx, rows)
+        if weights is not None and weights.requires_grad:
+            _note_graph(ctx, weights)
         ctx.plan = plan
         ctx.save_for_backward(rows, weights)
         return _unsort(rows, plan, weights)

@@ -296,6 +296,55 @@ def test_side_stream_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(captured, eager))
 
 
+def test_backward_in_a_graph_beside_an_eager_graph():
+    import sm120_moe_bench_b200 as vm
+    plan = vm.plan_tokens(ids_of(16, 2, 4, 40), 4)
+    x, w = rows_of(16, 32, torch.float32, 41).requires_grad_(), torch.rand(16, 2, device="cuda").requires_grad_()
+    eager = vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w)
+    for leaf in (lambda: vm.sort_tokens(x, plan), lambda: vm.unsort_tokens(vm.sort_tokens(x.detach(), plan), plan, w)):
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                leaf()
+    eager.sum().backward()
+    want = x.grad.clone(), w.grad.clone()
+    del eager
+    x.grad = w.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w).sum().backward()
+    g.replay()
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+
+
+def test_a_table_of_wild_rows_is_harmless():
+    """Rows outside the tensor (a plan that plan_tokens did not make) drop their pair; nothing is read or written there."""
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 8, 2, 4, 64
+    good = vm.plan_tokens(ids_of(M, T, E, 42), E)
+    rp = good.row_of_pair.clone()
+    rp[2, 1], rp[5, 0], rp[6, 1] = M * T, 2 ** 31 - 1, -2 ** 31
+    offsets = good.expert_offsets.clone()
+    offsets[0], offsets[2], offsets[-1] = -7, 10 ** 6, 2 ** 31 - 1
+    wild = vm.TokenPlan(offsets, rp, good.pair_of_row, E)
+    x = rows_of(M, K, torch.float32, 43)
+    fence = torch.full((M * T + 2, K), 3.0, device="cuda")
+    vm.sort_tokens(x, wild, out=fence[1:-1])
+    assert bool((fence[0] == 3).all()) and bool((fence[-1] == 3).all())
+    rows = rows_of(M * T, K, torch.float32, 44)
+    kept = (rp >= 0) & (rp < M * T)
+    want = torch.where(kept[:, :, None], rows[rp.clamp(0, M * T - 1).long()], 0.0).sum(1)
+    assert torch.equal(vm.unsort_tokens(rows, wild), want)
+    r = rows.requires_grad_()
+    torch.autograd.grad(vm.unsort_tokens(r, wild), r, x)
+    q = vm.quantize_int8(x, wild)
+    w = vm.quantize_int8(torch.randn(E, 32, K, device="cuda"))
+    vm.int8_matmul(q, w, wild, out_dtype=torch.float32)
+    odd = vm.Int8Rows(w.q[..., 1:62].contiguous(), w.scale)
+    vm.int8_matmul(vm.Int8Rows(q.q[:, :61], q.scale), odd, wild, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    assert vm.int8_status() == 0
+
+
 def test_refusals():
     import sm120_moe_bench_b200 as vm
     ids = ids_of(8, 2, 4, 32)

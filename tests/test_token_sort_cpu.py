@@ -72,6 +72,10 @@ def test_host_tensors_are_refused():
     ids = torch.zeros(4, 2, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA tensor"):
         vm.plan_tokens(ids, 4)
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    for bad in ((z(4), z(4, 2), z(8), 4), (z(5), z(4, 2), z(7), 4), (z(5).long(), z(4, 2), z(8), 4), (z(5), z(2, 4).t(), z(8), 4)):
+        with pytest.raises(ValueError):
+            vm.TokenPlan(*bad)
     plan = vm.TokenPlan(torch.zeros(5, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), 4)
     assert (plan.tokens, plan.topk, plan.rows) == (4, 2, 8)
     with pytest.raises(ValueError, match="CUDA tensor"):
