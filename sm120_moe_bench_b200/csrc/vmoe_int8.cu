@@ -89,7 +89,7 @@ static int launch_quantize_rows(const void* x, long long xs, long long rows, int
                                 int8_t* q, long long q_stride, float* scales, cudaStream_t st) {
     const unsigned grid = (unsigned)((rows + 8 / WPR - 1) / (8 / WPR));
     const auto a = static_cast<const uint8_t*>(x);
-    return cuda_status(row_of_pair
+    return launch_status(row_of_pair
         ? launch_pdl(i8_quantize_kernel<T_, VB, WPR, true>, grid, 256u, 0, st, a, xs, rows, vecs, T, row_of_pair, live, q, q_stride, scales)
         : launch_pdl(i8_quantize_kernel<T_, VB, WPR, false>, grid, 256u, 0, st, a, xs, rows, vecs, T, row_of_pair, live, q, q_stride, scales));
 }
@@ -180,7 +180,7 @@ static int launch_i8_tile(const I8Problem& p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    return cuda_status(p.swiglu ? cudaLaunchKernelEx(&cfg, i8_tile_kernel<true>, p, (int)aa, (int)aw)
+    return launch_status(p.swiglu ? cudaLaunchKernelEx(&cfg, i8_tile_kernel<true>, p, (int)aa, (int)aw)
                                 : cudaLaunchKernelEx(&cfg, i8_tile_kernel<false>, p, (int)aa, (int)aw));
 }
 
@@ -267,8 +267,9 @@ static int i8_product_any(I8Problem p, void* room, size_t bytes, cudaStream_t st
         if (pack_w) { q.w = w; q.w_stride = i8_pitch(p.K); q.w_expert_stride = (long long)p.wrows * i8_pitch(p.K); }
         const long long vecs = (long long)(i8_pitch(p.K) / 16) * ((pack_a ? p.M : 0) + (pack_w ? (long long)p.E * p.wrows : 0));
         if ((vecs + 255) / 256 > 0x7fffffffLL) return VMOE_ERR_LIMIT;
-        if (launch_pdl(i8_pack_kernel, (unsigned)((vecs + 255) / 256), 256u, 0, st, p, (int)pack_a, a, pack_w ? w : (int8_t*)nullptr) != cudaSuccess)
-            return VMOE_ERR_CUDA;
+        const int rc = launch_status(launch_pdl(i8_pack_kernel, (unsigned)((vecs + 255) / 256), 256u, 0, st, p, (int)pack_a, a,
+                                                pack_w ? w : (int8_t*)nullptr));
+        if (rc) return rc;
         p = q;
     }
     return i8_product(p, st);

@@ -234,7 +234,7 @@ static int launch_gemv(const I8Problem& p, const void* x, long long x_stride, in
     // two CTAs an SM, every warp the same number of channels
     const long long warps = 2LL * tc_sm_count() * (I8G_THREADS / 32), rounds = (p.N + warps - 1) / warps;
     const unsigned grid = (unsigned)((p.N + rounds * (I8G_THREADS / 32) - 1) / (rounds * (I8G_THREADS / 32)));
-    return cuda_status(launch_pdl(i8_gemv_kernel<VB, ROWS, SWIGLU>, grid, (unsigned)I8G_THREADS, smem, st, p,
+    return launch_status(launch_pdl(i8_gemv_kernel<VB, ROWS, SWIGLU>, grid, (unsigned)I8G_THREADS, smem, st, p,
                                   static_cast<const uint8_t*>(x), x_stride, x_dtype, x_vec));
 }
 template <int VB, bool SWIGLU>

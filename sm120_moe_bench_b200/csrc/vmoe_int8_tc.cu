@@ -551,7 +551,7 @@ static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
     const unsigned grid = (unsigned)(items < tc_sm_count() ? items : tc_sm_count());
     static SmemAllowed done;
     if (allow_smem(i8_tc_kernel<SWIGLU, O_>, I8P_SMEM, done) != cudaSuccess) return VMOE_ERR_CUDA;
-    return cuda_status(launch_pdl(i8_tc_kernel<SWIGLU, O_>, grid, (unsigned)I8P_THREADS, smem, st, P));
+    return launch_status(launch_pdl(i8_tc_kernel<SWIGLU, O_>, grid, (unsigned)I8P_THREADS, smem, st, P));
 }
 int launch_i8_tc(const I8Problem& p, cudaStream_t st) {
     if (p.swiglu)
@@ -599,7 +599,7 @@ static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, i8_split_kernel<SWIGLU>, P));
+    return launch_status(cudaLaunchKernelEx(&cfg, i8_split_kernel<SWIGLU>, P));
 }
 int launch_i8_split(const I8Problem& p, cudaStream_t st) { return p.swiglu ? launch_i8_split_t<true>(p, st) : launch_i8_split_t<false>(p, st); }
 

@@ -63,6 +63,12 @@ inline int vector_bytes(uintptr_t addresses, long long lengths) {
     return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
 }
 
+// A launch's status.  A refused launch must not leave its error for the next call's cudaGetLastError.
+inline int launch_status(cudaError_t e) {
+    if (e != cudaSuccess) cudaGetLastError();
+    return cuda_status(e);
+}
+
 // More than 48 KB of dynamic shared memory have to be allowed once per device and kernel; `done` is the caller's, one for each.
 struct SmemAllowed { bool on[64] = {}; };
 template <typename F>
@@ -72,6 +78,7 @@ inline cudaError_t allow_smem(F* kernel, size_t bytes, SmemAllowed& done) {
     if (e != cudaSuccess || (dev < 64 && done.on[dev])) return e;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess && dev < 64) done.on[dev] = true;
+    if (e != cudaSuccess) cudaGetLastError();
     return e;
 }
 

@@ -423,21 +423,21 @@ static int launch_plan(const int32_t* ids, const int32_t* expert_map, int map_le
     if (ctas == 1) {
         static SmemAllowed one;
         if (allow_smem(plan_kernel<false>, PLAN_SMEM, one) != cudaSuccess) return VMOE_ERR_CUDA;
-        return cuda_status(launch_pdl(plan_kernel<false>, 1u, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
+        return launch_status(launch_pdl(plan_kernel<false>, 1u, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
                                       (const int32_t*)nullptr, offsets, row_of_pair, pair_of_row));
     }
     static SmemAllowed many;
     if (allow_smem(plan_kernel<true>, PLAN_SMEM, many) != cudaSuccess) return VMOE_ERR_CUDA;
     const cudaError_t e = launch_pdl(plan_count_kernel, (unsigned)ctas, 1024u, (size_t)4 * E, st, ids, expert_map, map_len, P, E, run * warps, scratch);
-    if (e != cudaSuccess) return VMOE_ERR_CUDA;
-    return cuda_status(launch_pdl(plan_kernel<true>, (unsigned)ctas, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
+    if (e != cudaSuccess) return launch_status(e);
+    return launch_status(launch_pdl(plan_kernel<true>, (unsigned)ctas, (unsigned)warps * 32, smem, st, ids, expert_map, map_len, P, E, run,
                                   (const int32_t*)scratch, offsets, row_of_pair, pair_of_row));
 }
 
 template <typename T_, int VB, typename O_>
 static int launch_unsort(const uint8_t* rows, long long rs, uint8_t* out, long long os, long long vecs, int M, int T, const int32_t* rp,
                          const float* w, cudaStream_t st) {
-    auto go = [&](auto kernel, int U) { return cuda_status(launch_pdl(kernel, share_blocks(vecs, M, U), 256u, 0, st, rows, rs, out, os, vecs, M, T, rp, w)); };
+    auto go = [&](auto kernel, int U) { return launch_status(launch_pdl(kernel, share_blocks(vecs, M, U), 256u, 0, st, rows, rs, out, os, vecs, M, T, rp, w)); };
     if constexpr (VB == 16) {
         const int batches = (T + 4) / 5;
         switch ((T + batches - 1) / batches) {
@@ -458,7 +458,7 @@ template <typename V>
 static int launch_sort(const uint8_t* x, long long xs, uint8_t* rows, long long rs, long long vecs, int M, int T, const int32_t* rp,
                        const int32_t* kept, int zero_tail, cudaStream_t st) {
     constexpr int U = share_of(sizeof(V), 1 << 20);
-    auto go = [&](auto kernel, int u) { return cuda_status(launch_pdl(kernel, share_blocks(vecs, M, u), 256u, 0, st, x, xs, rows, rs, vecs, M, T, rp, kept, zero_tail)); };
+    auto go = [&](auto kernel, int u) { return launch_status(launch_pdl(kernel, share_blocks(vecs, M, u), 256u, 0, st, x, xs, rows, rs, vecs, M, T, rp, kept, zero_tail)); };
     if (share_of(sizeof(V), vecs) > 1) return go(sort_kernel<V, U>, U);
     return go(sort_kernel<V, 1>, 1);
 }
@@ -470,10 +470,10 @@ static int launch_grad(const void* dy, long long dys, const void* rows, long lon
     const auto a = static_cast<const uint8_t*>(dy), b = static_cast<const uint8_t*>(rows);
     const auto o = static_cast<uint8_t*>(drows);
     if (vecs <= 64)
-        return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 1>, (unsigned)((M + 7) / 8), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+        return launch_status(launch_pdl(unsort_grad_kernel<T_, VB, 1>, (unsigned)((M + 7) / 8), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
     if (vecs <= 256)
-        return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 4>, (unsigned)((M + 1) / 2), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
-    return cuda_status(launch_pdl(unsort_grad_kernel<T_, VB, 8>, (unsigned)M, 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+        return launch_status(launch_pdl(unsort_grad_kernel<T_, VB, 4>, (unsigned)((M + 1) / 2), 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
+    return launch_status(launch_pdl(unsort_grad_kernel<T_, VB, 8>, (unsigned)M, 256u, 0, st, a, dys, b, rs, o, drs, dw, vecs, M, T, rp, w, kept));
 }
 
 static int check_rows(int32_t M, int32_t T, int32_t E, int32_t K, int32_t dtype) {
@@ -571,7 +571,7 @@ int vmoe_unsort_tokens_grad(const void* dout, int64_t dout_stride, const void* r
     if (K > 0 && (!dout || !expert_offsets || !row_of_pair || (dweights && !rows))) return VMOE_ERR_NULL;
     if (dout_stride < 0 || (dweights && rows_stride < 0) || (drows && drows_stride < K)) return VMOE_ERR_SHAPE;
     if (K == 0)
-        return dweights ? cuda_status(cudaMemsetAsync(dweights, 0, (size_t)M * T * sizeof(float), st)) : VMOE_OK;
+        return dweights ? launch_status(cudaMemsetAsync(dweights, 0, (size_t)M * T * sizeof(float), st)) : VMOE_OK;
     const long long el = dtype == VMOE_F32 ? 4 : 2, ds = dout_stride * el;
     const long long rs = dweights ? rows_stride * el : 0, gs = drows ? drows_stride * el : 0;
     const uintptr_t ptrs = (uintptr_t)dout | (dweights ? (uintptr_t)rows : 0) | (uintptr_t)drows;

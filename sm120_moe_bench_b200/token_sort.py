@@ -106,6 +106,11 @@ class TokenPlan:
         self._rows_ptr = self._offsets_ptr + 4 * (num_experts + 1)
         return self
 
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """As ``Tensor.record_stream``: for a plan that is used on another stream than the one it was made on."""
+        for t in (self._buf,) if self._buf is not None else (self._offsets, self._rows, self._pairs):
+            t.record_stream(stream)
+
     @property
     def expert_offsets(self) -> torch.Tensor:
         if self._offsets is None:

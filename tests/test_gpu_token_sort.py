@@ -274,6 +274,8 @@ def test_side_stream_and_graph():
         plan = vm.plan_tokens(ids, E)
         side = vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w)
     torch.cuda.current_stream().wait_stream(s)
+    plan.record_stream(torch.cuda.current_stream())
+    assert torch.equal(side, vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w))
     plan = vm.plan_tokens(ids, E)
     assert torch.equal(side, vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w))
     # forward and backward captured together, replayed on other inputs
