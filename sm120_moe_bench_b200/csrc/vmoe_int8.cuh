@@ -20,8 +20,19 @@ struct I8Problem {
 
 __device__ __forceinline__ float i8_scaled(int acc, float sa, float sw) { return (__int2float_rn(acc) * sa) * sw; }
 
-// Above 20 the denominator rounds to 1 (and an infinite gate must not meet the quotient's correction step).
-__device__ __forceinline__ float i8_silu(float x) { return x > 20.f ? x : silu(x); }
+// x / (1 + exp(-x)) without a branch: an IEEE reciprocal brings one for its rare cases, and with it the 16 elements that an
+// epilogue thread has in hand run one after another (8192 x 4096 x (4096 gate + 4096 up): 293 us with it, 193 without).  The
+// approximate reciprocal gets one Newton step and the quotient one correction, which leaves it within an ulp of
+// the rounded quotient.  Above 20 the denominator rounds to 1 (and an infinite x must not meet the correction); it is kept
+// below 1e38, where the reciprocal becomes 0 and with it the quotient of a finite x below about -87.
+__device__ __forceinline__ float i8_silu(float x) {
+    const float d = fminf(1.f + expf(-x), 1e38f);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    r = fmaf(fmaf(-d, r, 1.f), r, r);
+    const float q = x * r;
+    return x > 20.f ? x : fmaf(fmaf(-d, q, x), r, q);
+}
 
 __device__ __forceinline__ void i8_store(void* out, long long at, int dtype, float v) {
     if (dtype == VMOE_F32) static_cast<float*>(out)[at] = v;
