@@ -1,7 +1,7 @@
 // The 8-bit integer product on the tensor cores (tcgen05.mma kind::i8, s8 x s8 -> s32, accumulators in tensor memory).
 //
 // In both kernels the MMA's rows (operand A) are output channels and its columns (operand B) are tokens, so the number of
-// tokens of an item is free in steps of 16 or 32: an expert with 5 rows costs 32 columns, one with 320 costs 192 + 128, and a
+// tokens of an item is free in steps of 16 or 32: an expert with 5 rows costs 16 columns, one with 320 costs 2 x 160, and a
 // decode batch streams every weight once.  A thread of the epilogue owns a channel; 32 lanes store 32 neighbours of a row.
 //
 //   i8_tc_kernel      persistent, grouped or large: 256 weight rows x up to 256 tokens per item
@@ -17,11 +17,6 @@ namespace vmoe {
 // A wait that ran out leaves its status here (read and cleared by vmoe_int8_read_status).
 __device__ int g_i8_status;
 
-__device__ __forceinline__ uint32_t i8_cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ void i8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
