@@ -29,15 +29,17 @@ class Int8Rows:
     __slots__ = ("q", "scale")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
-        if not q.is_cuda or q.dtype != torch.int8 or q.dim() not in (2, 3):
+        shape = q.shape
+        if not q.is_cuda or q.dtype != torch.int8 or len(shape) not in (2, 3):
             raise ValueError("q must be an int8 CUDA tensor [rows, K] or [experts, rows, K]")
-        if scale.dtype != torch.float32 or scale.device != q.device or scale.shape != q.shape[:-1] or not scale.is_contiguous():
+        if scale.dtype != torch.float32 or scale.device != q.device or scale.shape != shape[:-1] or not scale.is_contiguous():
             raise ValueError("scale must be a contiguous float32 tensor, one value for each row of q, on its device")
-        if q.shape[-1] > 1 and q.stride(-1) != 1:
+        K = shape[-1]
+        if K > 1 and q.stride(-1) != 1:
             raise ValueError("the codes of a row must lie next to each other")
-        if q.shape[-1] > MAX_K:
+        if K > MAX_K:
             raise ValueError(f"rows of at most {MAX_K} codes")
-        if q.shape[-2] > MAX_ROWS:
+        if shape[-2] > MAX_ROWS:
             raise ValueError(f"at most {MAX_ROWS} rows")
         self.q = q
         self.scale = scale
@@ -112,15 +114,17 @@ def int8_status(device: torch.device | str | int = "cuda") -> int:
 
 
 def _out_columns(w: Int8Rows, K: int, device, swiglu: bool, experts: int | None) -> int:
-    if w.q.device != device:
-        raise ValueError(f"the weights are on {w.q.device}, the rows on {device}")
-    if w.q.dim() != (2 if experts is None else 3):
+    q = w.q
+    shape = q.shape
+    if q.device != device:
+        raise ValueError(f"the weights are on {q.device}, the rows on {device}")
+    if len(shape) != (2 if experts is None else 3):
         raise ValueError("weights of several experts go with a plan, a single matrix goes without")
-    if experts is not None and w.q.shape[0] != experts:
-        raise ValueError(f"the plan has {experts} experts, the weights {w.q.shape[0]}")
-    if w.q.shape[-1] != K:
-        raise ValueError(f"rows of {K} codes times weights of {w.q.shape[-1]}")
-    n = w.q.shape[-2]
+    if experts is not None and shape[0] != experts:
+        raise ValueError(f"the plan has {experts} experts, the weights {shape[0]}")
+    if shape[-1] != K:
+        raise ValueError(f"rows of {K} codes times weights of {shape[-1]}")
+    n = shape[-2]
     if swiglu and n % 2:
         raise ValueError("swiglu needs gate and up rows")
     if n == 0:
@@ -165,9 +169,11 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
     _no_grad(x, "x")
     check_rows(x, "x")
     N = _out_columns(w, x.shape[1], x.device, swiglu, None)
+    stride = N
     if out is None:
-        out = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
+        out = x.new_empty((x.shape[0], N))
     else:
+        stride = max(out.stride(0), N)
         check_rows(out, "out", x.shape[0], x.device)
         if out.dtype != x.dtype or out.shape[1] != N or (x.shape[0] > 1 and out.stride(0) < N):
             raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
@@ -181,7 +187,7 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
             need += lib.vmoe_int8_pack_bytes(M, wq.shape[0], K, 1)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     launch(x.device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, wq.data_ptr(),
-           wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), max(out.stride(0), N), DTYPE_CODES[out.dtype],
+           wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), stride, DTYPE_CODES[out.dtype],
            scratch.data_ptr() if need else None, need)
     return out
 
@@ -217,7 +223,7 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
         raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids, not empty")
     q13, q2 = w13.q, w2.q
     pack = not (_aligned(q13) and _aligned(q2)) and _packs(w13, M * T)
-    out = torch.empty((M, K), dtype=x.dtype, device=x.device)
+    out = x.new_empty((M, K))
     need = lib.vmoe_int8_experts_scratch_bytes(M, T, E, K, N, pack)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
     launch(x.device, "vmoe_int8_experts", lib.vmoe_int8_experts, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, T, E, K, N,

@@ -50,6 +50,11 @@ def launch(device: torch.device, name: str, fn, *args) -> None:
 
 def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torch.device | None = None) -> torch.Tensor:
     """``t`` as a matrix of rows the kernels can read: 2-D, on the device, elements of a row next to each other."""
+    if t.is_cuda and t.dtype in DTYPE_CODES and t.dim() == 2:
+        n, k = t.shape
+        if (rows is None or n == rows) and (device is None or t.device == device) and (k <= 1 or t.stride(1) == 1) \
+                and n <= MAX_ROWS and k <= MAX_ROWS:
+            return t
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dtype not in DTYPE_CODES:
@@ -59,12 +64,10 @@ def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torc
     if rows is not None and t.shape[0] != rows:
         raise ValueError(f"{name} must have {rows} rows, got {t.shape[0]}")
     if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the plan on {device}")
+        raise ValueError(f"{name} is on {t.device}, expected on {device}")
     if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_ROWS:
         raise ValueError(f"{name} has a dimension of more than {MAX_ROWS}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"the elements of a row of {name} must lie next to each other")
-    return t
+    raise ValueError(f"the elements of a row of {name} must lie next to each other")
 
 
 def check_out(out: torch.Tensor, rows: int, like: torch.Tensor) -> torch.Tensor:
@@ -158,7 +161,7 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
             raise ValueError("expert_map is empty")
     P = M * T
     need = 0 if P <= ONE_CTA_PAIRS else lib.vmoe_plan_scratch_bytes(M, T, num_experts)
-    buf = torch.empty(num_experts + 1 + 2 * P + need // 4, dtype=torch.int32, device=dev)
+    buf = topk_ids.new_empty(num_experts + 1 + 2 * P + need // 4)
     plan = TokenPlan._over(buf, M, T, num_experts)
     rows = plan._rows_ptr
     launch(dev, "vmoe_plan_tokens", lib.vmoe_plan_tokens, topk_ids.data_ptr(), None if expert_map is None else expert_map.data_ptr(),
@@ -169,19 +172,19 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
 
 def _sort(x, plan: TokenPlan, out=None):
     K = x.shape[1]
-    rows = x.new_empty((plan.rows, K)) if out is None else out
+    rows, stride = (x.new_empty((plan.rows, K)), K) if out is None else (out, max(out.stride(0), K))
     launch(x.device, "vmoe_sort_tokens", lib.vmoe_sort_tokens, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], plan.tokens, plan.topk,
            plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr, out is None, rows.data_ptr(),
-           max(rows.stride(0), K))
+           stride)
     return rows
 
 
 def _unsort(rows, plan: TokenPlan, weights=None, out=None):
     K = rows.shape[1]
-    y = rows.new_empty((plan.tokens, K)) if out is None else out
+    y, stride = (rows.new_empty((plan.tokens, K)), K) if out is None else (out, max(out.stride(0), K))
     launch(rows.device, "vmoe_unsort_tokens", lib.vmoe_unsort_tokens, rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype],
            plan.tokens, plan.topk, K, plan._rows_ptr, None if weights is None else weights.data_ptr(), y.data_ptr(),
-           max(y.stride(0), K), DTYPE_CODES[y.dtype])
+           stride, DTYPE_CODES[y.dtype])
     return y
 
 
