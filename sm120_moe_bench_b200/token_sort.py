@@ -17,6 +17,7 @@ wait for): with one of these operators' graphs still alive the captured call rai
 """
 from __future__ import annotations
 
+import threading
 import weakref
 
 import torch
@@ -109,6 +110,9 @@ class TokenPlan:
         self._rows_ptr = self._offsets_ptr + 4 * (num_experts + 1)
         return self
 
+    def __reduce__(self):              # copies and pickles carry the tables, never the addresses
+        return TokenPlan, (self.expert_offsets, self.row_of_pair, self.pair_of_row, self.num_experts)
+
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """As ``Tensor.record_stream``: for a plan that is used on another stream than the one it was made on."""
         for t in (self._buf,) if self._buf is not None else (self._offsets, self._rows, self._pairs):
@@ -193,13 +197,23 @@ def _dense_rows(g: torch.Tensor) -> torch.Tensor:
     return g if g.shape[1] <= 1 or g.stride(1) == 1 else g.contiguous()
 
 
-def _note_graph(ctx, leaf: torch.Tensor) -> None:
-    """Leaves a mark of an eager graph on its leaf, and refuses to capture one while another's mark is alive."""
-    if not leaf.is_leaf:
+_eager_graphs = weakref.WeakSet()      # nodes of live eager graphs; each knows its leaves (weakly)
+_eager_lock = threading.Lock()
+
+
+def _note_graph(ctx, *tensors: torch.Tensor | None) -> None:
+    """Remembers an eager graph while it lives, and refuses to capture one of a leaf that has another alive."""
+    leaves = [weakref.ref(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves:
         return
     if not torch.cuda.is_current_stream_capturing():
-        leaf._vmoe_graph = weakref.ref(ctx)
-    elif getattr(leaf, "_vmoe_graph", None) is not None and leaf._vmoe_graph() is not None:
+        ctx.leaves = leaves
+        with _eager_lock:
+            _eager_graphs.add(ctx)
+        return
+    with _eager_lock:
+        others = [r() for g in _eager_graphs for r in g.leaves]
+    if any(o is not None and o is r() for o in others for r in leaves):
         raise RuntimeError("an eager graph of this leaf tensor is still alive (an output of it is held): drop it before capturing a graph "
                            "that differentiates the leaf again")
 
@@ -237,10 +251,7 @@ _unsort_backward_once = torch.autograd.function.once_differentiable(_unsort_back
 class _UnsortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, plan, weights):
-        if rows.requires_grad:
-            _note_graph(ctx, rows)
-        if weights is not None and weights.requires_grad:
-            _note_graph(ctx, weights)
+        _note_graph(ctx, rows, weights)
         ctx.plan = plan
         ctx.save_for_backward(rows, weights)
         return _unsort(rows, plan, weights)

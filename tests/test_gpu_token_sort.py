@@ -3,7 +3,9 @@
 Tolerances: copies are bit-equal.  A sum of T products in f32 is off by at most (T + 1) * 2^-24 * sum |w| |r| before it is
 rounded to the output type, which adds half a step (eps / 2 of the value; 2^-25 absolute among fp16's subnormals).  A dot
 product over K elements in f32, in any order, is off by at most (K + 1) * 2^-24 * sum |r| |dy|."""
+import copy
 import os
+import pickle
 
 import pytest
 import torch
@@ -246,6 +248,19 @@ def test_non_finite_values_stay_in_their_tokens():
     assert torch.equal(y[keep], clean[keep])
 
 
+def test_a_copied_plan_outlives_the_original():
+    import sm120_moe_bench_b200 as vm
+    ids, x = ids_of(30, 3, 7, 46), rows_of(30, 40, torch.float32, 47)
+    plan = vm.plan_tokens(ids, 7)
+    want = vm.sort_tokens(x, plan)
+    twin = copy.deepcopy(plan)
+    check_plan(twin, ids, 7)
+    assert twin._offsets_ptr == twin.expert_offsets.data_ptr() != plan._offsets_ptr
+    del plan
+    torch.full((4096,), -3, dtype=torch.int32, device="cuda")
+    assert torch.equal(vm.sort_tokens(x, twin), want)
+
+
 def test_more_than_four_gigabytes_of_rows():
     import sm120_moe_bench_b200 as vm
     M, T, E, K = 40000, 16, 32, 4096
@@ -309,6 +324,9 @@ def test_backward_in_a_graph_beside_an_eager_graph():
                 leaf()
     eager.sum().backward()
     want = x.grad.clone(), w.grad.clone()
+    other = rows_of(16, 32, torch.float32, 45).requires_grad_()            # another leaf's graph is no hindrance
+    held = vm.sort_tokens(other, plan)
+    assert copy.deepcopy(x).equal(x)
     del eager
     x.grad = w.grad = None
     g = torch.cuda.CUDAGraph()
@@ -316,6 +334,10 @@ def test_backward_in_a_graph_beside_an_eager_graph():
         vm.unsort_tokens(vm.sort_tokens(x, plan), plan, w).sum().backward()
     g.replay()
     assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+    held.sum().backward()
+    p = torch.nn.Parameter(x.detach())
+    graph = vm.sort_tokens(p, plan)                       # a parameter with a live graph is saved like any other
+    assert torch.equal(pickle.loads(pickle.dumps(p)), p) and graph.requires_grad
 
 
 def test_a_table_of_wild_rows_is_harmless():

@@ -1,6 +1,8 @@
 """Token sort without a GPU: argument checks of the C entry points and of the torch functions, none of which reach a device."""
+import copy
 import ctypes
 import os
+import pickle
 
 import pytest
 import torch
@@ -78,6 +80,9 @@ def test_host_tensors_are_refused():
             vm.TokenPlan(*bad)
     plan = vm.TokenPlan(torch.zeros(5, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), 4)
     assert (plan.tokens, plan.topk, plan.rows) == (4, 2, 8)
+    for twin in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        assert twin.expert_offsets.data_ptr() != plan.expert_offsets.data_ptr()
+        assert twin._offsets_ptr == twin.expert_offsets.data_ptr() and twin._rows_ptr == twin.row_of_pair.data_ptr()
     with pytest.raises(ValueError, match="CUDA tensor"):
         vm.sort_tokens(torch.zeros(4, 8), plan)
     with pytest.raises(ValueError, match="CUDA tensor"):
