@@ -383,7 +383,7 @@ int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
 
 /* The expert layer on 8-bit weights: plan, quantise into expert order, w13 with silu(gate) * up, quantise, w2, weighted
  * sum.  Rows between the products are f32.  w13 [E, 2 N, K] (gate rows first), w2 [E, K, N]; topk_ids, topk_weights [M, T];
- * expert_map as in vmoe_plan_tokens.  Six or seven launches; scratch 16-byte aligned, of
+ * expert_map as in vmoe_plan_tokens.  Five launches up to 1024 pairs, six or seven above; scratch 16-byte aligned, of
  * vmoe_int8_experts_scratch_bytes (0: sizes beyond the limits of vmoe_plan_tokens), with room to pack weights of any
  * alignment when pack != 0. */
 size_t vmoe_int8_experts_scratch_bytes(int32_t M, int32_t T, int32_t E, int32_t K, int32_t N, int32_t pack);

@@ -359,6 +359,36 @@ def test_expert_layer_without_kept_pairs_or_tokens():
     assert torch.equal(vm.int8_experts(x, w13, w2, twice, half), once)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,T,E,K,N,map_len", [(1, 1, 1, 1, 1, 0), (3, 16, 8192, 20, 8, 0), (64, 16, 300, 40, 24, 0), (1024, 1, 5, 33, 16, 0),
+                                               (1025, 1, 5, 33, 16, 0), (93, 11, 40, 130, 16, 70), (94, 11, 40, 130, 16, 70),
+                                               (7, 3, 257, 9000, 16, 0), (512, 2, 256, 64, 32, 300)])
+def test_expert_layer_of_any_ids_equals_its_parts(M, T, E, K, N, map_len, dtype):
+    """Ids that repeat within a token, lie outside the experts or the map; empty and all-zero rows; both sides of 1024 pairs,
+    where the rows are planned another way; rows apart."""
+    import sm120_moe_bench_b200 as vm
+    x = torch.randn(M, K + 3, generator=gen(60), device="cuda").to(dtype)[:, :K]
+    x[M // 2] = 0
+    ids = torch.randint(-2, (map_len or E) + 2, (M, T), generator=gen(61), device="cuda", dtype=torch.int32)
+    if T > 1:
+        ids[:, 1] = ids[:, 0]
+    emap = None
+    if map_len:
+        emap = torch.randint(-1, E + 1, (map_len,), generator=gen(62), device="cuda", dtype=torch.int32)
+    weights = torch.randn(M, T, generator=gen(63), device="cuda")
+    w13, w2 = random_rows(vm, (E, 2 * N, K), 64), random_rows(vm, (E, K, N), 66)
+    y = vm.int8_experts(x, w13, w2, ids, weights, emap)
+    plan = vm.plan_tokens(ids, E, emap)
+    h = vm.int8_matmul(vm.quantize_int8(x, plan), w13, plan, swiglu=True, out_dtype=torch.float32)
+    rows = vm.int8_matmul(vm.quantize_int8(h), w2, plan, out_dtype=torch.float32)
+    kept = (plan.row_of_pair >= 0).any(1)
+    assert torch.equal(y, vm.unsort_tokens(rows, plan, weights).to(dtype)) and torch.count_nonzero(y[~kept]) == 0
+    assert bool(y.isfinite().all()) or dtype == torch.float16
+    x[0, 0] = float("nan")
+    bad = vm.int8_experts(x, w13, w2, ids, weights, emap)
+    assert torch.equal(bad[1:], y[1:]) and bool(bad[0].isnan().all()) == bool(kept[0])
+
+
 def test_side_stream_and_graph():
     import sm120_moe_bench_b200 as vm
     M, T, E, K, N = 24, 3, 8, 512, 256
