@@ -319,7 +319,9 @@ int vmoe_permute_noalloc(const int32_t* topk_ids, const float* topk_weights,
  * Kept pairs are those whose id (through expert_map [map_len] when given) lies in [0, E); all others, ids outside the
  * map included, are dropped.  Rows are ordered by (expert, pair); a token may name an expert more than once.  The
  * tables are what build_group_tables (fused-moe/csrc/verdict_fused_grouped.cu:655-691) makes for FP4 rows.
- * Limits: T <= 16, E <= 8192, M * T < 2^31 - 1024 (VMOE_ERR_LIMIT).  Strides are in elements. */
+ * Limits: T <= 16, E <= 8192, M * T < 2^31 - 1024 (VMOE_ERR_LIMIT).  Strides are in elements.
+ * Here and in the 8-bit products below outputs and scratch must not share memory with an operand or with each other:
+ * blocks read and write in no order, and the entry points do not check it. */
 enum vmoe_dtype { VMOE_BF16 = 0, VMOE_F16 = 1, VMOE_F32 = 2 };
 
 size_t vmoe_plan_scratch_bytes(int32_t M, int32_t T, int32_t E);      /* 0 up to 4096 pairs */

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import lib
-from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, launch
+from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, launch, refuse_overlap
 
 MAX_K = 131071
 
@@ -137,7 +137,7 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
     """``out[m, n] = (a.q[m] . w.q[n]) * a.scale[m] * w.scale[n]``.
 
     With ``plan`` the rows are sorted by expert (``quantize_int8(x, plan)``) and each meets its expert's matrix of ``w``
-    ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``).  ``swiglu``: ``w``
+    ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``, which must not share memory with an operand).  ``swiglu``: ``w``
     holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``, ``[M, N]``."""
     if a.q.dim() != 2:
         raise ValueError("a must be rows [M, K]")
@@ -153,6 +153,7 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
         if out.device != a.q.device or out.shape[1] != N:
             raise ValueError(f"out must have {N} columns on {a.q.device}")
         _no_grad(out, "out")
+        refuse_overlap(out, plan, **{"a": a.q, "a's scales": a.scale, "w": w.q, "w's scales": w.scale})
     M, K = a.q.shape
     aq, wq = a.q, w.q
     E = 1 if plan is None else plan.num_experts
@@ -165,7 +166,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
 
 
 def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``x [M, K]`` (bf16 / fp16 / f32) quantised row by row, times ``w [N, K]``: ``[M, N]`` in the type of ``x``."""
+    """``x [M, K]`` (bf16 / fp16 / f32) quantised row by row, times ``w [N, K]``: ``[M, N]`` in the type of ``x``.
+    ``out`` must not share memory with ``x`` or ``w``."""
     _no_grad(x, "x")
     check_rows(x, "x")
     N = _out_columns(w, x.shape[1], x.device, swiglu, None)
@@ -178,6 +180,7 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
         if out.dtype != x.dtype or out.shape[1] != N or (x.shape[0] > 1 and out.stride(0) < N):
             raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
         _no_grad(out, "out")
+        refuse_overlap(out, x=x, **{"w": w.q, "w's scales": w.scale})
     M, K = x.shape
     wq = w.q
     need = 0

@@ -9,7 +9,7 @@ Rows are bf16, fp16 or f32 with any row stride (elements of a row next to each o
 choices in order and are rounded once; nothing depends on the order in which blocks run.  Dropped pairs (ids outside the
 experts, or not local under an ``expert_map``) take part in nothing: they have no row, add nothing to a sum, and their
 weights get a zero gradient.  They leave ``M * T - kept`` rows behind the last kept one; these are zero in every tensor
-made here (rows and gradients) and left as they were in a tensor given as ``out``.
+made here (rows and gradients) and left as they were in a tensor given as ``out``, which must not share memory with an operand.
 
 A backward pass is captured into a CUDA graph together with its forward pass.  An eager graph of the same leaf tensor has
 to be gone by then (a leaf's accumulator stays bound to the stream of the graph that made it, which the capture must not
@@ -69,6 +69,37 @@ def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torc
     if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_ROWS:
         raise ValueError(f"{name} has a dimension of more than {MAX_ROWS}")
     raise ValueError(f"the elements of a row of {name} must lie next to each other")
+
+
+def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the two share memory; columns of one buffer that lie side by side do not.  Where row pitches differ and the
+    byte ranges meet, yes."""
+    def span(t):
+        return t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    x, y = a.data_ptr(), b.data_ptr()
+    if x + span(a) <= y or y + span(b) <= x:
+        return False
+    if a.dim() == b.dim() == 2:
+        pitch = a.stride(0) * a.element_size()
+        if pitch > 0 and pitch == b.stride(0) * b.element_size():
+            wa, wb = (span(t[:1]) for t in (a, b))
+            at = (y - x) % pitch
+            return at < wa or at + wb > pitch
+    return True
+
+
+def refuse_overlap(out: torch.Tensor, plan: "TokenPlan | None" = None, **operands: torch.Tensor | None) -> None:
+    """The kernels read their operands and write ``out`` in no order."""
+    if plan is not None:
+        operands["the plan"] = plan._buf if plan._buf is not None else plan.row_of_pair
+        if plan._buf is None:
+            operands["the plan's offsets"] = plan.expert_offsets
+    for name, t in operands.items():
+        if t is not None and overlap(out, t):
+            raise ValueError(f"out shares memory with {name}")
 
 
 def check_out(out: torch.Tensor, rows: int, like: torch.Tensor) -> torch.Tensor:
@@ -269,7 +300,8 @@ def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = Non
     if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
-        return _sort(x, plan, check_out(out, plan.rows, x))
+        refuse_overlap(check_out(out, plan.rows, x), plan, x=x)
+        return _sort(x, plan, out)
     if x.requires_grad and torch.is_grad_enabled():
         return _SortTokens.apply(x, plan)
     return _sort(x, plan)
@@ -288,7 +320,8 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | N
     if out is not None:
         if grad or (torch.is_grad_enabled() and out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
-        return _unsort(rows, plan, weights, check_out(out, plan.tokens, rows))
+        refuse_overlap(check_out(out, plan.tokens, rows), plan, rows=rows, weights=weights)
+        return _unsort(rows, plan, weights, out)
     if grad:
         return _UnsortTokens.apply(rows, plan, weights)
     return _unsort(rows, plan, weights)

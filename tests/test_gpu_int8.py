@@ -459,3 +459,24 @@ def test_refusals():
             call()
     with torch.no_grad():
         vm.int8_experts(x.clone().requires_grad_(), w13, w2, ids, wt)
+
+
+@pytest.mark.parametrize("M", [1, 4, 9, 300])
+def test_out_over_an_operand_is_refused(M):
+    """Up to a few rows every block quantises them all for itself, while others already write out: x could be read overwritten."""
+    import sm120_moe_bench_b200 as vm
+    x, w = torch.randn(M, 64, generator=gen(90), device="cuda"), random_rows(vm, (64, 64), 91)
+    with pytest.raises(ValueError, match="shares memory with x"):
+        vm.int8_linear(x, w, out=x)
+    a = random_rows(vm, (M, 64), 93)
+    for out, name in ((a.q.view(torch.float32), "a"), (a.scale[:, None], "a's scales"), (w.scale[None], "w's scales"),
+                      (w.q.view(torch.float32)[:1], "w")):
+        n = out.shape[1]
+        if out.shape[0] != M:
+            continue
+        with pytest.raises(ValueError, match=f"shares memory with {name}"):
+            vm.int8_matmul(a, vm.Int8Rows(w.q[:n], w.scale[:n]), out=out)
+    wide = torch.zeros(M, 128, device="cuda")
+    wide[:, :64] = x
+    vm.int8_linear(wide[:, :64], w, out=wide[:, 64:])     # columns side by side
+    assert torch.equal(wide[:, :64], x) and torch.equal(wide[:, 64:], vm.int8_linear(x, w))

@@ -402,3 +402,35 @@ def test_refusals():
         vm.unsort_tokens(rows[:15], plan, w)
     # the operator still answers afterwards
     assert torch.equal(vm.unsort_tokens(vm.sort_tokens(x, plan), plan), 2 * x)
+
+
+def test_out_over_an_operand_is_refused():
+    """Blocks read the operands and write out in no order: x under out would be sorted from rows that are overwritten already."""
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 8, 2, 4, 16
+    plan = vm.plan_tokens(ids_of(M, T, E, 50), E)
+    copied = copy.deepcopy(plan)
+    buf = rows_of(M * T, K, torch.float32, 51)
+    for out in (buf, buf.as_strided((M * T, K), (K, 1), 0)):
+        for p in (plan, copied):
+            with pytest.raises(ValueError, match="shares memory with x"):
+                vm.sort_tokens(buf[M:], p, out=out)
+    for out in (buf[:M], buf[4:4 + M]):
+        with pytest.raises(ValueError, match="shares memory with rows"):
+            vm.unsort_tokens(buf, plan, out=out)
+    one = vm.plan_tokens(ids_of(M, 1, E, 52), E)          # not even where every row stays a row
+    x = rows_of(M, K, torch.float32, 53)
+    with pytest.raises(ValueError, match="shares memory"):
+        vm.sort_tokens(x, one, out=x)
+    w = torch.ones(M, T, device="cuda")
+    with pytest.raises(ValueError, match="shares memory with weights"):
+        vm.unsort_tokens(rows_of(M * T, T, torch.float32, 54), plan, w, out=w)
+    for p in (plan, copied):
+        table = p.row_of_pair.view(torch.float32)
+        with pytest.raises(ValueError, match="the plan"):
+            vm.unsort_tokens(rows_of(M * T, T, torch.float32, 54), p, out=table)
+    # columns of one buffer side by side are two tensors
+    wide = rows_of(M * T, 2 * K, torch.float32, 55)
+    want = vm.unsort_tokens(wide[:, :K].contiguous(), plan, w)
+    vm.unsort_tokens(wide[:, :K], plan, w, out=wide[:M, K:])
+    assert torch.equal(wide[:M, K:], want)

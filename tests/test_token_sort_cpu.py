@@ -87,3 +87,38 @@ def test_host_tensors_are_refused():
         vm.sort_tokens(torch.zeros(4, 8), plan)
     with pytest.raises(ValueError, match="CUDA tensor"):
         vm.unsort_tokens(torch.zeros(8, 8), plan)
+
+
+def test_shared_memory_is_found():
+    from sm120_moe_bench_b200.token_sort import overlap
+
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    g = torch.Generator().manual_seed(1)
+
+    def view():
+        dtype = (torch.int8, torch.bfloat16, torch.float32)[int(torch.randint(3, (1,), generator=g))]
+        flat = buf.view(dtype)
+        rows, cols, pitch, at = (int(torch.randint(n, (1,), generator=g)) for n in (5, 7, 14, 60))
+        return flat.as_strided((rows, cols), (pitch, 1), at)
+
+    def touched(t):
+        size = t.element_size()
+        first = [t.storage_offset() + r * t.stride(0) + c for r in range(t.shape[0]) for c in range(t.shape[1])]
+        return {size * e + b for e in first for b in range(size)}
+
+    met = apart = 0
+    for _ in range(3000):
+        a, b = view(), view()
+        if touched(a) & touched(b):
+            met += 1
+            assert overlap(a, b) and overlap(b, a)
+        elif not overlap(a, b):
+            apart += 1
+            assert not overlap(b, a)
+    assert met > 300 and apart > 300
+    # side by side in one buffer, below one another, and columns that meet
+    wide = torch.zeros(9, 20)
+    assert not overlap(wide[:, :8], wide[:, 8:]) and not overlap(wide[:5, 8:], wide[:, :8]) and not overlap(wide[:4], wide[4:])
+    assert not overlap(wide[:, :0], wide) and not overlap(wide[3:4, :8], wide[:, 8:12])
+    assert overlap(wide[:, :8], wide[:, 7:]) and overlap(wide[:5], wide[4:]) and overlap(wide, wide[8, 19:])
+    assert overlap(torch.zeros(1, 4).expand(5, 4), wide) is False
