@@ -14,8 +14,9 @@ namespace vmoe {
 constexpr int I8G_THREADS = 256;
 constexpr int I8G_SMEM = 64 * 1024;                       // codes of all rows
 
-// VB = 16: the weights' rows start on 16-byte boundaries.  VB = 4: anywhere; a word is joined from the two aligned ones that
-// hold it, the second of which is read only where the row reaches into it.
+// VB = 16: the weights' rows start on 16-byte boundaries; the bytes behind a row's last whole vector go to a lane each, so that
+// nothing behind the row is read.  VB = 4: anywhere; a word is joined from the two aligned ones that hold it, the second of
+// which is read only where the row reaches into it.
 template <int VB> struct I8Word;
 template <> struct I8Word<16> { using type = uint4; };
 template <> struct I8Word<4>  { using type = uint32_t; };
@@ -141,7 +142,7 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
     pdl_begin();
     const int lane = threadIdx.x & 31, stride = gridDim.x * (I8G_THREADS / 32);
     int n = blockIdx.x * (I8G_THREADS / 32) + (threadIdx.x >> 5);
-    const int K = p.K, pitch = (K + 15) & ~15, words = (K + VB - 1) / VB;
+    const int K = p.K, pitch = (K + 15) & ~15, words = VB == 16 ? K / 16 : (K + 3) / 4, over = VB == 16 ? K & 15 : 0;
     const W* w[SETS];
     int shift[SETS];
     float scale[SETS] = {};                               // of the channel whose vectors come next: requested with them
@@ -180,7 +181,7 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
         float sw[SETS];
 #pragma unroll
         for (int s = 0; s < SETS; ++s) sw[s] = scale[s];
-        for (int c0 = 0; c0 < words; c0 += 32 * AHEAD) {
+        for (int c0 = 0; c0 == 0 || c0 < words; c0 += 32 * AHEAD) {       // once at least: it brings the next channel
             const bool last = c0 + 32 * AHEAD >= words;
             const int next = last ? 0 : c0 + 32 * AHEAD;
             const bool more = !last || n + stride < p.N;
@@ -189,7 +190,7 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
             for (int i = 0; i < AHEAD; ++i) {
                 const int c = c0 + lane + 32 * i;
                 if (c < words) {
-                    // bytes behind K meet zero codes
+                    // (of a row's last word) bytes behind K meet zero codes
 #pragma unroll
                     for (int m = 0; m < ROWS; ++m) {
                         if (m >= p.M) break;
@@ -203,6 +204,18 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
 #pragma unroll
                     for (int s = 0; s < SETS; ++s) have[s][i] = i8_weights(w[s], cn, shift[s], K);
                 }
+            }
+        }
+        if (lane < over) {
+            int tail[SETS];
+#pragma unroll
+            for (int s = 0; s < SETS; ++s) tail[s] = p.w[(long long)(s * p.N + n) * p.w_stride + K - over + lane];
+#pragma unroll
+            for (int m = 0; m < ROWS; ++m) {
+                if (m >= p.M) break;
+                const int a = static_cast<int8_t>(codes[(size_t)m * pitch + K - over + lane]);
+#pragma unroll
+                for (int s = 0; s < SETS; ++s) acc[s][m] += tail[s] * a;
             }
         }
         float mine = 0.f;

@@ -480,3 +480,25 @@ def test_out_over_an_operand_is_refused(M):
     wide[:, :64] = x
     vm.int8_linear(wide[:, :64], w, out=wide[:, 64:])     # columns side by side
     assert torch.equal(wide[:, :64], x) and torch.equal(wide[:, 64:], vm.int8_linear(x, w))
+
+
+@pytest.mark.parametrize("M", [1, 2, 4, 8])
+@pytest.mark.parametrize("K", [1, 15, 16, 17, 31, 1000, 1001, 4095, 4097, 4111, 8191])
+def test_few_rows_of_aligned_weights_with_a_ragged_end(M, K):
+    """Weights whose rows start on 16-byte boundaries and do not end on one: the last bytes are read one by one, nothing behind them."""
+    import sm120_moe_bench_b200 as vm
+    pitch = (K + 15) // 16 * 16
+    for N in (1, 2, 60, 5000):
+        a = random_rows(vm, (M, K), 94)
+        store = torch.randint(-128, 128, (N * pitch + 16,), generator=gen(95), device="cuda", dtype=torch.int8)
+        w = vm.Int8Rows(store[:N * pitch].view(N, pitch)[:, :K], torch.rand(N, generator=gen(96), device="cuda"))
+        y = vm.int8_matmul(a, w, out_dtype=torch.float32)
+        check_product(y, exact_product(a, w))
+        store.view(-1)[N * pitch:] = 99
+        for r in range(0, N, 7):
+            store[r * pitch + K:(r + 1) * pitch] = 99     # what lies behind a row counts for nothing
+        assert torch.equal(vm.int8_matmul(a, w, out_dtype=torch.float32), y)
+        if N % 2 == 0:
+            check_swiglu(vm.int8_matmul(a, w, swiglu=True, out_dtype=torch.float32), exact_product(a, w), N // 2)
+        x = torch.randn(M, K, generator=gen(97), device="cuda").bfloat16()
+        assert torch.equal(vm.int8_linear(x, w), vm.int8_matmul(vm.quantize_int8(x), w))
