@@ -398,6 +398,10 @@ int vmoe_int8_experts(const void* x, int64_t x_stride, int32_t dtype, int32_t M,
 /* Status word of the 8-bit products on the current device: VMOE_OK, or VMOE_ERR_TIMEOUT when a bounded wait inside one of
  * them ran out since the last reading (that product's output is not complete).  Synchronises the stream, clears the word. */
 int vmoe_int8_read_status(void* stream);
+/* Limit of every wait inside the 8-bit products launched (or captured) from now on, for the whole process, in microseconds:
+ * one second unless set.  0, for tests of what follows: every block of the tensor-core products holds its first copy back
+ * until one of its waits has run out (after a millisecond). */
+int vmoe_int8_set_wait_limit(int32_t microseconds);
 
 #ifdef __cplusplus
 }

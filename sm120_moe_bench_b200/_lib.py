@@ -106,6 +106,7 @@ SIGNATURES = {
                                     _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, C.c_int64, _P, _P, C.c_int64, C.c_int32, _P, C.c_size_t,
                                     _P]),
     "vmoe_int8_read_status": (C.c_int, [_P]),
+    "vmoe_int8_set_wait_limit": (C.c_int, [C.c_int32]),
 }
 
 

@@ -10,12 +10,34 @@
 #include "vmoe_int8.cuh"
 #include "vmoe_tc_common.cuh"
 
+#include <atomic>
 #include <string.h>
 
 namespace vmoe {
 
 // A wait that ran out leaves its status here (read and cleared by vmoe_int8_read_status).
 __device__ int g_i8_status;
+// Limit of a wait in microseconds; 0: the producers hold their first copies back until a wait has run out
+// (vmoe_int8_set_wait_limit).
+static std::atomic<int> g_i8_wait_us{(int)(MBAR_WAIT_LIMIT_NS / 1000)};
+
+// When a wait runs out: the role that gave up sets the CTA's flag and the status word and ends its loop; the others follow by
+// their own limits.  Behind the barrier that ends the roles, a CTA with its flag set waits, with mbar_wait's limit, for the
+// copies and MMAs that nobody waited for (i8_unwind): nothing of it is under way when it leaves.
+__device__ __forceinline__ bool i8_wait(uint64_t* bar, uint32_t parity, unsigned long long limit_ns) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const unsigned long long t0 = global_timer_ns();
+    for (uint32_t i = 1;; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63u) == 0 && global_timer_ns() - t0 > limit_ns) return false;
+    }
+}
+// No copy for now, for tests: until the CTA's flag is set, or mbar_wait's limit has passed.
+static __device__ __noinline__ void i8_hold(const int* abort_flag) {
+    const unsigned long long t0 = global_timer_ns();
+    while (*reinterpret_cast<const volatile int*>(abort_flag) == 0 && global_timer_ns() - t0 < MBAR_WAIT_LIMIT_NS) {}
+    __syncwarp();
+}
 
 __device__ __forceinline__ void i8_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -57,7 +79,7 @@ constexpr int I8P_TOKENS = 256;                           // tokens per item at 
 
 struct I8Shared {
     uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
-    uint64_t tmem_full[2], tmem_empty[2];
+    uint64_t tmem_full[2], tmem_empty[2], done;           // done: every MMA has completed
     uint32_t tmem_base;
     int abort_flag;
     int blocks;                                           // token blocks of all experts
@@ -69,7 +91,9 @@ struct I8TcParams {
     CUtensorMap map_w;                                    // [E, weight rows, K]
     CUtensorMap map_a64, map_a16;                         // token rows [M, K] in boxes of 64 and 16 (split: of the tile's tokens)
     I8Problem p;
+    unsigned long long wait_ns;                           // limit of a wait
     int kblocks, ctiles, stages, tokens;                  // tokens: most of an item
+    int hold;                                             // the first copies come when a wait has run out
 };
 
 struct I8Item { int expert, ctile, row0, rows, n; };
@@ -96,9 +120,18 @@ __device__ __forceinline__ void i8_abort(int* flag) {
     atomicExch(&g_i8_status, VMOE_ERR_TIMEOUT);
     atomicExch(flag, 1);
 }
-// After a wait that ran out: the copies of the last stages have to land (or their own limit pass) before the CTA leaves.
-__device__ __forceinline__ void i8_drain(uint64_t* full, uint32_t issued, int stages) {
-    for (uint32_t g = issued > (uint32_t)stages ? issued - stages : 0; g < issued; ++g) mbar_wait(&full[g % stages], (g / stages) & 1);
+// issued: the producer's stages; committed: `done` stands for all MMAs already.  The whole CTA calls it.
+static __device__ __noinline__ void i8_unwind(uint64_t* full, uint32_t issued, int stages, uint64_t* done, bool committed, bool leader) {
+    const int warp = threadIdx.x >> 5;
+    if (warp == 0) {
+        for (uint32_t g = issued > (uint32_t)stages ? issued - stages : 0; g < issued; ++g) mbar_wait(&full[g % stages], (g / stages) & 1);
+    } else if (warp == 1) {
+        if (leader && !committed) tc_commit(done);
+        __syncwarp();
+        mbar_wait(done, 0);
+    }
+    __syncwarp();
+    __syncthreads();
 }
 
 template <typename O_> __device__ __forceinline__ void i8_put(O_* at, float v);
@@ -124,6 +157,7 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
     if (tid == 0) {
         for (int i = 0; i < stages; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&sh->tmem_full[i], 1); mbar_init(&sh->tmem_empty[i], I8P_EPI_WARPS); }
+        mbar_init(&sh->done, 1);
         sh->abort_flag = 0;
         mbar_fence_init();
     }
@@ -157,21 +191,23 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
     __syncthreads();
     const long long total = (long long)sh->blocks * P.ctiles;
     const int kblocks = P.kblocks;
+    uint32_t g = 0;                                       // stages of the producer, of the MMA warp
+    bool leader = false;
 
     if (warp == 0) {
         // ------------------------------------------------------------- producer: the item's weight rows and token rows
-        const bool leader = elect_one();
-        uint32_t g = 0;
+        leader = elect_one();
         bool ok = true;
+        int gone = 0;                                     // the flag, as of the last stage
+        if (P.hold && blockIdx.x < total) i8_hold(&sh->abort_flag);
         for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
             const I8Item u = i8_item(P, s_pref, s_off, item);
             const int ch = u.ctile * (SWIGLU ? 128 : I8P_ROWS);
             for (int kb = 0; kb < kblocks; ++kb) {
                 const int slot = g % stages;
                 bool w = true;
-                if (g >= (uint32_t)stages) w = mbar_wait(&sh->empty[slot], ((g / stages) - 1) & 1);
-                if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
-                if (*reinterpret_cast<volatile int*>(&sh->abort_flag)) { ok = false; break; }
+                if (g >= (uint32_t)stages) w = i8_wait(&sh->empty[slot], ((g / stages) - 1) & 1, P.wait_ns);
+                if (!__all_sync(0xffffffffu, w && !gone)) { ok = false; break; }
                 uint8_t* st = smem + (size_t)slot * stage_bytes;
                 uint64_t* bar = &sh->full[slot];
                 if (leader) {
@@ -184,19 +220,17 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
                     for (; r < u.n; r += I8_BOX_SMALL)
                         tma_load_2d(st + 2 * I8_A_BYTES + r * I8_KB, &P.map_a16, kb * I8_KB, u.row0 + r, bar);
                 }
+                gone = *reinterpret_cast<volatile int*>(&sh->abort_flag);
                 __syncwarp();
                 ++g;
             }
         }
-        if (!ok) {
-            if (leader) i8_abort(&sh->abort_flag);
-            __syncwarp();
-            i8_drain(sh->full, g, stages);
-        }
+        if (!ok && leader) i8_abort(&sh->abort_flag);
+        __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issuer (warp-uniform loop, one elected lane issues)
-        const bool leader = elect_one();
-        uint32_t g = 0, it = 0;
+        leader = elect_one();
+        uint32_t it = 0;
         bool ok = true;
         const uint32_t smem16 = smem_u32(smem) >> 4;
         for (long long item = blockIdx.x; item < total && ok; item += gridDim.x) {
@@ -204,11 +238,11 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
             const uint32_t idesc = i8_idesc(128, u.n);
             const uint32_t buf = two ? it & 1 : 0, use = two ? it >> 1 : it, acc = tmem + buf * I8P_TOKENS;
             bool w = true;
-            if (use >= 1) w = mbar_wait(&sh->tmem_empty[buf], (use - 1) & 1);
+            if (use >= 1) w = i8_wait(&sh->tmem_empty[buf], (use - 1) & 1, P.wait_ns);
             if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
             for (int kb = 0; kb < kblocks; ++kb) {
                 const int slot = g % stages;
-                if (!__all_sync(0xffffffffu, mbar_wait(&sh->full[slot], (g / stages) & 1))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, i8_wait(&sh->full[slot], (g / stages) & 1, P.wait_ns))) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t st16 = smem16 + slot * (stage_bytes >> 4);
 #pragma unroll
@@ -255,7 +289,7 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
             const int ch2 = SWIGLU ? p.N + ch : ch + 128;
             const float sw0 = ch < p.N ? wsc[ch] : 0.f;
             const float sw1 = (SWIGLU ? ch : ch2) < p.N ? wsc[ch2] : 0.f;
-            const bool w = mbar_wait(&sh->tmem_full[buf], use & 1);
+            const bool w = i8_wait(&sh->tmem_full[buf], use & 1, P.wait_ns);
             if (!__all_sync(0xffffffffu, w)) { if (lane == 0) i8_abort(&sh->abort_flag); break; }
             tc_fence_after();
             const uint32_t tacc = tmem + buf * I8P_TOKENS + ((uint32_t)(quad * 32) << 16);
@@ -304,6 +338,7 @@ i8_tc_kernel(const __grid_constant__ I8TcParams P) {
     }
     tc_fence_before();
     __syncthreads();
+    if (sh->abort_flag) i8_unwind(sh->full, g, stages, &sh->done, false, leader);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC_TMEM_COLS) : "memory");
@@ -330,6 +365,8 @@ __device__ __forceinline__ int4 i8_ld_peer(uint32_t addr) {
     return r;
 }
 
+constexpr int I8_NOTHING = -0x7fffffff - 1;               // stands for the partial sums of a CTA whose waits ran out; no sum of
+                                                          // I8_MAX_K products of codes has this value
 template <bool SWIGLU>
 __global__ void __launch_bounds__(I8S_THREADS, 1)
 i8_split_kernel(const __grid_constant__ I8TcParams P) {
@@ -357,15 +394,16 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_base;
+    bool ok = true, leader = false;
+    uint32_t issued = 0;
 
     if (warp == 0) {
-        const bool leader = elect_one();
-        bool ok = true;
-        uint32_t issued = 0;
+        leader = elect_one();
+        if (P.hold) i8_hold(&sh.abort_flag);
         for (int kb = kb0; kb < kb1; ++kb) {
             const int g = kb - kb0, slot = g % stages;
             bool w = true;
-            if (g >= stages) w = mbar_wait(&sh.empty[slot], ((g / stages) - 1) & 1);
+            if (g >= stages) w = i8_wait(&sh.empty[slot], ((g / stages) - 1) & 1, P.wait_ns);
             if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
             uint8_t* st = smem + (size_t)slot * stage_bytes;
             if (leader) {
@@ -381,17 +419,13 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
             }
             ++issued;
         }
-        if (!ok) {
-            if (leader) i8_abort(&sh.abort_flag);
-            i8_drain(sh.full, issued, stages);
-        }
+        if (!ok && leader) i8_abort(&sh.abort_flag);
     } else if (warp == 1) {
-        const bool leader = elect_one();
-        bool ok = true;
+        leader = elect_one();
         const uint32_t smem16 = smem_u32(smem) >> 4, idesc = i8_idesc(128, n);
         for (int kb = kb0; kb < kb1; ++kb) {
             const int g = kb - kb0, slot = g % stages;
-            if (!__all_sync(0xffffffffu, mbar_wait(&sh.full[slot], (g / stages) & 1))) { ok = false; break; }
+            if (!__all_sync(0xffffffffu, i8_wait(&sh.full[slot], (g / stages) & 1, P.wait_ns))) { ok = false; break; }
             tc_fence_after();
             const uint32_t st16 = smem16 + slot * (stage_bytes >> 4);
 #pragma unroll
@@ -407,7 +441,7 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
     } else {
         // partial sums to shared memory, [token][channel]; the stages are free once every MMA has completed
         const int quad = warp & 3;
-        if (!mbar_wait(&sh.done, 0)) {
+        if (!__all_sync(0xffffffffu, i8_wait(&sh.done, 0, P.wait_ns))) {
             if (lane == 0) i8_abort(&sh.abort_flag);
         } else {
             tc_fence_after();
@@ -423,6 +457,11 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
     }
     tc_fence_before();
     __syncthreads();
+    if (sh.abort_flag) {
+        i8_unwind(sh.full, issued, stages, &sh.done, ok, leader);
+        for (int i = tid; i < n * 128; i += I8S_THREADS) reinterpret_cast<int*>(smem)[i] = I8_NOTHING;
+        __syncthreads();                                  // (alone in its cluster it reads them itself)
+    }
     if (split > 1) i8_cluster_sync();
     // The CTAs of the cluster share the tile's tokens out; a thread owns four neighbouring channels of a token.
     const uint32_t base = smem_u32(smem);
@@ -430,44 +469,45 @@ i8_split_kernel(const __grid_constant__ I8TcParams P) {
     const int t_end = min(rows, (rank + 1) * per);
     constexpr int QUADS = SWIGLU ? 16 : 32;               // groups of four channels per token
     const bool vec = ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0 && p.N % 4 == 0;
-    if (!sh.abort_flag)
-        for (int i = tid + rank * per * QUADS; i < t_end * QUADS; i += I8S_THREADS) {
-            const int t = i / QUADS, c = (i % QUADS) * 4, ch = ch0 + c;
-            if (ch >= p.N) continue;
-            int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0};
-            const uint32_t at = base + (uint32_t)(t * 128 + c) * 4;
-            for (int r = 0; r < split; ++r) {
-                const uint32_t a = i8_cluster_addr(at, r);
-                const int4 x = i8_ld_peer(a);
-                s0[0] += x.x; s0[1] += x.y; s0[2] += x.z; s0[3] += x.w;
-                if (SWIGLU) {
-                    const int4 y = i8_ld_peer(a + 64 * 4);
-                    s1[0] += y.x; s1[1] += y.y; s1[2] += y.z; s1[3] += y.w;
-                }
-            }
-            const float sa = p.a_scale[tok0 + t];
-            float o[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int n_ = min(ch + k, p.N - 1);
-                o[k] = i8_scaled(s0[k], sa, p.w_scale[n_]);
-                if (SWIGLU) o[k] = i8_scaled(s1[k], sa, p.w_scale[p.N + n_]) * i8_silu(o[k]);
-            }
-            const long long at_out = (long long)(tok0 + t) * p.out_stride + ch;
-            if (vec && p.out_dtype == VMOE_F32) {
-                *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at_out) = make_float4(o[0], o[1], o[2], o[3]);
-            } else if (vec) {
-                union { uint2 w; __nv_bfloat16 b[4]; __half h[4]; } q;
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (p.out_dtype == VMOE_BF16) q.b[k] = __float2bfloat16_rn(o[k]); else q.h[k] = __float2half_rn(o[k]);
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at_out) = q.w;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (ch + k < p.N) i8_store(p.out, at_out + k, p.out_dtype, o[k]);
+    for (int i = tid + rank * per * QUADS; i < t_end * QUADS; i += I8S_THREADS) {
+        const int t = i / QUADS, c = (i % QUADS) * 4, ch = ch0 + c;
+        if (ch >= p.N) continue;
+        int s0[4] = {0, 0, 0, 0}, s1[4] = {0, 0, 0, 0}, low = 0;
+        const uint32_t at = base + (uint32_t)(t * 128 + c) * 4;
+        for (int r = 0; r < split; ++r) {
+            const uint32_t a = i8_cluster_addr(at, r);
+            const int4 x = i8_ld_peer(a);
+            low = min(low, x.x);
+            s0[0] += x.x; s0[1] += x.y; s0[2] += x.z; s0[3] += x.w;
+            if (SWIGLU) {
+                const int4 y = i8_ld_peer(a + 64 * 4);
+                s1[0] += y.x; s1[1] += y.y; s1[2] += y.z; s1[3] += y.w;
             }
         }
+        const float sa = p.a_scale[tok0 + t];
+        float o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int n_ = min(ch + k, p.N - 1);
+            o[k] = i8_scaled(s0[k], sa, p.w_scale[n_]);
+            if (SWIGLU) o[k] = i8_scaled(s1[k], sa, p.w_scale[p.N + n_]) * i8_silu(o[k]);
+        }
+        if (low == I8_NOTHING) continue;
+        const long long at_out = (long long)(tok0 + t) * p.out_stride + ch;
+        if (vec && p.out_dtype == VMOE_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at_out) = make_float4(o[0], o[1], o[2], o[3]);
+        } else if (vec) {
+            union { uint2 w; __nv_bfloat16 b[4]; __half h[4]; } q;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (p.out_dtype == VMOE_BF16) q.b[k] = __float2bfloat16_rn(o[k]); else q.h[k] = __float2half_rn(o[k]);
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + at_out) = q.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (ch + k < p.N) i8_store(p.out, at_out + k, p.out_dtype, o[k]);
+        }
+    }
     __syncthreads();
     if (split > 1) i8_cluster_sync();                     // nobody leaves while its partial sums are read
     if (warp == 1) {
@@ -523,11 +563,18 @@ static int i8_tokens(const I8Problem& p, int kblocks, int ctiles) {
     return best;
 }
 
+static void i8_limits(I8TcParams* P) {
+    const int us = g_i8_wait_us.load(std::memory_order_relaxed);
+    P->hold = us == 0;
+    P->wait_ns = us ? 1000ull * (unsigned)us : 1000000ull;
+}
+
 template <bool SWIGLU, typename O_>
 static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
     I8TcParams P;
     memset(&P, 0, sizeof(P));
     P.p = p;
+    i8_limits(&P);
     P.kblocks = (p.K + I8_KB - 1) / I8_KB;
     P.ctiles = SWIGLU ? (p.N + 127) / 128 : (p.N + I8P_ROWS - 1) / I8P_ROWS;
     P.tokens = i8_tokens(p, P.kblocks, P.ctiles);
@@ -562,6 +609,7 @@ static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
     I8TcParams P;
     memset(&P, 0, sizeof(P));
     P.p = p;
+    i8_limits(&P);
     P.kblocks = (p.K + I8_KB - 1) / I8_KB;
     P.ctiles = SWIGLU ? (p.N + 63) / 64 : (p.N + 127) / 128;
     const int ttiles = (p.M + I8S_TOKENS - 1) / I8S_TOKENS;
@@ -600,6 +648,12 @@ static int launch_i8_split_t(const I8Problem& p, cudaStream_t st) {
 int launch_i8_split(const I8Problem& p, cudaStream_t st) { return p.swiglu ? launch_i8_split_t<true>(p, st) : launch_i8_split_t<false>(p, st); }
 
 }  // namespace vmoe
+
+extern "C" int vmoe_int8_set_wait_limit(int32_t microseconds) {
+    if (microseconds < 0) return VMOE_ERR_SHAPE;
+    vmoe::g_i8_wait_us.store(microseconds, std::memory_order_relaxed);
+    return VMOE_OK;
+}
 
 extern "C" int vmoe_int8_read_status(void* stream) {
     int v = 0;

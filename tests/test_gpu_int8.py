@@ -502,3 +502,28 @@ def test_few_rows_of_aligned_weights_with_a_ragged_end(M, K):
             check_swiglu(vm.int8_matmul(a, w, swiglu=True, out_dtype=torch.float32), exact_product(a, w), N // 2)
         x = torch.randn(M, K, generator=gen(97), device="cuda").bfloat16()
         assert torch.equal(vm.int8_linear(x, w), vm.int8_matmul(vm.quantize_int8(x), w))
+
+
+@pytest.mark.parametrize("M,N,K,E", [(20, 300, 2048, 0), (48, 512, 4096, 0), (129, 640, 256, 0), (700, 1024, 4096, 0), (2000, 1024, 640, 0),
+                                     (50, 96, 512, 8), (900, 256, 1024, 4)])
+def test_a_wait_that_runs_out(M, N, K, E):
+    """With a limit of zero the first wait for data runs out in every block, and a copy starts after it.  The call returns, leaves
+    its status, stores nothing that is not a right result, and the next call is right.  (Split over a cluster or not, persistent,
+    per expert.)"""
+    import sm120_moe_bench_b200 as vm
+    from sm120_moe_bench_b200._lib import lib
+    plan = vm.plan_tokens((torch.arange(M, device="cuda", dtype=torch.int32) % E)[:, None].contiguous(), E) if E else None
+    a, w = random_rows(vm, (M, K), 98), random_rows(vm, (E, 2 * N, K) if E else (2 * N, K), 99)
+    assert vm.int8_status() == 0
+    for swiglu in (False, True):
+        want = vm.int8_matmul(a, w, plan, swiglu=swiglu, out_dtype=torch.float32)
+        out = torch.full_like(want, 12345.0)
+        try:
+            assert lib.vmoe_int8_set_wait_limit(0) == 0
+            vm.int8_matmul(a, w, plan, swiglu=swiglu, out=out)
+        finally:
+            lib.vmoe_int8_set_wait_limit(10 ** 6)
+        assert vm.int8_status() == 6
+        assert bool(((out == 12345) | (out == want)).all())
+        assert torch.equal(vm.int8_matmul(a, w, plan, swiglu=swiglu, out_dtype=torch.float32), want)
+        assert vm.int8_status() == 0

@@ -90,3 +90,9 @@ def test_linear_and_experts_checks():
     for name in ("x", "ids", "wt", "w13", "s13", "w2", "s2", "out"):
         assert experts(**{name: None}) == 1, name
     assert experts(scratch=None) == 4 and experts(bytes_=64) == 4 and experts(scratch=b + 8) == 3
+
+
+def test_wait_limit_checks():
+    lib = _lib()
+    assert lib.vmoe_int8_set_wait_limit(-1) == 2
+    assert lib.vmoe_int8_set_wait_limit(10 ** 6) == 0     # what it is from the start
