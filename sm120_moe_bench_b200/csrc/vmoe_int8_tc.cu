@@ -541,6 +541,11 @@ bool i8_tc_ok(const I8Problem& p) {
 }
 
 constexpr size_t I8P_SMEM = 227 * 1024;
+// Shared memory of the persistent kernel; an item size goes with a number of experts if two stages fit.
+static constexpr size_t i8_tc_smem(int tokens, int E, int stages) {
+    return (size_t)stages * (2 * I8_A_BYTES + (size_t)tokens * I8_KB) + sizeof(I8Shared) + 2 * ((size_t)E + 1) * sizeof(int) + 1024;
+}
+static_assert(i8_tc_smem(64, I8_TC_MAX_EXPERTS, 2) <= I8P_SMEM, "the smallest items go with every number of experts");
 
 // Tokens per item.  Grouped: from the average rows per expert (the counts are on the device); 64 experts, N = 1024, K = 4096,
 // items of 64 / 128 / 256 tokens: 16 rows each 46 / 47 / 48 us, 100 rows 64 / 56 / 57, 160 rows 85 / 75 / 66, 320 rows
@@ -550,7 +555,9 @@ constexpr size_t I8P_SMEM = 227 * 1024;
 static int i8_tokens(const I8Problem& p, int kblocks, int ctiles) {
     if (p.offsets) {
         const long long per = p.M / p.E;
-        return per <= 32 ? 64 : per <= 128 ? 128 : I8P_TOKENS;
+        int u = per <= 32 ? 64 : per <= 128 ? 128 : I8P_TOKENS;
+        while (u > 64 && i8_tc_smem(u, p.E, 2) > I8P_SMEM) u /= 2;       // from 11496 and 15592 experts on
+        return u;
     }
     int best = 128;
     long long least = -1;
@@ -578,11 +585,9 @@ static int launch_i8_tc_t(const I8Problem& p, cudaStream_t st) {
     P.kblocks = (p.K + I8_KB - 1) / I8_KB;
     P.ctiles = SWIGLU ? (p.N + 127) / 128 : (p.N + I8P_ROWS - 1) / I8P_ROWS;
     P.tokens = i8_tokens(p, P.kblocks, P.ctiles);
-    const size_t stage = 2 * I8_A_BYTES + (size_t)P.tokens * I8_KB;
-    const size_t rest = sizeof(I8Shared) + 2 * ((size_t)p.E + 1) * sizeof(int) + 1024;
     P.stages = I8P_MAX_STAGES;
-    while (P.stages > 2 && P.stages * stage + rest > I8P_SMEM) --P.stages;
-    const size_t smem = P.stages * stage + rest;
+    while (P.stages > 2 && i8_tc_smem(P.tokens, p.E, P.stages) > I8P_SMEM) --P.stages;
+    const size_t smem = i8_tc_smem(P.tokens, p.E, P.stages);
     if (smem > I8P_SMEM) return VMOE_ERR_LIMIT;
     int rc;
     if ((rc = i8_map_w(&P.map_w, p, SWIGLU ? 128 : I8P_ROWS))) return rc;

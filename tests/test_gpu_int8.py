@@ -527,3 +527,24 @@ def test_a_wait_that_runs_out(M, N, K, E):
         assert bool(((out == 12345) | (out == want)).all())
         assert torch.equal(vm.int8_matmul(a, w, plan, swiglu=swiglu, out_dtype=torch.float32), want)
         assert vm.int8_status() == 0
+
+
+@pytest.mark.parametrize("E,per", [(8192, 130), (11495, 130), (11496, 130), (13000, 200), (15591, 40), (15592, 40), (16384, 130), (16384, 3), (16385, 3)])
+def test_thousands_of_experts(E, per):
+    """The experts' tables lie beside the operands in shared memory: item sizes that leave no room for them are not taken."""
+    import sm120_moe_bench_b200 as vm
+    M, N, K = E * per, 8, 16
+    offsets = torch.arange(0, M + 1, per, device="cuda", dtype=torch.int32)
+    pairs = torch.arange(M, device="cuda", dtype=torch.int32)
+    plan = vm.TokenPlan(offsets, pairs[:, None], pairs, E)
+    a, w = random_rows(vm, (M, K), 100), random_rows(vm, (E, N, K), 102)
+    exact = torch.bmm(a.q.view(E, per, K).double(), w.q.double().transpose(1, 2))
+    want = (exact * a.scale.view(E, per, 1).double() * w.scale.view(E, 1, N).double()).view(M, N)
+    check_product(vm.int8_matmul(a, w, plan, out_dtype=torch.float32), want)
+    check_swiglu(vm.int8_matmul(a, w, plan, swiglu=True, out_dtype=torch.float32), want, N // 2)
+    odd = vm.Int8Rows(w.q[..., :K - 1].contiguous(), w.scale)         # packed first
+    short = vm.Int8Rows(a.q[:, :K - 1], a.scale)
+    exact = torch.bmm(short.q.reshape(E, per, K - 1).double(), odd.q.double().transpose(1, 2))
+    want = (exact * a.scale.view(E, per, 1).double() * w.scale.view(E, 1, N).double()).view(M, N)
+    check_product(vm.int8_matmul(short, odd, plan, out_dtype=torch.float32), want)
+    assert vm.int8_status() == 0
