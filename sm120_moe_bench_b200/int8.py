@@ -8,14 +8,14 @@
 
 The integer sums are exact, the scales are applied in f32 and the result is rounded once; a result does not depend on the
 batch around it.  These are inference operators: they have no gradient, and floating tensors that require one are refused
-while gradients are enabled.
+while gradients are enabled, as are those that carry a forward-mode tangent.
 """
 from __future__ import annotations
 
 import torch
 
 from ._lib import lib
-from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, launch, refuse_overlap
+from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, has_tangent, launch, refuse_overlap
 
 MAX_K = 131071
 
@@ -52,6 +52,8 @@ class Int8Rows:
 def _no_grad(t: torch.Tensor, name: str) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: the 8-bit operators have none")
+    if has_tangent(t):
+        raise ValueError(f"{name} carries a forward-mode derivative: the 8-bit operators have none")
 
 
 def _codes(rows: int, K: int, device) -> torch.Tensor:

@@ -13,7 +13,8 @@ made here (rows and gradients) and left as they were in a tensor given as ``out`
 
 A backward pass is captured into a CUDA graph together with its forward pass.  An eager graph of the same leaf tensor has
 to be gone by then (a leaf's accumulator stays bound to the stream of the graph that made it, which the capture must not
-wait for): with one of these operators' graphs still alive the captured call raises.
+wait for): with one of these operators' graphs still alive the captured call raises.  Derivatives are reverse-mode: a tensor
+that carries a forward-mode tangent is refused.
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import threading
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 
@@ -69,6 +71,16 @@ def check_rows(t: torch.Tensor, name: str, rows: int | None = None, device: torc
     if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_ROWS:
         raise ValueError(f"{name} has a dimension of more than {MAX_ROWS}")
     raise ValueError(f"the elements of a row of {name} must lie next to each other")
+
+
+def has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether one of them carries a forward-mode derivative: ``requires_grad`` does not tell, and the kernels would drop it."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _refuse_tangent(*tensors: torch.Tensor | None) -> None:
+    if has_tangent(*tensors):
+        raise NotImplementedError("the token sort has no forward-mode derivatives, only reverse-mode ones")
 
 
 def overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -258,12 +270,14 @@ class _SortTokens(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
+        _refuse_tangent(grad)
         grad = _dense_rows(grad)
         # with create_graph the gradient is differentiable itself
         return (unsort_tokens if torch.is_grad_enabled() else _unsort)(grad, ctx.plan), None
 
 
 def _unsort_backward(ctx, grad):
+    _refuse_tangent(grad)
     rows, weights = ctx.saved_tensors
     plan, grad = ctx.plan, _dense_rows(grad)
     M, T, K = plan.tokens, plan.topk, rows.shape[1]
@@ -297,6 +311,7 @@ def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = Non
     """``rows[r] = x[token of row r]``: the token rows ``[M, K]`` in expert order, ``[M * T, K]``.  Differentiable in ``x``
     (a token's gradient is the sum over its rows) unless ``out`` is given."""
     check_rows(x, "x", plan.tokens, plan.device)
+    _refuse_tangent(x, out)
     if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
@@ -311,6 +326,7 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | N
     """``out[m] = sum_t weights[m, t] * rows[row of (m, t)]``: rows ``[M * T, K]`` in expert order back to tokens ``[M, K]``.
     ``weights`` f32 ``[M, T]`` (None = 1).  Differentiable in ``rows`` and ``weights`` unless ``out`` is given."""
     check_rows(rows, "rows", plan.rows, plan.device)
+    _refuse_tangent(rows, weights, out)
     if weights is not None:
         if weights.device != rows.device or weights.dtype != torch.float32 or tuple(weights.shape) != (plan.tokens, plan.topk):
             raise ValueError(f"weights must be a float32 tensor [{plan.tokens}, {plan.topk}] on the device of rows")

@@ -548,3 +548,21 @@ def test_thousands_of_experts(E, per):
     want = (exact * a.scale.view(E, per, 1).double() * w.scale.view(E, 1, N).double()).view(M, N)
     check_product(vm.int8_matmul(short, odd, plan, out_dtype=torch.float32), want)
     assert vm.int8_status() == 0
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+    import sm120_moe_bench_b200 as vm
+    w = random_rows(vm, (8, 32), 104)
+    w13, w2 = random_rows(vm, (2, 32, 32), 106), random_rows(vm, (2, 32, 16), 108)
+    x, ids, wt = torch.randn(6, 32, generator=gen(110), device="cuda"), torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.ones(6, 2, device="cuda")
+    a, out = vm.quantize_int8(x), torch.zeros(6, 8, device="cuda")
+    with forward_ad.dual_level():
+        dx, dwt, dout = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, wt, out))
+        for call in (lambda: vm.quantize_int8(dx), lambda: vm.quantize_int8(dx[None].contiguous()), lambda: vm.int8_linear(dx, w),
+                     lambda: vm.int8_experts(dx, w13, w2, ids, wt), lambda: vm.int8_experts(x, w13, w2, ids, dwt),
+                     lambda: vm.int8_linear(x, w, out=dout), lambda: vm.int8_matmul(a, w, out=dout)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with pytest.raises(ValueError, match="forward-mode"), mode():
+                    call()
+        vm.int8_linear(x, w)

@@ -434,3 +434,34 @@ def test_out_over_an_operand_is_refused():
     want = vm.unsort_tokens(wide[:, :K].contiguous(), plan, w)
     vm.unsort_tokens(wide[:, :K], plan, w, out=wide[:M, K:])
     assert torch.equal(wide[:M, K:], want)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor does not require a gradient, and a result without its tangent would be a derivative of zero."""
+    from torch.autograd import forward_ad
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 6, 2, 4, 8
+    plan = vm.plan_tokens(ids_of(M, T, E, 56), E)
+    x, rows, w = rows_of(M, K, torch.float32, 57), rows_of(M * T, K, torch.float32, 58), torch.rand(M, T, device="cuda")
+    want = vm.sort_tokens(x, plan), vm.unsort_tokens(rows, plan, w)
+    with forward_ad.dual_level():
+        dx, dr, dw = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, rows, w))
+        for call in (lambda: vm.sort_tokens(dx, plan), lambda: vm.unsort_tokens(dr, plan, w), lambda: vm.unsort_tokens(rows, plan, dw),
+                     lambda: vm.unsort_tokens(dr, plan), lambda: vm.sort_tokens(x, plan, out=dr), lambda: vm.unsort_tokens(rows, plan, w, out=dx),
+                     lambda: vm.sort_tokens(forward_ad.make_dual(x.clone().requires_grad_(), x), plan)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with pytest.raises(NotImplementedError), mode():
+                    call()
+        assert torch.equal(vm.sort_tokens(x, plan), want[0]) and torch.equal(vm.unsort_tokens(rows, plan, w), want[1])
+    xr, rr, wr = (t.clone().requires_grad_() for t in (x, rows, w))
+    sorted_x, y = vm.sort_tokens(xr, plan), vm.unsort_tokens(rr, plan, wr)
+    with forward_ad.dual_level():                         # the incoming gradient has a tangent
+        dg, dy = forward_ad.make_dual(rows, rows), forward_ad.make_dual(x, x)
+        for create in (False, True):
+            for call in (lambda: torch.autograd.grad(sorted_x, xr, dg, retain_graph=True, create_graph=create),
+                         lambda: torch.autograd.grad(y, rr, dy, retain_graph=True, create_graph=create),
+                         lambda: torch.autograd.grad(y, wr, dy, retain_graph=True, create_graph=create)):
+                with pytest.raises(NotImplementedError):
+                    call()
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda t: vm.sort_tokens(t, plan), (x,), (x,))

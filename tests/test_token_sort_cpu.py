@@ -122,3 +122,17 @@ def test_shared_memory_is_found():
     assert not overlap(wide[:, :0], wide) and not overlap(wide[3:4, :8], wide[:, 8:12])
     assert overlap(wide[:, :8], wide[:, 7:]) and overlap(wide[:5], wide[4:]) and overlap(wide, wide[8, 19:])
     assert overlap(torch.zeros(1, 4).expand(5, 4), wide) is False
+
+
+def test_forward_mode_tangents_are_seen():
+    from torch.autograd import forward_ad
+    from sm120_moe_bench_b200.token_sort import has_tangent
+
+    x = torch.ones(3)
+    assert not has_tangent(x)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones(3))
+        assert has_tangent(dual) and has_tangent(None, x, dual * 2) and not has_tangent(x, None) and not dual.requires_grad
+        with torch.no_grad():                             # forward mode does not mind
+            assert has_tangent(dual)
+    assert not has_tangent(dual)
