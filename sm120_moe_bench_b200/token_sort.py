@@ -14,7 +14,8 @@ made here (rows and gradients) and left as they were in a tensor given as ``out`
 A backward pass is captured into a CUDA graph together with its forward pass.  An eager graph of the same leaf tensor has
 to be gone by then (a leaf's accumulator stays bound to the stream of the graph that made it, which the capture must not
 wait for): with one of these operators' graphs still alive the captured call raises.  Derivatives are reverse-mode: a tensor
-that carries a forward-mode tangent is refused.
+that carries a forward-mode tangent is refused.  So is recording a call with torch.jit.trace or make_fx; torch.compile runs it
+as it is.
 """
 from __future__ import annotations
 
@@ -39,8 +40,24 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
+_tracing, _dispatch_modes, _function_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+
+
+def traced() -> bool:
+    """Whether torch.jit.trace or make_fx records what runs now.  They see torch's own operators, not a kernel launched
+    beside them: the recorded program would hold the allocations and return them as they are."""
+    if _tracing():
+        return True
+    if not (_dispatch_modes() or _function_modes()):      # make_fx pushes one of either kind (0.2 us so far)
+        return False
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
+
+
 def launch(device: torch.device, name: str, fn, *args) -> None:
     """Call a C entry point on the device of its tensors, on that device's current stream."""
+    if traced():
+        raise RuntimeError(f"{name}: a kernel of this library cannot be traced (its launch would be missing from the recorded program)")
     index = device.index
     if index == _current_device():
         status = fn(*args, _raw_stream(index))

@@ -465,3 +465,35 @@ def test_forward_mode_is_refused():
                     call()
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.jvp(lambda t: vm.sort_tokens(t, plan), (x,), (x,))
+
+
+def test_traces_are_refused():
+    """torch.jit.trace and make_fx record torch's operators only: a trace would return the memory that was allocated for a result."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    import sm120_moe_bench_b200 as vm
+    ids = ids_of(6, 2, 4, 59)
+    plan = vm.plan_tokens(ids, 4)
+    x, rows, w = rows_of(6, 32, torch.float32, 60), rows_of(12, 32, torch.float32, 61), torch.rand(6, 2, device="cuda")
+    q = vm.quantize_int8(rows_of(8, 32, torch.float32, 62))
+    w13, w2 = vm.quantize_int8(torch.randn(4, 32, 32, device="cuda")), vm.quantize_int8(torch.randn(4, 32, 16, device="cuda"))
+    codes = vm.quantize_int8(x)
+    calls = (lambda t: vm.sort_tokens(t, plan), lambda t: vm.unsort_tokens(torch.cat([t, t]), plan, w), lambda t: vm.int8_linear(t, q),
+             lambda t: vm.quantize_int8(t).q, lambda t: t + vm.int8_matmul(codes, q).sum(), lambda t: vm.int8_experts(t, w13, w2, ids, w),
+             lambda t: t + vm.plan_tokens(ids, 4).expert_offsets.sum(), lambda t: vm.sort_tokens(t * 1, plan, out=rows.clone()))
+    for call in calls:
+        for trace in (lambda: make_fx(call)(x), lambda: make_fx(call, pre_dispatch=True)(x), lambda: torch.jit.trace(call, x, check_trace=False),
+                      lambda: make_fx(call)(x.clone().requires_grad_())):
+            with pytest.raises((RuntimeError, ValueError)):
+                trace()
+    assert torch.equal(vm.unsort_tokens(vm.sort_tokens(x, plan), plan), 2 * x)
+    # torch.compile runs the calls as they are
+    def step(t, weights):
+        return vm.unsort_tokens(vm.sort_tokens(t * 2, plan), plan, weights) + 1
+
+    got = torch.compile(step, backend="eager")(x, w)
+    assert torch.equal(got, step(x, w))
+    a, b = (t.clone().requires_grad_() for t in (x, w)), (t.clone().requires_grad_() for t in (x, w))
+    a, b = tuple(a), tuple(b)
+    ga = torch.autograd.grad(torch.compile(step, backend="eager")(*a).sum(), a)
+    gb = torch.autograd.grad(step(*b).sum(), b)
+    assert all(torch.equal(p, r) for p, r in zip(ga, gb))

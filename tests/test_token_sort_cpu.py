@@ -136,3 +136,37 @@ def test_forward_mode_tangents_are_seen():
         with torch.no_grad():                             # forward mode does not mind
             assert has_tangent(dual)
     assert not has_tangent(dual)
+
+
+def test_tracing_is_seen():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from torch.utils.flop_counter import FlopCounterMode
+    from sm120_moe_bench_b200.token_sort import launch, traced
+
+    x, seen = torch.ones(3), []
+
+    def f(t):
+        seen.append(traced())
+        return t + 1
+
+    class Plain(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    f(x)
+    with Plain(), FlopCounterMode(display=False):
+        f(x)
+    assert seen == [False, False]                         # modes that only watch are no hindrance
+    seen.clear()
+    torch.jit.trace(f, x, check_trace=False)
+    for mode in ("real", "fake", "symbolic"):
+        for pre in (False, True):
+            make_fx(f, tracing_mode=mode, pre_dispatch=pre)(x)
+    with Plain():
+        make_fx(f)(x)
+    make_fx(torch.func.functionalize(f))(x)
+    assert len(seen) >= 9 and all(seen)
+    assert not traced()
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda t: launch(torch.device("cuda", 0), "f", lambda *a: 0) or t)(x)
