@@ -13,6 +13,7 @@ while gradients are enabled, as are those that carry a forward-mode tangent.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import lib
 from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, has_tangent, launch, refuse_overlap
@@ -54,6 +55,11 @@ def _no_grad(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} requires a gradient: the 8-bit operators have none")
     if has_tangent(t):
         raise ValueError(f"{name} carries a forward-mode derivative: the 8-bit operators have none")
+
+
+def _no_grad_scales(rows: Int8Rows, name: str) -> None:
+    if rows.scale.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(rows.scale, f"{name}.scale")
 
 
 def _codes(rows: int, K: int, device) -> torch.Tensor:
@@ -141,6 +147,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
     With ``plan`` the rows are sorted by expert (``quantize_int8(x, plan)``) and each meets its expert's matrix of ``w``
     ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``, which must not share memory with an operand).  ``swiglu``: ``w``
     holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``, ``[M, N]``."""
+    _no_grad_scales(a, "a")
+    _no_grad_scales(w, "w")
     if a.q.dim() != 2:
         raise ValueError("a must be rows [M, K]")
     if plan is not None and (a.q.shape[0] != plan.rows or plan.device != a.q.device):
@@ -171,6 +179,7 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
     """``x [M, K]`` (bf16 / fp16 / f32) quantised row by row, times ``w [N, K]``: ``[M, N]`` in the type of ``x``.
     ``out`` must not share memory with ``x`` or ``w``."""
     _no_grad(x, "x")
+    _no_grad_scales(w, "w")
     check_rows(x, "x")
     N = _out_columns(w, x.shape[1], x.device, swiglu, None)
     stride = N
@@ -206,6 +215,8 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
     everything between is f32, and the sum is rounded once to the type of ``x``.  ``expert_map`` as in ``plan_tokens``."""
     _no_grad(x, "x")
     _no_grad(topk_weights, "topk_weights")
+    _no_grad_scales(w13, "w13")
+    _no_grad_scales(w2, "w2")
     if topk_ids.dim() != 2:
         raise ValueError("topk_ids must be an int32 tensor [tokens, choices]")
     check_rows(x, "x", topk_ids.shape[0], topk_ids.device)

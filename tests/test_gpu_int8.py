@@ -566,3 +566,29 @@ def test_forward_mode_is_refused():
                 with pytest.raises(ValueError, match="forward-mode"), mode():
                     call()
         vm.int8_linear(x, w)
+
+
+def test_scales_that_require_a_gradient_are_refused():
+    from torch.autograd import forward_ad
+    import sm120_moe_bench_b200 as vm
+    x, ids, wt = torch.randn(6, 32, generator=gen(111), device="cuda"), torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.ones(6, 2, device="cuda")
+    a, w = vm.quantize_int8(x), random_rows(vm, (8, 32), 112)
+    w13, w2 = random_rows(vm, (2, 32, 32), 114), random_rows(vm, (2, 32, 16), 116)
+
+    def calls(learn):
+        return (lambda: vm.int8_matmul(learn(a), w), lambda: vm.int8_matmul(a, learn(w)), lambda: vm.int8_linear(x, learn(w)),
+                lambda: vm.int8_experts(x, learn(w13), w2, ids, wt), lambda: vm.int8_experts(x, w13, learn(w2), ids, wt))
+
+    learnt = lambda r: vm.Int8Rows(r.q, torch.nn.Parameter(r.scale))
+    for call, plain in zip(calls(learnt), calls(lambda r: r)):
+        with pytest.raises(ValueError, match="scale requires a gradient"):
+            call()
+        with torch.no_grad():
+            assert torch.equal(call(), plain())
+    with forward_ad.dual_level():
+        for call in calls(lambda r: vm.Int8Rows(r.q, forward_ad.make_dual(r.scale, r.scale))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+    scale = torch.nn.Parameter(a.scale)
+    g, = torch.autograd.grad(vm.Int8Rows(a.q, scale).dequantize().sum(), scale)       # this is torch's own and has one
+    assert torch.equal(g, a.q.float().sum(1))
