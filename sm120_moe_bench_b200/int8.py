@@ -16,7 +16,7 @@ import torch
 from torch.autograd import forward_ad
 
 from ._lib import lib
-from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, check_out, check_rows, has_tangent, launch, refuse_overlap
+from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, changed, check_out, check_rows, has_tangent, launch, refuse_overlap
 
 MAX_K = 131071
 
@@ -172,6 +172,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
     launch(aq.device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, aq.data_ptr(), aq.stride(0), a.scale.data_ptr(), M, wq.data_ptr(),
            wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, E, None if plan is None else plan._offsets_ptr,
            swiglu, out is None, y.data_ptr(), max(y.stride(0), N), DTYPE_CODES[y.dtype], scratch.data_ptr() if need else None, need)
+    if out is not None:
+        changed(out)
     return y
 
 
@@ -183,7 +185,8 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
     check_rows(x, "x")
     N = _out_columns(w, x.shape[1], x.device, swiglu, None)
     stride = N
-    if out is None:
+    given = out is not None
+    if not given:
         out = x.new_empty((x.shape[0], N))
     else:
         stride = max(out.stride(0), N)
@@ -203,6 +206,8 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torc
     launch(x.device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, wq.data_ptr(),
            wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), stride, DTYPE_CODES[out.dtype],
            scratch.data_ptr() if need else None, need)
+    if given:
+        changed(out)
     return out
 
 

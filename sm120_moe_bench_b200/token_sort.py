@@ -54,6 +54,10 @@ def traced() -> bool:
     return get_proxy_mode() is not None
 
 
+# A tensor given as out is changed behind autograd's back: its version tells the graphs that saved it.
+changed = torch.autograd.graph.increment_version
+
+
 def launch(device: torch.device, name: str, fn, *args) -> None:
     """Call a C entry point on the device of its tensors, on that device's current stream."""
     if traced():
@@ -333,7 +337,9 @@ def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = Non
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
         refuse_overlap(check_out(out, plan.rows, x), plan, x=x)
-        return _sort(x, plan, out)
+        _sort(x, plan, out)
+        changed(out)
+        return out
     if x.requires_grad and torch.is_grad_enabled():
         return _SortTokens.apply(x, plan)
     return _sort(x, plan)
@@ -354,7 +360,9 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | N
         if grad or (torch.is_grad_enabled() and out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
         refuse_overlap(check_out(out, plan.tokens, rows), plan, rows=rows, weights=weights)
-        return _unsort(rows, plan, weights, out)
+        _unsort(rows, plan, weights, out)
+        changed(out)
+        return out
     if grad:
         return _UnsortTokens.apply(rows, plan, weights)
     return _unsort(rows, plan, weights)

@@ -497,3 +497,22 @@ def test_traces_are_refused():
     ga = torch.autograd.grad(torch.compile(step, backend="eager")(*a).sum(), a)
     gb = torch.autograd.grad(step(*b).sum(), b)
     assert all(torch.equal(p, r) for p, r in zip(ga, gb))
+
+
+def test_a_graph_that_saved_out_notices():
+    """Another graph holds the tensor that is overwritten: its backward pass must not use the new values."""
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 6, 2, 4, 32
+    plan = vm.plan_tokens(ids_of(M, T, E, 63), E)
+    x, rows, weights = rows_of(M, K, torch.float32, 64), rows_of(M * T, K, torch.float32, 65), torch.rand(M, T, device="cuda")
+    q, codes = vm.quantize_int8(rows_of(K, K, torch.float32, 66)), vm.quantize_int8(x)
+    for n, call in ((M * T, lambda out: vm.sort_tokens(x, plan, out=out)), (M, lambda out: vm.unsort_tokens(rows, plan, weights, out=out)),
+                    (M, lambda out: vm.int8_linear(x, q, out=out)), (M, lambda out: vm.int8_matmul(codes, q, out=out))):
+        gain, wide = torch.ones(n, K, device="cuda", requires_grad=True), torch.zeros(n + 2, K + 4, device="cuda")
+        for out in (torch.zeros(n, K, device="cuda"), wide[:n, 4:]):
+            y = (gain * out).sum()
+            assert call(out) is out
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+        with torch.inference_mode():                      # no versions there
+            call(torch.zeros(n, K, device="cuda"))
