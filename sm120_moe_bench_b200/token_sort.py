@@ -301,11 +301,12 @@ def _unsort_backward(ctx, grad):
     _refuse_tangent(grad)
     rows, weights = ctx.saved_tensors
     plan, grad = ctx.plan, _dense_rows(grad)
-    M, T, K = plan.tokens, plan.topk, rows.shape[1]
-    drows = rows.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
-    dw = torch.empty((M, T), dtype=torch.float32, device=rows.device) if ctx.needs_input_grad[2] else None
-    launch(rows.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0), rows.data_ptr(),
-           rows.stride(0), DTYPE_CODES[rows.dtype], M, T, plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
+    M, T, K = plan.tokens, plan.topk, grad.shape[1]
+    drows = grad.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
+    dw = torch.empty((M, T), dtype=torch.float32, device=grad.device) if ctx.needs_input_grad[2] else None
+    launch(grad.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0),
+           None if dw is None else rows.data_ptr(), 0 if dw is None else rows.stride(0), DTYPE_CODES[grad.dtype], M, T,
+           plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
            None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(), K,
            None if dw is None else dw.data_ptr())
     return drows, None, dw
@@ -319,7 +320,7 @@ class _UnsortTokens(torch.autograd.Function):
     def forward(ctx, rows, plan, weights):
         _note_graph(ctx, rows, weights)
         ctx.plan = plan
-        ctx.save_for_backward(rows, weights)
+        ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, weights)      # rows: the weights' gradient alone
         return _unsort(rows, plan, weights)
 
     @staticmethod

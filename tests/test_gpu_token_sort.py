@@ -516,3 +516,29 @@ def test_a_graph_that_saved_out_notices():
                 y.backward()
         with torch.inference_mode():                      # no versions there
             call(torch.zeros(n, K, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_are_kept_for_the_weights_gradient_alone(dtype):
+    import sm120_moe_bench_b200 as vm
+    M, T, E, K = 40, 3, 6, 72
+    plan = vm.plan_tokens(ids_of(M, T, E, 67), E)
+    rows, dy = rows_of(M * T, K, dtype, 68), rows_of(M, K, dtype, 69)
+    w = torch.rand(M, T, device="cuda")
+    for weights, kept in ((None, 0), (w, 1), (w.clone().requires_grad_(), 2)):
+        leaf = rows.clone().requires_grad_()
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: saved.append(t.shape) or t, lambda t: t):
+            y = vm.unsort_tokens(leaf, plan, weights)
+        assert saved == [rows.shape, w.shape][2 - kept:]
+        want, = torch.autograd.grad(y, leaf, dy)
+        # in between the rows may change
+        inner = leaf * 1
+        y = vm.unsort_tokens(inner, plan, weights)
+        inner.mul_(2)
+        if kept == 2:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                torch.autograd.grad(y, leaf, dy)
+        else:
+            # d inner = the rows' gradient; the product with 2 is later than y
+            assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want)
