@@ -374,10 +374,14 @@ int vmoe_int8_matmul(const int8_t* a, int64_t a_stride, const float* a_scale, in
                      int32_t swiglu, int32_t zero_tail, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,
                      size_t scratch_bytes, void* stream);
 
-/* x [M, K] (bf16 / fp16 / f32) quantised row by row, times w [N, K] (swiglu: [2 N, K]): one launch for a few rows (up to
- * four, up to eight of small weights), which needs no scratch; else two, the codes in `scratch` (16-byte aligned,
+/* x [M, K] (bf16 / fp16 / f32) quantised row by row, times w [N, K] (swiglu: [2 N, K]).  One launch where
+ * vmoe_int8_one_launch says so, which needs no scratch; else two, the codes in `scratch` (16-byte aligned,
  * vmoe_int8_linear_scratch_bytes).  vmoe_int8_pack_bytes(M, weight rows, K, 1) more let weights of any alignment be packed
- * in a third launch. */
+ * in a third launch.  Without scratch up to eight rows of 64 KB of codes (lengths rounded up to 16) take the one launch
+ * whatever the weights' size, more are refused (VMOE_ERR_WORKSPACE).
+ * vmoe_int8_one_launch: whether the dense product of M rows (quantised inside or codes) is best done in one launch.  align:
+ * a power of two that divides the weights' address and row stride in bytes.  1 = yes. */
+int vmoe_int8_one_launch(int32_t M, int32_t weight_rows, int32_t K, int32_t align);
 size_t vmoe_int8_linear_scratch_bytes(int32_t M, int32_t K);
 int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, const int8_t* w, int64_t w_stride, const float* w_scale,
                      int32_t N, int32_t K, int32_t swiglu, void* out, int64_t out_stride, int32_t out_dtype, void* scratch,

@@ -98,6 +98,7 @@ SIGNATURES = {
     "vmoe_int8_matmul": (C.c_int, [_P, C.c_int64, _P, C.c_int32, _P, C.c_int64, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P,
                                    C.c_int32, C.c_int32, _P, C.c_int64, C.c_int32, _P, C.c_size_t, _P]),
     "vmoe_int8_pack_bytes": (C.c_size_t, [C.c_int32] * 4),
+    "vmoe_int8_one_launch": (C.c_int, [C.c_int32] * 4),
     "vmoe_int8_linear_scratch_bytes": (C.c_size_t, [C.c_int32, C.c_int32]),
     "vmoe_int8_linear": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int32, C.c_int32, C.c_int32, _P, C.c_int64,
                                    C.c_int32, _P, C.c_size_t, _P]),

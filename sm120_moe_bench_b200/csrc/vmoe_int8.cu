@@ -374,7 +374,7 @@ static int i8_problem(I8Problem* p, const int8_t* a, long long a_stride, const f
 // 48 rows (16 items of 128 tokens) 8.6 against 14.8 us, 256 rows (32) 14.0 against 15.0, 512 rows (64) 18.0 against 15.5.
 static int i8_product(const I8Problem& p, cudaStream_t st) {
     if (i8_gemv_ok(p)) return launch_i8_gemv(p, nullptr, 0, 0, st);
-    if (!i8_tc_ok(p) || p.E > I8_TC_MAX_EXPERTS) return launch_i8_tile(p, st);
+    if (!i8_tc_ok(p) || p.E > I8_TC_MAX_EXPERTS) return i8_gemv_fits(p) ? launch_i8_gemv(p, nullptr, 0, 0, st) : launch_i8_tile(p, st);
     if (!p.offsets) {
         const long long items = (p.M + 127LL) / 128 * ((p.N + (p.swiglu ? 127LL : 255LL)) / (p.swiglu ? 128 : 256));
         if (items < 48) return launch_i8_split(p, st);
@@ -503,9 +503,10 @@ int vmoe_int8_linear(const void* x, int64_t x_stride, int32_t dtype, int32_t M, 
     const long long el = dtype == VMOE_F32 ? 4 : 2;
     if ((uintptr_t)x & (el - 1)) return VMOE_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (i8_gemv_ok(p)) return launch_i8_gemv(p, x, x_stride * el, dtype, st);
     const size_t need = vmoe_int8_linear_scratch_bytes(M, K);
-    if (!scratch || scratch_bytes < need) return VMOE_ERR_WORKSPACE;
+    const bool room = scratch && scratch_bytes >= need;
+    if (i8_gemv_ok(p) || (!room && i8_gemv_fits(p))) return launch_i8_gemv(p, x, x_stride * el, dtype, st);
+    if (!room) return VMOE_ERR_WORKSPACE;
     if ((uintptr_t)scratch & 15) return VMOE_ERR_ALIGN;
     int8_t* q = reinterpret_cast<int8_t*>(base);
     float* scale = reinterpret_cast<float*>(base + i8_align((size_t)M * pitch));

@@ -114,7 +114,8 @@ struct I8RowScale {
 
 // A few rows (vmoe_int8_gemv.cu): x, when not NULL, holds them as bf16 / fp16 / f32 and p.a is not read.
 constexpr int I8_GEMV_ROWS = 8;
-bool i8_gemv_ok(const I8Problem& p);
+bool i8_gemv_fits(const I8Problem& p);                   // it can take the product
+bool i8_gemv_ok(const I8Problem& p);                     // and is the better kernel for it
 int  launch_i8_gemv(const I8Problem& p, const void* x, long long x_stride_bytes, int x_dtype, cudaStream_t st);
 
 // tensor-core kernels (vmoe_int8_tc.cu)

@@ -230,13 +230,33 @@ i8_gemv_kernel(const I8Problem p, const uint8_t* x, long long x_stride, int x_dt
     }
 }
 
-// Measured against quantiser + tensor-core product (K = 4096, us): N = 2048, 1 / 4 / 8 rows 4.3 / 6.3 / 9.4 against 12;
-// N = 4096, 1 / 4 / 6 rows 6.4 / 9.0 / 11.9 against 10; N = 8192, 1 / 4 / 6 rows 9.3 / 13.2 / 17.2 against 12.8.  So up to four
-// rows, up to eight of weights of at most 8 MB; rows the tensor cores could only read after packing up to eight.
+// When this kernel is the better one, against quantiser + tensor-core product (weights that no copy can read: + packing).
+// A channel costs it 0.27 ns (1 row) to 0.5 (8 rows) however short it is, a KB of weights 0.14 ns (1 row, HBM speed), 0.17, 0.2
+// and 0.22 (4 rows), and the rows are quantised in every block; the others cost 3 to 5 us more to begin with.  us:
+//   K = 1024   8192 channels, 1 / 4 / 8 rows   5.4 / 6.8 / 8.8 against 9.3      16384, 1 / 2 / 4   7.8 / 8.5 / 10.0 against 9.0
+//              131072, 1 / 4   42 / 59 against 28 (K = 256: 37 / 53 against 12)
+//   K = 4096   8192, 1 / 3 / 4   8.9 / 11.4 / 12.5 against 13.0                 16384, 2 / 3 / 4   15.2 / 17.1 / 18.7 against 17.5
+//              32768, 1 / 2 / 3  24.4 / 26.1 / 29.4 against 26.8                131072, 1 / 2 / 4  83 / 92 / 112 against 87
+//   K = 8192   1024, 4 / 8       10.5 / 17.1 against 9.9                        8192, 1 / 2 / 3    14.6 / 16.6 / 20.1 against 18.9
+//   rows of words (K = 1000)     4096, 1 / 8   5.3 / 9.5 against 10.4           16384, 1 / 4 / 8   11.9 / 17.5 / 24 against 16.2
+//                 (K = 4088)     4096, 1 / 4 / 8   10.8 / 15.8 / 23.8 against 15.9
+//   of bytes (K = 1001)          1024, 1 / 4 / 8   6.1 / 9.2 / 12.5 against 8.4     4096, 1 / 8   13.5 / 21.1 against 11.2
+//            (K = 4095)          4096, 1 / 8       43 / 71 against 21
+// A call on its own takes 10 us of the host with one launch and 17 to 20 with two or three, so near a draw it is this one.
+static bool i8_few_rows(long long M, long long wrows, long long K, int align) {
+    const long long MB = 1 << 20, bytes = wrows * K;
+    if (align < 4) return bytes <= (M <= 4 ? 2 * MB : MB);
+    if (M > 4) return bytes <= 8 * MB && (align < 16 || (K <= 4096 && wrows <= 8192));
+    if (align < 16) return true;
+    if (K < 2048) return wrows <= (M <= 2 && K >= 1024 ? 16384 : 8192);
+    return M == 1 || bytes <= (M == 2 ? 128 * MB : M == 3 ? 32 * MB : 24 * MB);
+}
+static int i8_row_align(unsigned long long address_or_stride) { return address_or_stride % 16 == 0 ? 16 : address_or_stride % 4 == 0 ? 4 : 1; }
+static bool i8_gemv_takes(long long M, long long K) { return M <= I8_GEMV_ROWS && K > 0 && M * ((K + 15) & ~15LL) <= I8G_SMEM; }
+
+bool i8_gemv_fits(const I8Problem& p) { return p.E == 1 && !p.offsets && p.w_stride >= p.K && i8_gemv_takes(p.M, p.K); }
 bool i8_gemv_ok(const I8Problem& p) {
-    if (p.E != 1 || p.offsets || p.M > I8_GEMV_ROWS || p.K <= 0 || p.w_stride < p.K) return false;
-    if ((long long)p.M * ((p.K + 15) & ~15) > I8G_SMEM) return false;
-    return p.M <= 4 || (long long)p.wrows * p.K <= (8 << 20) || (((uintptr_t)p.w | (unsigned long long)p.w_stride) & 15) != 0;
+    return i8_gemv_fits(p) && i8_few_rows(p.M, p.wrows, p.K, i8_row_align((unsigned long long)(uintptr_t)p.w | (unsigned long long)p.w_stride));
 }
 
 template <int VB, int ROWS, bool SWIGLU>
@@ -269,3 +289,8 @@ int launch_i8_gemv(const I8Problem& p, const void* x, long long x_stride_bytes, 
 }
 
 }  // namespace vmoe
+
+extern "C" int vmoe_int8_one_launch(int32_t M, int32_t weight_rows, int32_t K, int32_t align) {
+    return M > 0 && weight_rows > 0 && align > 0 && vmoe::i8_gemv_takes(M, K) &&
+           vmoe::i8_few_rows(M, weight_rows, K, vmoe::i8_row_align((unsigned long long)align));
+}

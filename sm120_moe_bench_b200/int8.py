@@ -50,16 +50,12 @@ class Int8Rows:
         return self.q.float() * self.scale[..., None]
 
 
-def _no_grad(t: torch.Tensor, name: str) -> None:
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient: the 8-bit operators have none")
-    if has_tangent(t):
-        raise ValueError(f"{name} carries a forward-mode derivative: the 8-bit operators have none")
-
-
-def _no_grad_scales(rows: Int8Rows, name: str) -> None:
-    if rows.scale.requires_grad or forward_ad._current_level >= 0:
-        _no_grad(rows.scale, f"{name}.scale")
+def _no_grad(**tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient: the 8-bit operators have none")
+        if has_tangent(t):
+            raise ValueError(f"{name} carries a forward-mode derivative: the 8-bit operators have none")
 
 
 def _codes(rows: int, K: int, device) -> torch.Tensor:
@@ -87,7 +83,8 @@ def quantize_int8(x: torch.Tensor, plan: TokenPlan | None = None) -> Int8Rows:
 
     ``x`` is ``[rows, K]``, or ``[E, rows, K]`` contiguous for the weights of several experts.  With ``plan`` the rows of ``x``
     are tokens and the codes come sorted by expert, ``[M * T, K]`` (rows behind the last kept one are undefined)."""
-    _no_grad(x, "x")
+    if x.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(x=x)
     if x.dim() == 3:
         if plan is not None:
             raise ValueError("a plan sorts token rows [M, K]")
@@ -103,15 +100,24 @@ def quantize_int8(x: torch.Tensor, plan: TokenPlan | None = None) -> Int8Rows:
 
 
 def _aligned(q: torch.Tensor) -> bool:
-    """Whether the tensor cores can read these rows as they are."""
-    return (q.data_ptr() | q.stride(-2) | (q.stride(0) if q.dim() == 3 else 0)) % 16 == 0
+    """Whether the tensor cores can read these matrices as they are."""
+    return (q.data_ptr() | q.stride(1) | q.stride(0)) % 16 == 0
 
 
-def _packs(w: Int8Rows, rows: int) -> bool:
-    """Whether unaligned weights are worth a copy for a product with this many rows (figures at the C side's
-    ``i8_product_any``): not below one row per matrix, since the copy reads every matrix, nor for the few rows of a dense
-    product whose kernel reads weights at any alignment."""
-    return rows > 8 if w.q.dim() == 2 else rows >= w.q.shape[0]
+def _one_launch(rows: int, n: int, k: int, address: int, stride: int) -> bool:
+    """Whether a dense product of this many rows with weights ``[n, k]`` is done in one launch, without scratch."""
+    if rows > 8:
+        return False
+    odd = (address | stride) & 15
+    if rows <= 4 and n <= 8192 and 0 < k <= 8192 and stride >= k and n * k <= (1 << 21 if odd else 1 << 24):
+        return True                                       # the C side says so too; asking costs half a microsecond
+    return (n == 1 or stride >= k) and lib.vmoe_int8_one_launch(rows, n, k, 16 | odd) == 1
+
+
+def _packs(q: torch.Tensor, rows: int) -> bool:
+    """Whether unaligned matrices of several experts are worth a copy for a product with this many rows: not below one row per
+    matrix, since the copy reads every matrix."""
+    return rows >= q.shape[0]
 
 
 def int8_status(device: torch.device | str | int = "cuda") -> int:
@@ -145,32 +151,37 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
     """``out[m, n] = (a.q[m] . w.q[n]) * a.scale[m] * w.scale[n]``.
 
     With ``plan`` the rows are sorted by expert (``quantize_int8(x, plan)``) and each meets its expert's matrix of ``w``
-    ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``, which must not share memory with an operand).  ``swiglu``: ``w``
-    holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``, ``[M, N]``."""
-    _no_grad_scales(a, "a")
-    _no_grad_scales(w, "w")
-    if a.q.dim() != 2:
+    ``[E, N, K]``; rows behind the last kept one are zero (left as they were in a tensor given as ``out``, which must not share
+    memory with an operand).  ``swiglu``: ``w`` holds gate rows and up rows (``[2N, K]``) and the result is ``silu(gate) * up``,
+    ``[M, N]``."""
+    if a.scale.requires_grad or w.scale.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(**{"a.scale": a.scale, "w.scale": w.scale})
+    aq, wq = a.q, w.q
+    if aq.dim() != 2:
         raise ValueError("a must be rows [M, K]")
-    if plan is not None and (a.q.shape[0] != plan.rows or plan.device != a.q.device):
-        raise ValueError(f"the plan has {plan.rows} rows on {plan.device}, a {a.q.shape[0]} on {a.q.device}")
-    N = _out_columns(w, a.q.shape[1], a.q.device, swiglu, None if plan is None else plan.num_experts)
+    (M, K), device = aq.shape, aq.device
+    if plan is not None and (M != plan.rows or plan.device != device):
+        raise ValueError(f"the plan has {plan.rows} rows on {plan.device}, a {M} on {device}")
+    N = _out_columns(w, K, device, swiglu, None if plan is None else plan.num_experts)
     if out is None:
         if out_dtype not in DTYPE_CODES:
             raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-        y = torch.empty(a.q.shape[0], N, dtype=out_dtype, device=a.q.device)
+        y = torch.empty(M, N, dtype=out_dtype, device=device)
     else:
-        y = check_out(out, a.q.shape[0], out)
-        if out.device != a.q.device or out.shape[1] != N:
-            raise ValueError(f"out must have {N} columns on {a.q.device}")
-        _no_grad(out, "out")
-        refuse_overlap(out, plan, **{"a": a.q, "a's scales": a.scale, "w": w.q, "w's scales": w.scale})
-    M, K = a.q.shape
-    aq, wq = a.q, w.q
+        y = check_out(out, M, out)
+        if out.device != device or out.shape[1] != N:
+            raise ValueError(f"out must have {N} columns on {device}")
+        _no_grad(out=out)
+        refuse_overlap(out, plan, **{"a": aq, "a's scales": a.scale, "w": wq, "w's scales": w.scale})
     E = 1 if plan is None else plan.num_experts
-    need = 0 if (_aligned(aq) and _aligned(wq)) or not _packs(w, M) else lib.vmoe_int8_pack_bytes(M, wq.shape[-2], K, E)
-    scratch = torch.empty(need, dtype=torch.uint8, device=aq.device) if need else None
-    launch(aq.device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, aq.data_ptr(), aq.stride(0), a.scale.data_ptr(), M, wq.data_ptr(),
-           wq.stride(-2), 0 if plan is None else wq.stride(0), w.scale.data_ptr(), N, K, E, None if plan is None else plan._offsets_ptr,
+    need, channels, a_at, a_pitch, w_at, w_pitch = 0, 2 * N if swiglu else N, aq.data_ptr(), aq.stride(0), wq.data_ptr(), wq.stride(-2)
+    each = 0 if plan is None else wq.stride(0)
+    # unaligned operands are copied where that pays (figures at the C side's i8_product_any and i8_few_rows)
+    if (a_at | a_pitch | w_at | w_pitch | each) & 15 and (_packs(wq, M) if plan is not None else not _one_launch(M, channels, K, w_at, w_pitch)):
+        need = lib.vmoe_int8_pack_bytes(M, channels, K, E)
+    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    launch(device, "vmoe_int8_matmul", lib.vmoe_int8_matmul, a_at, a_pitch, a.scale.data_ptr(), M, w_at,
+           w_pitch, each, w.scale.data_ptr(), N, K, E, None if plan is None else plan._offsets_ptr,
            swiglu, out is None, y.data_ptr(), max(y.stride(0), N), DTYPE_CODES[y.dtype], scratch.data_ptr() if need else None, need)
     if out is not None:
         changed(out)
@@ -180,31 +191,30 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, plan: TokenPlan | None = None, *, swig
 def int8_linear(x: torch.Tensor, w: Int8Rows, *, swiglu: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """``x [M, K]`` (bf16 / fp16 / f32) quantised row by row, times ``w [N, K]``: ``[M, N]`` in the type of ``x``.
     ``out`` must not share memory with ``x`` or ``w``."""
-    _no_grad(x, "x")
-    _no_grad_scales(w, "w")
+    if x.requires_grad or w.scale.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(**{"x": x, "w.scale": w.scale})
     check_rows(x, "x")
-    N = _out_columns(w, x.shape[1], x.device, swiglu, None)
+    (M, K), device, wq = x.shape, x.device, w.q
+    N = _out_columns(w, K, device, swiglu, None)
     stride = N
     given = out is not None
     if not given:
-        out = x.new_empty((x.shape[0], N))
+        out = x.new_empty((M, N))
     else:
         stride = max(out.stride(0), N)
-        check_rows(out, "out", x.shape[0], x.device)
-        if out.dtype != x.dtype or out.shape[1] != N or (x.shape[0] > 1 and out.stride(0) < N):
+        check_rows(out, "out", M, device)
+        if out.dtype != x.dtype or out.shape[1] != N or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be {x.dtype} with {N} columns and rows that do not overlap")
-        _no_grad(out, "out")
-        refuse_overlap(out, x=x, **{"w": w.q, "w's scales": w.scale})
-    M, K = x.shape
-    wq = w.q
-    need = 0
-    if M > 4 or not 0 < K <= 8192 or wq.stride(0) < K:    # else the rows are quantised inside the product
+        _no_grad(out=out)
+        refuse_overlap(out, x=x, **{"w": wq, "w's scales": w.scale})
+    need, address, pitch, channels = 0, wq.data_ptr(), wq.stride(0), 2 * N if swiglu else N
+    if not _one_launch(M, channels, K, address, pitch):   # else the rows are quantised inside the product
         need = lib.vmoe_int8_linear_scratch_bytes(M, K)
-        if not _aligned(wq) and _packs(w, M):
-            need += lib.vmoe_int8_pack_bytes(M, wq.shape[0], K, 1)
-    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    launch(x.device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, wq.data_ptr(),
-           wq.stride(0), w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), stride, DTYPE_CODES[out.dtype],
+        if (address | pitch) & 15:
+            need += lib.vmoe_int8_pack_bytes(M, channels, K, 1)
+    scratch = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    launch(device, "vmoe_int8_linear", lib.vmoe_int8_linear, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], M, address,
+           pitch, w.scale.data_ptr(), N, K, swiglu, out.data_ptr(), stride, DTYPE_CODES[out.dtype],
            scratch.data_ptr() if need else None, need)
     if given:
         changed(out)
@@ -218,10 +228,8 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
     ``x [M, K]`` bf16 / fp16 / f32; ``w13 [E, 2N, K]`` (gate rows first); ``w2 [E, K, N]``; ids int32 and weights f32 ``[M, T]``.
     Tokens are quantised once and copied into expert order, the activations between the two products once more per row;
     everything between is f32, and the sum is rounded once to the type of ``x``.  ``expert_map`` as in ``plan_tokens``."""
-    _no_grad(x, "x")
-    _no_grad(topk_weights, "topk_weights")
-    _no_grad_scales(w13, "w13")
-    _no_grad_scales(w2, "w2")
+    if x.requires_grad or topk_weights.requires_grad or w13.scale.requires_grad or w2.scale.requires_grad or forward_ad._current_level >= 0:
+        _no_grad(**{"x": x, "topk_weights": topk_weights, "w13.scale": w13.scale, "w2.scale": w2.scale})
     if topk_ids.dim() != 2:
         raise ValueError("topk_ids must be an int32 tensor [tokens, choices]")
     check_rows(x, "x", topk_ids.shape[0], topk_ids.device)
@@ -243,7 +251,7 @@ def int8_experts(x: torch.Tensor, w13: Int8Rows, w2: Int8Rows, topk_ids: torch.T
                                    or not expert_map.is_contiguous() or expert_map.numel() == 0):
         raise ValueError("expert_map must be a contiguous int32 vector on the device of topk_ids, not empty")
     q13, q2 = w13.q, w2.q
-    pack = not (_aligned(q13) and _aligned(q2)) and _packs(w13, M * T)
+    pack = not (_aligned(q13) and _aligned(q2)) and _packs(q13, M * T)
     out = x.new_empty((M, K))
     need = lib.vmoe_int8_experts_scratch_bytes(M, T, E, K, N, pack)
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device)

@@ -46,12 +46,8 @@ _tracing, _dispatch_modes, _function_modes = torch._C._is_tracing, torch._C._len
 def traced() -> bool:
     """Whether torch.jit.trace or make_fx records what runs now.  They see torch's own operators, not a kernel launched
     beside them: the recorded program would hold the allocations and return them as they are."""
-    if _tracing():
-        return True
-    if not (_dispatch_modes() or _function_modes()):      # make_fx pushes one of either kind (0.2 us so far)
-        return False
     from torch.fx.experimental.proxy_tensor import get_proxy_mode
-    return get_proxy_mode() is not None
+    return _tracing() or get_proxy_mode() is not None
 
 
 # A tensor given as out is changed behind autograd's back: its version tells the graphs that saved it.
@@ -60,7 +56,8 @@ changed = torch.autograd.graph.increment_version
 
 def launch(device: torch.device, name: str, fn, *args) -> None:
     """Call a C entry point on the device of its tensors, on that device's current stream."""
-    if traced():
+    # (make_fx pushes a mode of either kind; looking for them takes 0.15 us)
+    if _tracing() or ((_dispatch_modes() or _function_modes()) and traced()):
         raise RuntimeError(f"{name}: a kernel of this library cannot be traced (its launch would be missing from the recorded program)")
     index = device.index
     if index == _current_device():
@@ -241,7 +238,7 @@ def plan_tokens(topk_ids: torch.Tensor, num_experts: int, expert_map: torch.Tens
 def _sort(x, plan: TokenPlan, out=None):
     K = x.shape[1]
     rows, stride = (x.new_empty((plan.rows, K)), K) if out is None else (out, max(out.stride(0), K))
-    launch(x.device, "vmoe_sort_tokens", lib.vmoe_sort_tokens, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], plan.tokens, plan.topk,
+    launch(plan.device, "vmoe_sort_tokens", lib.vmoe_sort_tokens, x.data_ptr(), x.stride(0), DTYPE_CODES[x.dtype], plan.tokens, plan.topk,
            plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr, out is None, rows.data_ptr(),
            stride)
     return rows
@@ -250,9 +247,9 @@ def _sort(x, plan: TokenPlan, out=None):
 def _unsort(rows, plan: TokenPlan, weights=None, out=None):
     K = rows.shape[1]
     y, stride = (rows.new_empty((plan.tokens, K)), K) if out is None else (out, max(out.stride(0), K))
-    launch(rows.device, "vmoe_unsort_tokens", lib.vmoe_unsort_tokens, rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype],
+    launch(plan.device, "vmoe_unsort_tokens", lib.vmoe_unsort_tokens, rows.data_ptr(), rows.stride(0), DTYPE_CODES[rows.dtype],
            plan.tokens, plan.topk, K, plan._rows_ptr, None if weights is None else weights.data_ptr(), y.data_ptr(),
-           stride, DTYPE_CODES[y.dtype])
+           stride, DTYPE_CODES[rows.dtype])
     return y
 
 
@@ -333,7 +330,8 @@ def sort_tokens(x: torch.Tensor, plan: TokenPlan, out: torch.Tensor | None = Non
     """``rows[r] = x[token of row r]``: the token rows ``[M, K]`` in expert order, ``[M * T, K]``.  Differentiable in ``x``
     (a token's gradient is the sum over its rows) unless ``out`` is given."""
     check_rows(x, "x", plan.tokens, plan.device)
-    _refuse_tangent(x, out)
+    if forward_ad._current_level >= 0:
+        _refuse_tangent(x, out)
     if out is not None:
         if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
             raise ValueError("out cannot be given where a gradient is wanted")
@@ -350,9 +348,10 @@ def unsort_tokens(rows: torch.Tensor, plan: TokenPlan, weights: torch.Tensor | N
     """``out[m] = sum_t weights[m, t] * rows[row of (m, t)]``: rows ``[M * T, K]`` in expert order back to tokens ``[M, K]``.
     ``weights`` f32 ``[M, T]`` (None = 1).  Differentiable in ``rows`` and ``weights`` unless ``out`` is given."""
     check_rows(rows, "rows", plan.rows, plan.device)
-    _refuse_tangent(rows, weights, out)
+    if forward_ad._current_level >= 0:
+        _refuse_tangent(rows, weights, out)
     if weights is not None:
-        if weights.device != rows.device or weights.dtype != torch.float32 or tuple(weights.shape) != (plan.tokens, plan.topk):
+        if weights.device != rows.device or weights.dtype != torch.float32 or weights.shape != (plan.tokens, plan.topk):
             raise ValueError(f"weights must be a float32 tensor [{plan.tokens}, {plan.topk}] on the device of rows")
         if not weights.is_contiguous():
             raise ValueError("weights must be contiguous")

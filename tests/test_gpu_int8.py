@@ -592,3 +592,25 @@ def test_scales_that_require_a_gradient_are_refused():
     scale = torch.nn.Parameter(a.scale)
     g, = torch.autograd.grad(vm.Int8Rows(a.q, scale).dequantize().sum(), scale)       # this is torch's own and has one
     assert torch.equal(g, a.q.float().sum(1))
+
+
+@pytest.mark.parametrize("K,N", [(256, 8192), (256, 8200), (1024, 16384), (1024, 16392), (4096, 2048), (4096, 2056), (4096, 6144), (4096, 6152), (8192, 24),
+                                 (1001, 1047), (1001, 1048), (1001, 2095), (1001, 2096), (1000, 8388), (1000, 8390), (4095, 300), (9001, 64), (16392, 32)])
+def test_both_sides_of_the_few_row_rule(K, N):
+    """Where one launch does it all, where quantiser and product are two, where unaligned weights are packed: the same bits."""
+    import sm120_moe_bench_b200 as vm
+    from sm120_moe_bench_b200._lib import lib
+    x, w = torch.randn(9, K, generator=gen(118), device="cuda").bfloat16(), random_rows(vm, (N, K), 119)
+    a = vm.quantize_int8(x)
+    pairs = vm.Int8Rows(w.q[:N // 2 * 2], w.scale[:N // 2 * 2])
+    want, gated = vm.int8_linear(x, w), vm.int8_linear(x, pairs, swiglu=True)
+    check_product(want, exact_product(a, w))
+    for M in range(1, 9):
+        part = vm.Int8Rows(a.q[:M], a.scale[:M])
+        assert torch.equal(vm.int8_linear(x[:M], w), want[:M]) and torch.equal(vm.int8_matmul(part, w), want[:M])
+        assert torch.equal(vm.int8_linear(x[:M], pairs, swiglu=True), gated[:M])
+        if M * ((K + 15) // 16 * 16) <= 65536:            # from C without scratch
+            out = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+            assert lib.vmoe_int8_linear(x.data_ptr(), K, 0, M, w.q.data_ptr(), K, w.scale.data_ptr(), N, K, 0, out.data_ptr(), N, 0, None, 0,
+                                        torch.cuda.current_stream().cuda_stream) == 0
+            assert torch.equal(out, want[:M])

@@ -96,3 +96,32 @@ def test_wait_limit_checks():
     lib = _lib()
     assert lib.vmoe_int8_set_wait_limit(-1) == 2
     assert lib.vmoe_int8_set_wait_limit(10 ** 6) == 0     # what it is from the start
+
+
+def test_few_rows_rule():
+    one = _lib().vmoe_int8_one_launch
+    assert one(0, 64, 64, 16) == 0 and one(1, 0, 64, 16) == 0 and one(1, 64, 0, 16) == 0 and one(1, 64, 64, 0) == 0 and one(9, 64, 64, 16) == 0
+    # the codes have to fit 64 KB, whatever the alignment
+    for align in (16, 4, 1):
+        assert one(8, 16, 8192, align) == (align < 16) and one(8, 16, 8193, align) == 0 and one(4, 16, 16385, align) == 0 and one(1, 16, 65537, align) == 0
+    # a row more, or a channel more, never makes it the better kernel
+    for align in (16, 4, 1):
+        for K in (16, 256, 1024, 2048, 4096, 8192):
+            for N in (8, 512, 4096, 8192, 16384, 32768, 131072):
+                got = [one(M, N, K, align) for M in range(1, 9)]
+                assert got == sorted(got, reverse=True)
+                assert all(one(M, 2 * N, K, align) <= got[M - 1] for M in range(1, 9))
+    assert [one(M, 131072, 1024, 16) for M in (1, 2, 4, 8)] == [0, 0, 0, 0] and one(1, 131072, 4096, 16) == 1 and one(4, 131072, 4096, 16) == 0
+    assert [one(M, 2048, 4096, 16) for M in (1, 2, 4, 8)] == [1, 1, 1, 1] and one(1, 4096, 4095, 1) == 0 and one(4, 64, 128, 1) == 1
+
+
+def test_python_agrees_with_the_few_row_rule():
+    from sm120_moe_bench_b200.int8 import _one_launch
+    one = _lib().vmoe_int8_one_launch
+    for M in range(0, 11):
+        for K in (0, 1, 15, 16, 255, 1000, 1024, 2047, 2048, 4095, 4096, 8191, 8192, 8193, 16384, 65537):
+            for n in (1, 2, 60, 255, 256, 257, 1024, 2048, 4096, 8192, 8193, 16384, 131072):
+                for address, pitch in ((512, (K + 15) // 16 * 16), (512, K), (516, K + 4 - K % 4), (513, K)):
+                    want = one(M, n, K, 16 | (address | pitch) & 15)
+                    assert _one_launch(M, n, K, address, max(pitch, 1)) == bool(want) or M == 0, (M, n, K, address, pitch)
+    assert not _one_launch(2, 64, 64, 512, 32) and _one_launch(2, 1, 64, 512, 1)       # rows that overlap; one row has no pitch
