@@ -614,3 +614,40 @@ def test_both_sides_of_the_few_row_rule(K, N):
             assert lib.vmoe_int8_linear(x.data_ptr(), K, 0, M, w.q.data_ptr(), K, w.scale.data_ptr(), N, K, 0, out.data_ptr(), N, 0, None, 0,
                                         torch.cuda.current_stream().cuda_stream) == 0
             assert torch.equal(out, want[:M])
+
+
+def silu_points():
+    inf = float("inf")
+    at = [0.0, -0.0, 2.0 ** -149, -2.0 ** -149, 1e-40, 2.0 ** -126, 1e-30, -1e-30, 2.0 ** -24, -2.0 ** -12, 0.5, 1.0, -1.0, 8.0, -8.0, 16.0, -16.0, 16.635,
+          20.0, -20.0, -87.0, -87.3, -87.33, -87.3365, -87.337, -87.5, -88.0, -88.72, -88.73, -89.0, -103.0, -104.0, -1000.0, 88.0, 1000.0, 3.4e38, -3.4e38]
+    c = torch.tensor(at, device="cuda")
+    near = [c]
+    for way in (inf, -inf):
+        n = c
+        for _ in range(3):
+            n = torch.nextafter(n, torch.full_like(n, way))
+            near.append(n)
+    g = gen(120)
+    return torch.cat(near + [torch.linspace(-110, 110, 100001, device="cuda"), torch.linspace(-4, 4, 20001, device="cuda"),
+                             20 * torch.randn(40000, generator=g, device="cuda"), torch.exp(20 * torch.randn(20000, generator=g, device="cuda")),
+                             -torch.exp(6 * torch.randn(20000, generator=g, device="cuda"))])
+
+
+@pytest.mark.parametrize("M", [1, 8, 9, 40])
+def test_silu_over_its_range(M):
+    """A code of 1 times a channel's scale is any gate, times an up of 1: the result is the silu itself, of each kernel.  It may be
+    off by 6 * 2^-24 (expf 4, the sum and the quotient half a step each) and 2^-40 for products of those; half a step among
+    the subnormals; and is flushed to 0 below -87.33, where silu is above -1.04e-36."""
+    import sm120_moe_bench_b200 as vm
+    x = silu_points()
+    n = x.numel()
+    a = vm.Int8Rows(torch.ones(M, 1, dtype=torch.int8, device="cuda"), torch.ones(M, device="cuda"))
+    w = vm.Int8Rows(torch.ones(2 * n, 1, dtype=torch.int8, device="cuda"), torch.cat([x, torch.ones(n, device="cuda")]))
+    y = vm.int8_matmul(a, w, swiglu=True, out_dtype=torch.float32)
+    assert torch.equal(y, y[:1].expand(M, n))
+    want = silu64(x.double())
+    tol = (6 * 2.0 ** -24 + 2.0 ** -40) * want.abs() + 2.0 ** -150 + torch.where(x < -87.33, 1.04e-36, 0.0).double()
+    assert bool(((y[0].double() - want).abs() <= tol).all())
+    ends = vm.Int8Rows(torch.ones(8, 1, dtype=torch.int8, device="cuda"), torch.tensor([float("inf"), float("-inf"), float("nan"), 1.0, 1, 1, 1, 1], device="cuda"))
+    y = vm.int8_matmul(a, ends, swiglu=True, out_dtype=torch.float32)
+    assert bool((y[:, 0] == float("inf")).all()) and bool(y[:, 1:3].isnan().all()) and bool(y[:, 3].isfinite().all())
