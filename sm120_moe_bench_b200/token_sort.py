@@ -258,6 +258,7 @@ def _dense_rows(g: torch.Tensor) -> torch.Tensor:
     return g if g.shape[1] <= 1 or g.stride(1) == 1 else g.contiguous()
 
 
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 _eager_graphs = weakref.WeakSet()      # nodes of live eager graphs; each knows its leaves (weakly)
 _eager_lock = threading.Lock()
 
@@ -267,7 +268,7 @@ def _note_graph(ctx, *tensors: torch.Tensor | None) -> None:
     leaves = [weakref.ref(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     if not leaves:
         return
-    if not torch.cuda.is_current_stream_capturing():
+    if not _capturing():
         ctx.leaves = leaves
         with _eager_lock:
             _eager_graphs.add(ctx)
@@ -288,20 +289,23 @@ class _SortTokens(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad):
-        _refuse_tangent(grad)
+        if forward_ad._current_level >= 0:
+            _refuse_tangent(grad)
         grad = _dense_rows(grad)
         # with create_graph the gradient is differentiable itself
         return (unsort_tokens if torch.is_grad_enabled() else _unsort)(grad, ctx.plan), None
 
 
 def _unsort_backward(ctx, grad):
-    _refuse_tangent(grad)
+    if forward_ad._current_level >= 0:
+        _refuse_tangent(grad)
     rows, weights = ctx.saved_tensors
+    want_rows, _, want_weights = ctx.needs_input_grad
     plan, grad = ctx.plan, _dense_rows(grad)
     M, T, K = plan.tokens, plan.topk, grad.shape[1]
-    drows = grad.new_empty((plan.rows, K)) if ctx.needs_input_grad[0] else None
-    dw = torch.empty((M, T), dtype=torch.float32, device=grad.device) if ctx.needs_input_grad[2] else None
-    launch(grad.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0),
+    drows = grad.new_empty((plan.rows, K)) if want_rows else None
+    dw = torch.empty((M, T), dtype=torch.float32, device=plan.device) if want_weights else None
+    launch(plan.device, "vmoe_unsort_tokens_grad", lib.vmoe_unsort_tokens_grad, grad.data_ptr(), grad.stride(0),
            None if dw is None else rows.data_ptr(), 0 if dw is None else rows.stride(0), DTYPE_CODES[grad.dtype], M, T,
            plan.num_experts, K, plan._offsets_ptr, plan._rows_ptr,
            None if weights is None else weights.data_ptr(), None if drows is None else drows.data_ptr(), K,
