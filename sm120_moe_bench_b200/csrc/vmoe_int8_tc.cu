@@ -664,8 +664,11 @@ extern "C" int vmoe_int8_read_status(void* stream) {
     int v = 0;
     const int zero = 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (cudaMemcpyFromSymbolAsync(&v, vmoe::g_i8_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return VMOE_ERR_CUDA;
-    if (cudaStreamSynchronize(st) != cudaSuccess) return VMOE_ERR_CUDA;
+    if (cudaMemcpyFromSymbolAsync(&v, vmoe::g_i8_status, sizeof(v), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+        cudaStreamSynchronize(st) != cudaSuccess) {
+        cudaGetLastError();                               // not left for the next launch's check
+        return VMOE_ERR_CUDA;
+    }
     if (v != 0) cudaMemcpyToSymbolAsync(vmoe::g_i8_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
     return v;
 }

@@ -15,10 +15,11 @@ from __future__ import annotations
 import torch
 from torch.autograd import forward_ad
 
-from ._lib import lib
+from ._lib import check, lib
 from .token_sort import DTYPE_CODES, MAX_EXPERTS, MAX_ROWS, MAX_TOPK, TokenPlan, changed, check_out, check_rows, has_tangent, launch, refuse_overlap
 
 MAX_K = 131071
+TIMEOUT = 6               # VMOE_ERR_TIMEOUT
 
 
 class Int8Rows:
@@ -122,9 +123,14 @@ def _packs(q: torch.Tensor, rows: int) -> bool:
 
 def int8_status(device: torch.device | str | int = "cuda") -> int:
     """0, or the status of a bounded wait that ran out inside an 8-bit product on this device since the last call (6 = time-out,
-    as ``Workspace.status``).  Waits for the current stream."""
+    as ``Workspace.status``).  Waits for the current stream, so not while it is captured."""
     with torch.cuda.device(device):
-        return lib.vmoe_int8_read_status(torch.cuda.current_stream().cuda_stream)
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("int8_status waits for the stream, which a capture does not allow")
+        status = lib.vmoe_int8_read_status(torch.cuda.current_stream().cuda_stream)
+    if status not in (0, TIMEOUT):
+        check(status, "vmoe_int8_read_status")
+    return status
 
 
 def _out_columns(w: Int8Rows, K: int, device, swiglu: bool, experts: int | None) -> int:

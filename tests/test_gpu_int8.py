@@ -651,3 +651,16 @@ def test_silu_over_its_range(M):
     ends = vm.Int8Rows(torch.ones(8, 1, dtype=torch.int8, device="cuda"), torch.tensor([float("inf"), float("-inf"), float("nan"), 1.0, 1, 1, 1, 1], device="cuda"))
     y = vm.int8_matmul(a, ends, swiglu=True, out_dtype=torch.float32)
     assert bool((y[:, 0] == float("inf")).all()) and bool(y[:, 1:3].isnan().all()) and bool(y[:, 3].isfinite().all())
+
+
+def test_status_while_capturing_is_refused():
+    import sm120_moe_bench_b200 as vm
+    x, w = torch.randn(40, 64, generator=gen(121), device="cuda"), random_rows(vm, (64, 64), 122)
+    want = vm.int8_linear(x, w)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(RuntimeError, match="capture"):
+            vm.int8_status()
+        y = vm.int8_linear(x, w)                          # the capture goes on
+    g.replay()
+    assert torch.equal(y, want) and vm.int8_status() == 0
