@@ -6,7 +6,8 @@ namespace vmoe {
 // ---------------------------------------------------------------------------------
 // Rows to codes (the arithmetic: I8RowScale).  WPR warps per row, eight per CTA; a thread keeps up to eight vectors of the
 // row in registers, so that rows of up to 8 * 32 * WPR vectors are read once.  With row_of_pair a row is a token and its
-// codes go to the token's T sorted rows.
+// codes go to the token's T sorted rows.  8192 x 4096 bf16: 21 us (4.8 TB/s; at a copy's rate 15.4): four CTAs an SM leave 64
+// registers, and the 16-byte instances for 16-bit rows spill up to 36 bytes a thread.
 // ---------------------------------------------------------------------------------
 constexpr int I8_KEPT = 8;
 
@@ -371,7 +372,9 @@ static int i8_problem(I8Problem* p, const int8_t* a, long long a_stride, const f
 }
 
 // The kernel of a product, by its sizes and the alignment of its operands.  Dense, split against persistent, K = N = 4096:
-// 48 rows (16 items of 128 tokens) 8.6 against 14.8 us, 256 rows (32) 14.0 against 15.0, 512 rows (64) 18.0 against 15.5.
+// 48 rows (16 items of 128 tokens) 8.8 against 14.4 us, 256 rows (32) 14.7 against 14.6, 384 rows (48) 18.6 against 14.8.  Longer
+// reductions gain more by the split (1024 channels of 8192, 48 rows: 8.4 against 23.8), shorter ones lose (2048 x 2048: 11.8 against
+// 9.2; 8192 channels of 1024: 8.6 against 7.2), which the rule does not look at.
 static int i8_product(const I8Problem& p, cudaStream_t st) {
     if (i8_gemv_ok(p)) return launch_i8_gemv(p, nullptr, 0, 0, st);
     if (!i8_tc_ok(p) || p.E > I8_TC_MAX_EXPERTS) return i8_gemv_fits(p) ? launch_i8_gemv(p, nullptr, 0, 0, st) : launch_i8_tile(p, st);

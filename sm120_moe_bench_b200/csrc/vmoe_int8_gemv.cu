@@ -1,11 +1,13 @@
 // The 8-bit product for a few rows (decode of one to eight tokens), in one launch: the rows are quantised inside.  One token,
-// N = 2048, K = 4096: 4.3 us (8.4 MB of weights: 2 TB/s, a launch alone is 2 us); N = 8192: 9.3 us (3.6 TB/s).
+// N = 2048, K = 4096: 4.5 us (8.4 MB of weights: 1.9 TB/s, a launch alone is 2 us); N = 8192: 8.9 us (3.8 TB/s); N = 131072:
+// 83 us (6.5 TB/s).
 //
 // Bound by reading the weights once, and at these sizes by latency: a warp requests the first 4 KB of its first channel
 // (with swiglu of its gate and up rows) before anything else and quantises the rows -- every CTA for itself, 8 KB from L2
 // -- while they are on their way; from then on each vector it uses is replaced at once by the one that comes next, of the
 // same channel or of the warp's next one.  Codes lie in shared memory; four products per dp4a, integer sums joined by
-// one warp reduction, so the result is the other kernels' bit for bit.
+// one warp reduction, so the result is the other kernels' bit for bit.  With swiglu two channels' vectors are under way and
+// 192 to 232 bytes a thread spill at 128 registers (two CTAs an SM); its 8192 rows of weights take 8.2 us.
 #include "vmoe_int8.cuh"
 #include "vmoe_tc_common.cuh"
 
