@@ -17,8 +17,8 @@ constexpr int I8G_THREADS = 256;
 constexpr int I8G_SMEM = 64 * 1024;                       // codes of all rows
 
 // VB = 16: the weights' rows start on 16-byte boundaries; the bytes behind a row's last whole vector go to a lane each, so that
-// nothing behind the row is read.  VB = 4: anywhere; a word is joined from the two aligned ones that hold it, the second of
-// which is read only where the row reaches into it.
+// nothing behind the row is read.  VB = 4: anywhere; a word is joined from the two aligned ones that hold it.  Only aligned words
+// with a byte of the row in them are read, so a row's first and last may bring up to three bytes beside it.
 template <int VB> struct I8Word;
 template <> struct I8Word<16> { using type = uint4; };
 template <> struct I8Word<4>  { using type = uint32_t; };
